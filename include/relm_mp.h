@@ -51,7 +51,9 @@ enum relm_mp_status {
     RELM_MP_ERR_HIP = 5        /* HIP runtime / launch error */
 };
 
-enum relm_mp_dtype { RELM_MP_F32 = 0, RELM_MP_F64 = 1 };
+/* The message-passing ops take F32 and F64, the readout ops (at the end) F32, BF16
+ * and F16. */
+enum relm_mp_dtype { RELM_MP_F32 = 0, RELM_MP_F64 = 1, RELM_MP_BF16 = 2, RELM_MP_F16 = 3 };
 
 enum relm_mp_mode { RELM_MP_MODE_SUM = 0, RELM_MP_MODE_LOGSUMEXP = 1 };
 
@@ -514,6 +516,31 @@ int relm_mp_film_mish_backward_sums(const float* s, const float* dy, int64_t row
                                     const float* gamma, const float* beta, const float* add,
                                     float* ds, float* sums, void* workspace, size_t workspace_bytes,
                                     relm_mp_stream_t stream);
+
+/* ---- readout ops (no counterpart in the reference) --------------------------
+ * What a program runs on the object states that the message passing leaves:
+ * the norm of a residual stream, cross attention of per-graph queries to the
+ * objects, and the orthogonalised update of the weights that they train.
+ * dtype: RELM_MP_F32, RELM_MP_BF16 or RELM_MP_F16; sums and statistics are float.
+ * None of these calls synchronises or allocates. */
+
+/* Root-mean-square norm with the residual's addition over rows [rows, width]:
+ * h = x + r, y = h / sqrt(mean(h^2) + eps) * w.  r may be NULL (h = x); h may be NULL
+ * (not kept), else it receives the sum rounded to dtype; rstd may be NULL, else [rows]
+ * floats 1 / sqrt(mean + eps) for the backward.  No output overlaps an input. */
+int relm_mp_add_rms_norm(int dtype, const void* x, const void* r, const void* w, int64_t rows, int64_t width,
+                         float eps, void* y, void* h, float* rstd, relm_mp_stream_t stream);
+/* The same with y in 8 bits for serving: q [rows, width] e4m3 bytes, scale [rows] floats
+ * = max|y| / 448 of the row (1 for a row of zeros): y ~ q * scale. */
+int relm_mp_add_rms_norm_fp8(int dtype, const void* x, const void* r, const void* w, int64_t rows, int64_t width,
+                             float eps, void* q, float* scale, void* h, relm_mp_stream_t stream);
+/* Backward: dx [rows, width] (the gradient of x and of r alike) and dw [width] from dy
+ * and dh (may be NULL: zero), the gradients of y and h, and the forward's h and rstd.
+ * dw is added in a fixed order.  workspace: *_workspace_size bytes, 16-byte aligned. */
+size_t relm_mp_add_rms_norm_backward_workspace_size(int dtype, int64_t rows, int64_t width);
+int relm_mp_add_rms_norm_backward(int dtype, const void* dy, const void* dh, const void* h, const void* w,
+                                  const float* rstd, int64_t rows, int64_t width, void* dx, void* dw,
+                                  void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
 
 #ifdef __cplusplus
 }

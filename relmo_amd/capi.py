@@ -25,6 +25,8 @@ ERR_HIP = 5
 
 F32 = 0
 F64 = 1
+BF16 = 2
+F16 = 3
 PLAN_INVERSE = 1
 PLAN_CSR = 2
 PLAN_SNAPSHOT = 1  # inverse-plan build flag: keep a snapshot of the indices
@@ -71,6 +73,10 @@ EXPORTED_SYMBOLS = (
     "relm_mp_film_mish_backward",
     "relm_mp_film_mish_backward_sums_workspace_size",
     "relm_mp_film_mish_backward_sums",
+    "relm_mp_add_rms_norm",
+    "relm_mp_add_rms_norm_fp8",
+    "relm_mp_add_rms_norm_backward_workspace_size",
+    "relm_mp_add_rms_norm_backward",
 )
 
 
@@ -188,6 +194,13 @@ _SIGNATURES = {
     "relm_mp_film_mish_backward_sums_workspace_size": (_sz, [_vp, ctypes.c_int32, _i64]),
     "relm_mp_film_mish_backward_sums": (
         _int, [_vp, _vp, _i64, _i64, _vp, ctypes.c_int32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "relm_mp_add_rms_norm": (
+        _int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "relm_mp_add_rms_norm_fp8": (
+        _int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "relm_mp_add_rms_norm_backward_workspace_size": (_sz, [_int, _i64, _i64]),
+    "relm_mp_add_rms_norm_backward": (
+        _int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
     "relm_mp_plan_match": (
         _int,
         [_vp, _vp, _i64, ctypes.POINTER(_PP), ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), _vp,

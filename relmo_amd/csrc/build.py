@@ -26,8 +26,9 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = os.environ.get("RELM_MP_OFFLOAD_ARCH", "gfx950")
 
 HIP_SOURCES = ["plan_kernels.hip", "small_plan_kernels.hip", "reduce_kernels.hip", "pack_kernels.hip", "match_kernels.hip",
-               "film_kernels.hip",
-               "capi.hip"]
+               "film_kernels.hip", "norm_kernels.hip",
+               "capi.hip", "capi_readout.hip"]
+TORCH_SOURCES = ["relm_mp_ops.cpp", "readout_ops.cpp"]
 HIP_LIB = PKG_DIR / "librelm_mp_hip.so"
 TORCH_EXT = PKG_DIR / "relm_mp_ops.so"
 
@@ -100,7 +101,7 @@ def build_torch_ext(verbose: bool = False) -> Path:
         f"-I{tdir / 'include'}",
         f"-I{tdir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
         f"-I{ROCM / 'include'}",
-        str(CSRC / "relm_mp_ops.cpp"),
+        *(str(CSRC / src) for src in TORCH_SOURCES),
         f"-L{PKG_DIR}",
         "-lrelm_mp_hip",
         f"-L{tdir / 'lib'}",

@@ -216,6 +216,16 @@ hipError_t launch_film_mish_backward_sums(const float* s, const float* dy, int64
                                           const float* gamma, const float* beta, const float* add,
                                           float* ds, float* sums, double* partial, hipStream_t st);
 
+// ---- residual norm (norm_kernels.hip) ----------------------------------------
+// Rows [rows, width] of the values' type; r, h and rstd may be NULL; scale != NULL:
+// y is e4m3 bytes under a scale per row.
+hipError_t launch_add_rms_norm(int dtype, const void* x, const void* r, const void* w, int64_t rows, int64_t width,
+                               float eps, void* y, void* h, float* rstd, float* scale, hipStream_t st);
+size_t add_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t width);
+hipError_t launch_add_rms_norm_backward(int dtype, const void* dy, const void* dh, const void* h, const void* w,
+                                        const float* rstd, int64_t rows, int64_t width, void* dx, void* dw, float* partial,
+                                        hipStream_t st);
+
 // ---- content comparison (match_kernels.hip) -------------------------------
 constexpr int kMaxMatch = RELM_MP_MAX_MATCH;
 // After the launches mismatch[c] == gen iff the snapshot of plans[c] differs

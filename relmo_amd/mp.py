@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 
+from . import mp_readout as _readout
 from .mp_autograd import (
     _FaninReduceLogSumExpFunction,
     _FaninReduceSumFunction,
@@ -201,6 +202,47 @@ def _lgan_relation_graph_step(relation_pair_x, rr_src, rr_dst, tn_rel, tn_ent, n
     )
 
 
+def add_rms_norm(
+    x: torch.Tensor,
+    residual: torch.Tensor | None,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(y, h)``: the residual stream ``h = x + residual`` and its root-mean-square norm
+    ``y = h / sqrt(mean(h^2, -1) + eps) * weight``, in one pass.
+
+    ``x`` and ``residual`` [..., width] and ``weight`` [width] share a dtype (float32,
+    bfloat16 or float16 on the GPU).  The sum and its statistics are float32, rounded once
+    as each output is stored; the norm is that of the unrounded sum.  ``residual=None``
+    leaves the addition out (``h`` is ``x``).  No counterpart in relmo."""
+
+    require_torch("add_rms_norm")
+    return _readout.add_rms_norm(x, residual, weight, float(eps))
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """``x / sqrt(mean(x^2, -1) + eps) * weight`` (:func:`add_rms_norm` without a residual)."""
+
+    require_torch("rms_norm")
+    return _readout.rms_norm(x, weight, float(eps))
+
+
+def add_rms_norm_fp8(
+    x: torch.Tensor,
+    residual: torch.Tensor | None,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`add_rms_norm` with ``y`` in 8 bits, for serving: ``(q, scale, h)``.
+
+    ``q`` is float8_e4m3fn and ``scale`` float32 [...], one per row: ``max|y| / 448`` (1 for
+    a row of zeros), so ``y ~ q * scale`` and no value saturates.  A row with a NaN or
+    infinite ``y`` has that as its scale.  No gradient."""
+
+    require_torch("add_rms_norm_fp8")
+    return _readout.add_rms_norm_fp8(x, residual, weight, float(eps))
+
+
 @contextlib.contextmanager
 def plan_scope():
     """Trust scope for the library's index plans (no counterpart in relmo).
@@ -235,6 +277,8 @@ __all__ = [
     "MODE_SUM",
     "TORCH_IMPORT_ERROR",
     "activation_code",
+    "add_rms_norm",
+    "add_rms_norm_fp8",
     "assert_runtime_compat",
     "available",
     "fanin_pack_from_edges",
@@ -245,4 +289,5 @@ __all__ = [
     "fanout_pack_multi",
     "fanout_scatter",
     "plan_scope",
+    "rms_norm",
 ]
