@@ -542,6 +542,72 @@ int relm_mp_add_rms_norm_backward(int dtype, const void* dy, const void* dh, con
                                   const float* rstd, int64_t rows, int64_t width, void* dx, void* dw,
                                   void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
 
+/* ---- cross attention of per-graph queries to the graphs' objects ---------------
+ * Graph b has the queries [q_offsets[b], q_offsets[b + 1]) and the keys
+ * [k_offsets[b], k_offsets[b + 1]); query head h reads key head h / (heads / kv_heads).
+ * Per graph, head and query, over the graph's kept keys j:
+ *   s_j = scale * <q, k_j>, p = softmax(s), out = sum_j p_j v_j, lse = log(sum_j exp s_j);
+ * a query without a kept key has out = 0 and lse = -inf.  Values of keys that are not
+ * kept never enter, whatever they hold.  Softmax statistics and sums are float. */
+
+/* How a batch's work is laid over workgroups; made once per batch from its lengths and
+ * used by every call on it.  `table` is the plan's table in device memory. */
+typedef struct relm_mp_attention_plan {
+    int64_t q_rows;        /* queries of the batch                                       */
+    int64_t k_rows;        /* keys of the batch                                          */
+    int32_t heads;
+    int32_t kv_heads;
+    int64_t graphs;
+    int64_t table_bytes;
+    int32_t row_tile;      /* queries x shared heads of a workgroup's item               */
+    int32_t key_tile;      /* keys of an item of the key gradients                       */
+    int32_t num_items;     /* row items: rows of a graph against a range of its keys     */
+    int32_t num_parts;     /* of them, items over part of their keys                     */
+    int32_t num_joins;     /* rows whose parts are joined                                */
+    int32_t num_key_items; /* key items: keys of a graph against a range of its rows     */
+    int32_t num_key_parts;
+    int32_t num_key_joins;
+    const void* table;
+} relm_mp_attention_plan;
+
+/* Host only.  q_offsets and k_offsets: graphs + 1 host values from 0 to q_rows / k_rows,
+ * ascending.  table NULL: fills *plan but for its pointer (table_bytes among it); else
+ * also writes the table into `table` (host memory of table_bytes), which the caller
+ * copies to the device and stores in plan->table. */
+int relm_mp_attention_plan_build(const int64_t* q_offsets, const int64_t* k_offsets, int64_t graphs,
+                                 int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads,
+                                 void* table, size_t table_bytes, relm_mp_attention_plan* plan);
+
+/* Values [rows, heads, head_dim] with neighbouring values side by side; strides in values. */
+typedef struct relm_mp_head_rows {
+    const void* data;
+    int64_t row_stride;
+    int64_t head_stride;
+} relm_mp_head_rows;
+
+#define RELM_MP_MAX_HEAD_DIM 128
+
+size_t relm_mp_cross_attention_workspace_size(const relm_mp_attention_plan* plan, int64_t head_dim);
+/* out [q_rows, heads, head_dim] and lse [q_rows, heads] (float, may be NULL) contiguous;
+ * key_mask [k_rows] bytes, zero where the key is not kept (NULL: all are). */
+int relm_mp_cross_attention(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* q,
+                            const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim,
+                            const uint8_t* key_mask, float scale, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
+
+/* Backward from grad (of out), the forward's inputs, out and lse:
+ *   delta = <grad, out>, ds_j = p_j (<grad, v_j> - delta), dq = scale sum_j ds_j k_j,
+ *   dk_j = scale sum ds_j q, dv_j = sum p_j grad (over the queries and heads that read j).
+ * dq [q_rows, heads, head_dim], dk and dv [k_rows, kv_heads, head_dim] contiguous, fully
+ * written (keys that nothing reads get 0), added in a fixed order. */
+size_t relm_mp_cross_attention_backward_workspace_size(const relm_mp_attention_plan* plan, int64_t head_dim);
+int relm_mp_cross_attention_backward(int dtype, const relm_mp_attention_plan* plan,
+                                     const relm_mp_head_rows* grad, const relm_mp_head_rows* q,
+                                     const relm_mp_head_rows* k, const relm_mp_head_rows* v,
+                                     int64_t head_dim, const uint8_t* key_mask, float scale,
+                                     const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                     void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

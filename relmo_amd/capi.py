@@ -77,6 +77,11 @@ EXPORTED_SYMBOLS = (
     "relm_mp_add_rms_norm_fp8",
     "relm_mp_add_rms_norm_backward_workspace_size",
     "relm_mp_add_rms_norm_backward",
+    "relm_mp_attention_plan_build",
+    "relm_mp_cross_attention_workspace_size",
+    "relm_mp_cross_attention",
+    "relm_mp_cross_attention_backward_workspace_size",
+    "relm_mp_cross_attention_backward",
 )
 
 
@@ -131,12 +136,43 @@ class IndexPart(ctypes.Structure):
     ]
 
 
+class AttentionPlan(ctypes.Structure):
+    """Mirror of ``struct relm_mp_attention_plan``."""
+
+    _fields_ = [
+        ("q_rows", ctypes.c_int64),
+        ("k_rows", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("graphs", ctypes.c_int64),
+        ("table_bytes", ctypes.c_int64),
+        ("row_tile", ctypes.c_int32),
+        ("key_tile", ctypes.c_int32),
+        ("num_items", ctypes.c_int32),
+        ("num_parts", ctypes.c_int32),
+        ("num_joins", ctypes.c_int32),
+        ("num_key_items", ctypes.c_int32),
+        ("num_key_parts", ctypes.c_int32),
+        ("num_key_joins", ctypes.c_int32),
+        ("table", ctypes.c_void_p),
+    ]
+
+
+class HeadRows(ctypes.Structure):
+    """Mirror of ``struct relm_mp_head_rows``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _sz = ctypes.c_size_t
 _vp = ctypes.c_void_p
 _cp = ctypes.c_char_p
 _PP = ctypes.POINTER(Plan)
+_AP = ctypes.POINTER(AttentionPlan)
+_HR = ctypes.POINTER(HeadRows)
+_f32 = ctypes.c_float
 
 _SIGNATURES = {
     "relm_mp_last_error": (_cp, []),
@@ -195,12 +231,20 @@ _SIGNATURES = {
     "relm_mp_film_mish_backward_sums": (
         _int, [_vp, _vp, _i64, _i64, _vp, ctypes.c_int32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "relm_mp_add_rms_norm": (
-        _int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _vp]),
+        _int, [_int, _vp, _vp, _vp, _i64, _i64, _f32, _vp, _vp, _vp, _vp]),
     "relm_mp_add_rms_norm_fp8": (
-        _int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _vp]),
+        _int, [_int, _vp, _vp, _vp, _i64, _i64, _f32, _vp, _vp, _vp, _vp]),
     "relm_mp_add_rms_norm_backward_workspace_size": (_sz, [_int, _i64, _i64]),
     "relm_mp_add_rms_norm_backward": (
         _int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "relm_mp_attention_plan_build": (
+        _int, [_vp, _vp, _i64, _i64, _i64, ctypes.c_int32, ctypes.c_int32, _vp, _sz, _AP]),
+    "relm_mp_cross_attention_workspace_size": (_sz, [_AP, _i64]),
+    "relm_mp_cross_attention": (
+        _int, [_int, _AP, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "relm_mp_cross_attention_backward_workspace_size": (_sz, [_AP, _i64]),
+    "relm_mp_cross_attention_backward": (
+        _int, [_int, _AP, _HR, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "relm_mp_plan_match": (
         _int,
         [_vp, _vp, _i64, ctypes.POINTER(_PP), ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), _vp,

@@ -1,0 +1,71 @@
+// What the attention kernels and the plan that lays their work out share.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include "relm_mp.h"
+
+namespace relm_mp {
+
+// Rows of a graph: its queries times the heads that share a key head, row r being
+// query r / group and head r % group of the key head.  A row item is a range of a
+// graph's rows against a range of its keys, a key item a range of keys against a
+// range of rows; every item is run once per key head.
+struct AttnItem {
+    int32_t q_first;    // the graph's first query
+    int32_t row0;       // first row of the item within the graph
+    int32_t rows;
+    int32_t key_first;  // first key of the item in the batch
+    int32_t keys;
+    int32_t part;       // -1: the item's rows (keys) are whole; else where its sums go
+    int32_t pad[2];
+};
+
+// Rows (keys) whose parts [part0, part0 + parts) are joined.
+struct AttnJoin {
+    int32_t q_first;
+    int32_t row0;
+    int32_t rows;
+    int32_t key_first;
+    int32_t keys;
+    int32_t part0;
+    int32_t parts;
+    int32_t pad;
+};
+static_assert(sizeof(AttnItem) == 32 && sizeof(AttnJoin) == 32, "table records");
+
+// The tables of a plan, one after the other.
+inline const AttnItem* plan_items(const relm_mp_attention_plan& p) { return static_cast<const AttnItem*>(p.table); }
+inline const AttnJoin* plan_joins(const relm_mp_attention_plan& p) {
+    return reinterpret_cast<const AttnJoin*>(plan_items(p) + p.num_items);
+}
+inline const AttnItem* plan_key_items(const relm_mp_attention_plan& p) {
+    return reinterpret_cast<const AttnItem*>(plan_joins(p) + p.num_joins);
+}
+inline const AttnJoin* plan_key_joins(const relm_mp_attention_plan& p) {
+    return reinterpret_cast<const AttnJoin*>(plan_key_items(p) + p.num_key_items);
+}
+
+// Floats that the parts need: per part, key head and row the sum's head_dim values with
+// its maximum and total (forward), its values (dq), or two rows of values per key (dk, dv).
+inline size_t attention_part_floats(const relm_mp_attention_plan& p, int64_t head_dim) {
+    return static_cast<size_t>(p.num_parts) * p.kv_heads * p.row_tile * (head_dim + 2);
+}
+inline size_t attention_key_part_floats(const relm_mp_attention_plan& p, int64_t head_dim) {
+    return static_cast<size_t>(p.num_key_parts) * p.kv_heads * p.key_tile * 2 * head_dim;
+}
+
+struct AttnOperands {
+    relm_mp_head_rows q, k, v, grad;
+    int64_t head_dim;
+    const uint8_t* key_mask;
+    float scale;
+    void* out;       // forward's output; the backward reads it
+    float* lse;
+    float* delta;    // backward: [q_rows, heads]
+    void *dq, *dk, *dv;
+    float* parts;
+};
+
+}  // namespace relm_mp

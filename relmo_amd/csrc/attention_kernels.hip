@@ -1,0 +1,964 @@
+// Cross attention of per-graph queries to their graph's keys, forward and backward:
+//
+//   s = scale * q k^T,  p = softmax(s),  out = p v,  lse = log(sum exp s)
+//   delta = <grad, out>,  ds = p (grad v^T - delta),
+//   dq = scale * ds k,  dk = scale * ds^T q,  dv = p^T grad
+//
+// One pass over the keys with the running maximum and total of each row's softmax;
+// the scores stay in registers.  The scores are computed transposed (keys down,
+// queries across): a lane then holds four neighbouring keys of one query, which is
+// what the next product wants as an operand, so probabilities go from one matrix
+// instruction to the next without leaving the lane, and a query's statistics are one
+// value per lane.  Scores, statistics, totals and all accumulators are float;
+// probabilities and ds are rounded to the values' type for the products that read
+// them (each such rounding is independent of the others and of the size of the
+// outputs' own; with float values nothing is rounded).
+#include <hip/hip_runtime.h>
+
+#include "attention.h"
+#include "device_utils.h"
+#include "internal.h"
+#include "mfma_tiles.h"
+#include "value_types.h"
+
+namespace relm_mp {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kInf = __builtin_inff();
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A row's operand at its place: [rows, heads, head_dim] by strides.  `whole`: every row
+// of every head starts on a dword, so that 16-byte accesses serve; else a value at a time.
+template <typename T>
+struct Rows {
+    const T* data;
+    int64_t row_stride, head_stride;
+    bool whole;
+};
+
+template <typename T>
+Rows<T> rows_of(const relm_mp_head_rows& r) {
+    const auto dword = [](int64_t bytes) { return bytes % 4 == 0; };
+    return {static_cast<const T*>(r.data), r.row_stride, r.head_stride,
+            dword(reinterpret_cast<intptr_t>(r.data)) && dword(r.row_stride * static_cast<int64_t>(sizeof(T))) &&
+                dword(r.head_stride * static_cast<int64_t>(sizeof(T)))};
+}
+
+// Values [col, col + N) of a row of `dim` at p, zero past its end.
+template <typename T, int N>
+__device__ __forceinline__ T __attribute__((ext_vector_type(N))) take(const T* p, int col, int dim, bool whole) {
+    using Vec = T __attribute__((ext_vector_type(N)));
+    Vec v;
+    if (whole && col + N <= dim) {
+        if constexpr (sizeof(T) * N <= 16) {
+            v = *reinterpret_cast<const ValueVec<T, N>*>(p + col);
+        } else {
+            constexpr int M = 16 / sizeof(T);
+#pragma unroll
+            for (int c = 0; c < N / M; ++c) {
+                const ValueVec<T, M> part = *reinterpret_cast<const ValueVec<T, M>*>(p + col + c * M);
+#pragma unroll
+                for (int j = 0; j < M; ++j) v[c * M + j] = part[j];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = col + j < dim ? p[col + j] : static_cast<T>(0.0f);
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void put4(T* p, int col, int dim, bool whole, f32x4 x) {
+    if (whole && col + 4 <= dim) {
+        ValueVec<T, 4> v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = round_to<T>(x[j]);
+        *reinterpret_cast<ValueVec<T, 4>*>(p + col) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < dim) p[col + j] = round_to<T>(x[j]);
+    }
+}
+
+template <typename T>
+struct Args {
+    Rows<T> q, k, v, grad;
+    const uint8_t* key_mask;
+    int dim;
+    int heads, kv_heads, group;
+    int row_tile, key_tile;
+    float scale;
+    int num_items;
+    const AttnItem* items;
+    const AttnJoin* joins;
+    T* out;
+    float* lse;
+    float* delta;
+    T *dq, *dk, *dv;
+    float* parts;
+    bool out_whole;  // rows of head_dim values side by side start on dwords
+};
+
+// A workgroup's item and key head.  Neighbouring heads of an item share the lines of
+// its rows, and neighbouring items a graph's keys: they run on one XCD.
+struct Work {
+    AttnItem it;
+    int head;
+};
+__device__ __forceinline__ Work work_of(const AttnItem* items, int num_items, int kv_heads) {
+    const int flat = static_cast<int>(xcd_tile(blockIdx.x, static_cast<int64_t>(num_items) * kv_heads));
+    const int item = flat / kv_heads;
+    return {items[item], flat - item * kv_heads};
+}
+
+// Where row r of a graph lies: its query and head (the head counted over all heads).
+struct Place {
+    int64_t row;
+    int head;
+};
+template <typename T>
+__device__ __forceinline__ Place place_of(const Args<T>& a, int q_first, int kv_head, int r) {
+    const int q = r / a.group;
+    return {static_cast<int64_t>(q_first) + q, kv_head * a.group + (r - q * a.group)};
+}
+
+// BN rows of an operand in flight from global memory to LDS: a thread holds its share of
+// the tile in registers while the tile before it is computed on.  Rows of LDS are padded
+// by 16 bytes, which spreads a column's rows over the banks.
+template <typename T, int DP>
+constexpr int kLdsStride = DP + 16 / static_cast<int>(sizeof(T));
+
+template <typename T, int DP, int BN>
+struct TileLoad {
+    static constexpr int kV = 16 / static_cast<int>(sizeof(T));
+    static constexpr int kUnits = DP / kV;  // of a row
+    static constexpr int kRounds = (BN * kUnits + kThreads - 1) / kThreads;
+    using Vec = T __attribute__((ext_vector_type(kV)));
+    Vec v[kRounds];
+
+    // place(row) gives the row's pointer, NULL for a row of zeros
+    template <typename F>
+    __device__ __forceinline__ void fetch(F&& place, int dim, bool whole) {
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            const int u = i * kThreads + static_cast<int>(threadIdx.x);
+            const int row = u / kUnits, col = (u % kUnits) * kV;
+            const T* p = u < BN * kUnits ? place(row) : nullptr;
+            if (p != nullptr)
+                v[i] = take<T, kV>(p, col, dim, whole);
+            else
+                v[i] = Vec(static_cast<T>(0.0f));
+        }
+    }
+    // keep(row): whether the row's values enter (a row that does not is stored as zeros)
+    template <typename F>
+    __device__ __forceinline__ void store(T* tile, F&& keep) const {
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            const int u = i * kThreads + static_cast<int>(threadIdx.x);
+            const int row = u / kUnits, col = (u % kUnits) * kV;
+            if (u < BN * kUnits)
+                *reinterpret_cast<Vec*>(tile + row * kLdsStride<T, DP> + col) = keep(row) ? v[i] : Vec(static_cast<T>(0.0f));
+        }
+    }
+};
+
+// Which of a tile's BN keys are kept: bit k of the words.
+template <int BN>
+struct KeyBits {
+    uint8_t byte[BN / 64];
+    uint64_t bits[BN / 64];
+    // asks for the mask's bytes of keys [first, first + left)
+    __device__ __forceinline__ void fetch(const uint8_t* mask, int64_t first, int left) {
+#pragma unroll
+        for (int w = 0; w < BN / 64; ++w) {
+            const int k = w * 64 + lane_id();
+            byte[w] = k < left ? (mask != nullptr ? mask[first + k] : 1) : 0;
+        }
+    }
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int w = 0; w < BN / 64; ++w) bits[w] = __ballot(byte[w] != 0);
+    }
+    __device__ __forceinline__ bool has(int k) const {
+        const uint64_t w = BN == 128 && (k & 64) ? bits[BN / 64 - 1] : bits[0];
+        return (w >> (k % 64)) & 1;
+    }
+    // the 32 keys from k on
+    __device__ __forceinline__ uint32_t chunk(int k) const {
+        const uint64_t w = BN == 128 && (k & 64) ? bits[BN / 64 - 1] : bits[0];
+        return static_cast<uint32_t>(w >> (k % 64));
+    }
+};
+
+// Fragments of 16 rows of q (or grad) that a wave keeps: lane l holds row l % 16.
+template <typename T, int DP>
+struct RowFrags {
+    Frag<T> f[DP / 32];
+    __device__ __forceinline__ void fetch(const T* p, int dim, bool whole) {
+        const int g = lane_id() / 16;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+            if (p != nullptr)
+                f[c] = take<T, 8>(p, c * 32 + g * 8, dim, whole);
+            else
+                f[c] = Frag<T>(static_cast<T>(0.0f));
+        }
+    }
+};
+
+// Scores (before scaling) of 32 keys by 16 rows, keys down: two tiles of 16 keys.
+template <typename T, int DP>
+__device__ __forceinline__ void keys_by_rows(const T* keys, int key0, const RowFrags<T, DP>& rows, f32x4 (&s)[2]) {
+    const int l = lane_id();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4(0.0f);
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+            s[t] = mma<T>(lds_frag<T>(keys, kLdsStride<T, DP>, key0 + 16 * t + l % 16, c * 32 + (l / 16) * 8), rows.f[c], s[t]);
+    }
+}
+
+// Entries of the lane's keys that are not kept become `value`.
+__device__ __forceinline__ void leave_out(f32x4 (&s)[2], uint32_t kept, float value) {
+    if (kept == 0xffffffffu) return;
+    const uint32_t mine = kept >> (4 * (lane_id() / 16));
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (!((mine >> (16 * t + i)) & 1)) s[t][i] = value;
+}
+
+// Over the four lanes that share a query (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float lanes_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// Shapes of the row kernels: a wave has RT tiles of 16 rows; WM waves have rows of their
+// own and 4 / WM share each row tile, taking different keys of a tile.
+template <int RT, int WM>
+struct RowShape {
+    static constexpr int kRows = 16 * RT * WM;             // of a workgroup
+    static constexpr int kSharers = kWaves / WM;           // waves on one row tile
+    static constexpr int kKeys = kSharers == 4 ? 128 : 64; // of a tile in LDS
+    static constexpr int kChunks = kKeys / (32 * kSharers);  // 32-key chunks of a wave per tile
+};
+
+// Forward.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with the running maximum m:
+// when a key tile raises it, what has been added up is scaled by exp(m_old - m_new).
+template <typename T, int DP, int RT, int WM>
+__global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
+    using S = RowShape<RT, WM>;
+    constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
+    constexpr int kTileBytes = 2 * BN * ST * static_cast<int>(sizeof(T));
+    constexpr int kMergeBytes = S::kSharers > 1 ? kWaves * 16 * RT * (DP + 2) * 4 : 0;
+    __shared__ __align__(16) char lds[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+    T* kt = reinterpret_cast<T*>(lds);
+    T* vt = kt + BN * ST;
+    const Work w = work_of(a.items, a.num_items, a.kv_heads);
+    const int l = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, g = l / 16;
+    const int row_wave = wave / S::kSharers, key_wave = wave % S::kSharers;
+    const float sl2 = a.scale * kLog2e;
+
+    RowFrags<T, DP> qf[RT];
+    Place at[RT];
+    bool real[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = (row_wave * RT + r) * 16 + l % 16;
+        real[r] = row < w.it.rows;
+        at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
+        qf[r].fetch(real[r] ? a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride : nullptr, a.dim, a.q.whole);
+    }
+    f32x4 o[RT][ND];
+    float m[RT], total[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        m[r] = -kInf;
+        total[r] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) o[r][n] = f32x4(0.0f);
+    }
+
+    TileLoad<T, DP, BN> kl, vl;
+    KeyBits<BN> bits;
+    const auto fetch = [&](int k0) {
+        const int left = w.it.keys - k0;
+        const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
+        const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
+        const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
+        kl.fetch([&](int row) { return row < left ? kp + row * a.k.row_stride : nullptr; }, a.dim, a.k.whole);
+        vl.fetch([&](int row) { return row < left ? vp + row * a.v.row_stride : nullptr; }, a.dim, a.v.whole);
+        bits.fetch(a.key_mask, first, left);
+    };
+    if (w.it.keys > 0) fetch(0);
+    for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
+        bits.settle();
+        __syncthreads();
+        kl.store(kt, [](int) { return true; });  // scores of keys that are not kept are replaced, not used
+        vl.store(vt, [&](int row) { return a.key_mask == nullptr || bits.has(row); });
+        __syncthreads();
+        const KeyBits<BN> now = bits;
+        if (k0 + BN < w.it.keys) fetch(k0 + BN);
+        f32x4 s[RT][S::kChunks][2];
+        float top[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) top[r] = -kInf;
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+            const int key0 = (key_wave * S::kChunks + c) * 32;
+            const uint32_t kept = now.chunk(key0);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                keys_by_rows<T, DP>(kt, key0, qf[r], s[r][c]);
+                leave_out(s[r][c], kept, -kInf);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], s[r][c][t][i]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            // the maximum of scale * log2(e) * s; the factor is positive
+            const float most = fmaxf(m[r], lanes_max(top[r]) * sl2);
+            if (__any(most > m[r])) {
+                const float shrink = exp2_of(m[r] - (most == -kInf ? 0.0f : most));
+                total[r] *= shrink;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) o[r][n] *= shrink;
+                m[r] = most;
+            }
+            const float base = m[r] == -kInf ? 0.0f : m[r];
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = exp2_of(fmaf(s[r][c][t][i], sl2, -base));
+                        s[r][c][t][i] = p;
+                        total[r] += p;
+                    }
+        }
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+            const int key0 = (key_wave * S::kChunks + c) * 32;
+            Frag<T> p[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) p[r] = frag_of<T>(s[r][c][0], s[r][c][1]);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const Frag<T> vf = lds_frag_t<T>(vt, ST, key0, n * 16);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) o[r][n] = mma<T>(vf, p[r], o[r][n]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) total[r] = lanes_sum(total[r]);
+
+    const auto finish = [&](int row, Place p, int col, f32x4 sum, float top, float sum_p) {
+        if (w.it.part < 0) {
+            const float inv = sum_p == 0.0f ? 0.0f : 1.0f / sum_p;
+            put4<T>(a.out + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * inv);
+            if (col == 0 && a.lse != nullptr)
+                a.lse[p.row * a.heads + p.head] = sum_p == 0.0f ? -kInf : (top + log2f(sum_p)) * kLn2;
+        } else {
+            const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
+            float* to = a.parts + slot * (a.dim + 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < a.dim) to[2 + col + j] = sum[j];
+            if (col == 0) {
+                to[0] = top;
+                to[1] = sum_p;
+            }
+        }
+    };
+    if constexpr (S::kSharers == 1) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+            if (real[r])
+#pragma unroll
+                for (int n = 0; n < ND; ++n)
+                    finish((row_wave * RT + r) * 16 + l % 16, at[r], n * 16 + g * 4, o[r][n], m[r], total[r]);
+    } else {
+        // the sharers' sums, brought to the largest of their maxima, meet in LDS
+        constexpr int R = 16 * RT;
+        float* tops = reinterpret_cast<float*>(lds);  // [kWaves][R]
+        float* totals = tops + kWaves * R;
+        float* sums = totals + kWaves * R;            // [kWaves][R][DP]
+        __syncthreads();
+        if (g == 0) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                tops[wave * R + r * 16 + l] = m[r];
+                totals[wave * R + r * 16 + l] = total[r];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+                *reinterpret_cast<f32x4*>(sums + (wave * R + r * 16 + l % 16) * DP + n * 16 + g * 4) = o[r][n];
+        __syncthreads();
+        for (int u = static_cast<int>(threadIdx.x); u < w.it.rows * (DP / 4); u += kThreads) {
+            const int row = u / (DP / 4), col = (u % (DP / 4)) * 4;
+            if (col >= a.dim) continue;
+            const int slot = (row / R) * S::kSharers * R + row % R;  // the first sharer's
+            float top = -kInf, sum_p = 0.0f;
+#pragma unroll
+            for (int v = 0; v < S::kSharers; ++v) top = fmaxf(top, tops[v * R + slot]);
+            const float base = top == -kInf ? 0.0f : top;
+            f32x4 sum = f32x4(0.0f);
+#pragma unroll
+            for (int v = 0; v < S::kSharers; ++v) {
+                const float share = exp2_of(tops[v * R + slot] - base);
+                sum_p = fmaf(totals[v * R + slot], share, sum_p);
+                sum += *reinterpret_cast<const f32x4*>(sums + (v * R + slot) * DP + col) * share;
+            }
+            finish(row, place_of(a, w.it.q_first, w.head, w.it.row0 + row), col, sum, top, sum_p);
+        }
+    }
+}
+
+// Joins the parts of a row: out = sum_p 2^(m_p - m) sum_p / sum_p 2^(m_p - m) total_p.
+// A workgroup per row and key head; its thread groups take every kThreads / DP-th part.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
+    constexpr int G = kThreads / DP;
+    __shared__ float lds_top[kThreads], lds_total[G], lds_sum[G][DP];
+    const AttnJoin j = a.joins[blockIdx.x / a.row_tile];
+    const int row = static_cast<int>(blockIdx.x) % a.row_tile, head = static_cast<int>(blockIdx.y);
+    if (row >= j.rows) return;
+    const int t = static_cast<int>(threadIdx.x), d = t % DP, grp = t / DP;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.row_tile * (a.dim + 2);
+    const float* part = a.parts + ((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.row_tile + row) * (a.dim + 2);
+    float top = -kInf;
+    for (int p = t; p < j.parts; p += kThreads) top = fmaxf(top, part[p * step]);
+    lds_top[t] = top;
+    __syncthreads();
+    for (int o = kThreads / 2; o > 0; o /= 2) {
+        if (t < o) lds_top[t] = fmaxf(lds_top[t], lds_top[t + o]);
+        __syncthreads();
+    }
+    top = lds_top[0];
+    const float base = top == -kInf ? 0.0f : top;
+    float sum = 0.0f, total = 0.0f;
+    const bool mine = d < a.dim;
+    for (int p = grp; p < j.parts; p += G) {
+        const float share = exp2_of(part[p * step] - base);
+        total = fmaf(part[p * step + 1], share, total);
+        if (mine) sum = fmaf(part[p * step + 2 + d], share, sum);
+    }
+    lds_sum[grp][d] = sum;
+    if (d == 0) lds_total[grp] = total;
+    __syncthreads();
+    if (grp != 0 || !mine) return;
+    for (int i = 1; i < G; ++i) {
+        sum += lds_sum[i][d];
+        total += lds_total[i];
+    }
+    const Place p = place_of(a, j.q_first, head, j.row0 + row);
+    a.out[(p.row * a.heads + p.head) * a.dim + d] = round_to<T>(total == 0.0f ? 0.0f : sum * (1.0f / total));
+    if (d == 0 && a.lse != nullptr) a.lse[p.row * a.heads + p.head] = total == 0.0f ? -kInf : (top + log2f(total)) * kLn2;
+}
+
+// Scores to probabilities and their gradients in place: s becomes p, dp becomes ds.
+__device__ __forceinline__ void backward_scores(f32x4 (&s)[2], f32x4 (&dp)[2], uint32_t kept, float sl2, float lse2, float delta) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = exp2_of(fmaf(s[t][i], sl2, -lse2));
+            s[t][i] = p;
+            dp[t][i] = p * (dp[t][i] - delta);
+        }
+    leave_out(s, kept, 0.0f);
+    leave_out(dp, kept, 0.0f);
+}
+
+// Half values lose bits below 2^-14, where ds of keys with small probabilities lies.  A lane
+// holds ds of one query (key) and the sum over keys (queries) that it enters: both are kept
+// in units of a power of two, which falls as the largest ds seen so far rises (like the
+// forward's running maximum), so that that one is held as 2^14 to 2^15.  Other types have
+// float's range: unit 1.
+constexpr float kFirstUnit = 1152921504606846976.0f;  // 2^60
+
+template <typename T>
+constexpr float kStartUnit = std::is_same_v<T, f16> ? kFirstUnit : 1.0f;
+
+template <typename T, int N>
+__device__ __forceinline__ void into_unit(f32x4 (&ds)[2], float& unit, f32x4 (&sum)[N]) {
+    if constexpr (std::is_same_v<T, f16>) {
+        float most = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(ds[t][i]));
+        most = lanes_max(most);
+        if (__any(most * unit > 32768.0f)) {
+            const int e = static_cast<int>(__float_as_uint(most) >> 23);  // 127 + floor(log2(most))
+            const float fresh = fminf(unit, __uint_as_float(static_cast<unsigned>(min(268 - e, 187)) << 23));
+            const float change = fresh * (1.0f / unit);
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[n] *= change;
+            unit = fresh;
+        }
+        ds[0] *= unit;
+        ds[1] *= unit;
+    }
+}
+
+// A row's log2 total for the backward; +inf (all probabilities 0) for a row that had no
+// finite score.
+__device__ __forceinline__ float lse2_of(float lse) { return lse == -kInf ? kInf : lse * kLog2e; }
+
+// dq of a row item: like the forward, with the probabilities recomputed from lse.  The
+// item over a row's first keys also leaves its delta for the key kernel.
+template <typename T, int DP, int RT, int WM>
+__global__ __launch_bounds__(kThreads) void k_attention_dq(Args<T> a) {
+    using S = RowShape<RT, WM>;
+    constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
+    constexpr int kTileBytes = 2 * BN * ST * static_cast<int>(sizeof(T));
+    constexpr int kMergeBytes = S::kSharers > 1 ? kWaves * 16 * RT * DP * 4 : 0;
+    __shared__ __align__(16) char lds[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+    T* kt = reinterpret_cast<T*>(lds);
+    T* vt = kt + BN * ST;
+    const Work w = work_of(a.items, a.num_items, a.kv_heads);
+    const int l = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, g = l / 16;
+    const int row_wave = wave / S::kSharers, key_wave = wave % S::kSharers;
+    const float sl2 = a.scale * kLog2e;
+
+    RowFrags<T, DP> qf[RT], gf[RT];
+    Place at[RT];
+    bool real[RT];
+    float lse2[RT], delta[RT], unit[RT];
+    f32x4 dq[RT][ND];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = (row_wave * RT + r) * 16 + l % 16;
+        real[r] = row < w.it.rows;
+        at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
+        qf[r].fetch(real[r] ? a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride : nullptr, a.dim, a.q.whole);
+        gf[r].fetch(real[r] ? a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride : nullptr, a.dim,
+                    a.grad.whole);
+        RowFrags<T, DP> of;
+        of.fetch(real[r] ? a.out + (at[r].row * a.heads + at[r].head) * a.dim : nullptr, a.dim, a.out_whole);
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
+        delta[r] = lanes_sum(sum);
+        lse2[r] = real[r] ? lse2_of(a.lse[at[r].row * a.heads + at[r].head]) : kInf;
+        unit[r] = kStartUnit<T>;
+        if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
+#pragma unroll
+        for (int n = 0; n < ND; ++n) dq[r][n] = f32x4(0.0f);
+    }
+
+    TileLoad<T, DP, BN> kl, vl;
+    KeyBits<BN> bits;
+    const auto fetch = [&](int k0) {
+        const int left = w.it.keys - k0;
+        const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
+        const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
+        const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
+        kl.fetch([&](int row) { return row < left ? kp + row * a.k.row_stride : nullptr; }, a.dim, a.k.whole);
+        vl.fetch([&](int row) { return row < left ? vp + row * a.v.row_stride : nullptr; }, a.dim, a.v.whole);
+        bits.fetch(a.key_mask, first, left);
+    };
+    if (w.it.keys > 0) fetch(0);
+    for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
+        bits.settle();
+        __syncthreads();
+        kl.store(kt, [&](int row) { return a.key_mask == nullptr || bits.has(row); });
+        vl.store(vt, [](int) { return true; });
+        __syncthreads();
+        const KeyBits<BN> now = bits;
+        if (k0 + BN < w.it.keys) fetch(k0 + BN);
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+            const int key0 = (key_wave * S::kChunks + c) * 32;
+            const uint32_t kept = now.chunk(key0);
+            Frag<T> ds[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                f32x4 s[2], dp[2];
+                keys_by_rows<T, DP>(kt, key0, qf[r], s);
+                keys_by_rows<T, DP>(vt, key0, gf[r], dp);
+                backward_scores(s, dp, kept, sl2, lse2[r], delta[r]);
+                into_unit<T>(dp, unit[r], dq[r]);
+                ds[r] = frag_of<T>(dp[0], dp[1]);
+            }
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const Frag<T> kf = lds_frag_t<T>(kt, ST, key0, n * 16);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) dq[r][n] = mma<T>(kf, ds[r], dq[r][n]);
+            }
+        }
+    }
+
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) dq[r][n] *= 1.0f / unit[r];
+    const auto finish = [&](int row, Place p, int col, f32x4 sum) {
+        if (w.it.part < 0) {
+            put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * a.scale);
+        } else {
+            const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < a.dim) a.parts[slot * a.dim + col + j] = sum[j];
+        }
+    };
+    if constexpr (S::kSharers == 1) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+            if (real[r])
+#pragma unroll
+                for (int n = 0; n < ND; ++n) finish((row_wave * RT + r) * 16 + l % 16, at[r], n * 16 + g * 4, dq[r][n]);
+    } else {
+        constexpr int R = 16 * RT;
+        float* sums = reinterpret_cast<float*>(lds);  // [kWaves][R][DP]
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+                *reinterpret_cast<f32x4*>(sums + (wave * R + r * 16 + l % 16) * DP + n * 16 + g * 4) = dq[r][n];
+        __syncthreads();
+        for (int u = static_cast<int>(threadIdx.x); u < w.it.rows * (DP / 4); u += kThreads) {
+            const int row = u / (DP / 4), col = (u % (DP / 4)) * 4;
+            const int slot = (row / R) * S::kSharers * R + row % R;  // the first sharer's
+            f32x4 sum = *reinterpret_cast<const f32x4*>(sums + slot * DP + col);
+#pragma unroll
+            for (int v = 1; v < S::kSharers; ++v) sum += *reinterpret_cast<const f32x4*>(sums + (v * R + slot) * DP + col);
+            if (col < a.dim) finish(row, place_of(a, w.it.q_first, w.head, w.it.row0 + row), col, sum);
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void k_attention_dq_join(Args<T> a) {
+    constexpr int G = kThreads / DP;
+    __shared__ float lds_sum[G][DP];
+    const AttnJoin j = a.joins[blockIdx.x / a.row_tile];
+    const int row = static_cast<int>(blockIdx.x) % a.row_tile, head = static_cast<int>(blockIdx.y);
+    if (row >= j.rows) return;
+    const int t = static_cast<int>(threadIdx.x), d = t % DP, grp = t / DP;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.row_tile * a.dim;
+    const float* part = a.parts + ((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.row_tile + row) * a.dim;
+    float sum = 0.0f;
+    if (d < a.dim)
+        for (int p = grp; p < j.parts; p += G) sum += part[p * step + d];
+    lds_sum[grp][d] = sum;
+    __syncthreads();
+    if (grp != 0 || d >= a.dim) return;
+    for (int i = 1; i < G; ++i) sum += lds_sum[i][d];
+    const Place p = place_of(a, j.q_first, head, j.row0 + row);
+    a.dq[(p.row * a.heads + p.head) * a.dim + d] = round_to<T>(sum * a.scale);
+}
+
+// Half values end at 2^-14 (below, they lose bits): the probabilities of a query with
+// tens of thousands of keys would.  They are at most 1, so dv adds them up in units of
+// 2^-15.
+template <typename T>
+constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
+
+// dk and dv of a key item: a wave keeps KT tiles of 16 keys and walks the graph's rows
+// (rows down, keys across, so that a lane's probabilities are the operand of the products
+// over rows).
+template <typename T, int DP, int KT>
+__global__ __launch_bounds__(kThreads) void k_attention_dkv(Args<T> a) {
+    constexpr int BR = 64, ST = kLdsStride<T, DP>, ND = DP / 16;
+    __shared__ __align__(16) T qt[BR * ST];
+    __shared__ __align__(16) T gt[BR * ST];
+    __shared__ __align__(16) float row_lse2[BR];
+    __shared__ __align__(16) float row_delta[BR];
+    // an item's keys are taken by key_tile / (64 KT) workgroups
+    const int slices = a.key_tile / (64 * KT);
+    const Work w = work_of(a.items, a.num_items, a.kv_heads * slices);
+    const int head = w.head / slices;
+    const int l = lane_id(), g = l / 16, wave = (w.head % slices) * kWaves + static_cast<int>(threadIdx.x) / kWave;
+    const float sl2 = a.scale * kLog2e;
+
+    RowFrags<T, DP> kf[KT], vf[KT];
+    bool kept[KT], real[KT];
+    float unit[KT];
+    f32x4 dk[KT][ND], dv[KT][ND];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const int key = (wave * KT + t) * 16 + l % 16;
+        const int64_t at = static_cast<int64_t>(w.it.key_first) + key;
+        real[t] = key < w.it.keys;
+        kept[t] = real[t] && (a.key_mask == nullptr || a.key_mask[at] != 0);
+        kf[t].fetch(kept[t] ? a.k.data + at * a.k.row_stride + head * a.k.head_stride : nullptr, a.dim, a.k.whole);
+        vf[t].fetch(kept[t] ? a.v.data + at * a.v.row_stride + head * a.v.head_stride : nullptr, a.dim, a.v.whole);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) dk[t][n] = dv[t][n] = f32x4(0.0f);
+        unit[t] = kStartUnit<T>;
+    }
+
+    TileLoad<T, DP, BR> ql, gl;
+    float lse_in = 0.0f, delta_in = 0.0f;
+    const auto fetch = [&](int r0) {
+        const int left = w.it.rows - r0;
+        ql.fetch([&](int row) {
+            const Place p = place_of(a, w.it.q_first, head, w.it.row0 + r0 + row);
+            return row < left ? a.q.data + p.row * a.q.row_stride + p.head * a.q.head_stride : nullptr;
+        }, a.dim, a.q.whole);
+        gl.fetch([&](int row) {
+            const Place p = place_of(a, w.it.q_first, head, w.it.row0 + r0 + row);
+            return row < left ? a.grad.data + p.row * a.grad.row_stride + p.head * a.grad.head_stride : nullptr;
+        }, a.dim, a.grad.whole);
+        const int row = static_cast<int>(threadIdx.x);
+        if (row < BR) {
+            lse_in = kInf;
+            delta_in = 0.0f;
+            if (row < left) {
+                const Place p = place_of(a, w.it.q_first, head, w.it.row0 + r0 + row);
+                lse_in = lse2_of(a.lse[p.row * a.heads + p.head]);
+                delta_in = a.delta[p.row * a.heads + p.head];
+            }
+        }
+    };
+    if (w.it.rows > 0) fetch(0);
+    for (int r0 = 0; r0 < w.it.rows; r0 += BR) {
+        __syncthreads();
+        ql.store(qt, [](int) { return true; });
+        gl.store(gt, [](int) { return true; });
+        if (threadIdx.x < BR) {
+            row_lse2[threadIdx.x] = lse_in;
+            row_delta[threadIdx.x] = delta_in;
+        }
+        __syncthreads();
+        const int left = w.it.rows - r0;
+        if (left > BR) fetch(r0 + BR);
+#pragma unroll
+        for (int c = 0; c < BR / 32; ++c) {
+            if (c * 32 >= left) break;
+            Frag<T> pf[KT], dsf[KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                f32x4 s[2], dp[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = c * 32 + h * 16;
+                    s[h] = dp[h] = f32x4(0.0f);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) {
+                        s[h] = mma<T>(lds_frag<T>(qt, ST, row + l % 16, i * 32 + g * 8), kf[t].f[i], s[h]);
+                        dp[h] = mma<T>(lds_frag<T>(gt, ST, row + l % 16, i * 32 + g * 8), vf[t].f[i], dp[h]);
+                    }
+                    const f32x4 lse2 = *reinterpret_cast<const f32x4*>(row_lse2 + row + g * 4);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + row + g * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = kept[t] ? exp2_of(fmaf(s[h][i], sl2, -lse2[i])) : 0.0f;
+                        s[h][i] = p;
+                        dp[h][i] = kept[t] ? p * (dp[h][i] - delta[i]) : 0.0f;
+                    }
+                }
+                pf[t] = frag_of<T>(s[0] * kProbabilityUnit<T>, s[1] * kProbabilityUnit<T>);
+                into_unit<T>(dp, unit[t], dk[t]);
+                dsf[t] = frag_of<T>(dp[0], dp[1]);
+            }
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const Frag<T> gf = lds_frag_t<T>(gt, ST, c * 32, n * 16);
+                const Frag<T> qf = lds_frag_t<T>(qt, ST, c * 32, n * 16);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    dv[t][n] = mma<T>(gf, pf[t], dv[t][n]);
+                    dk[t][n] = mma<T>(qf, dsf[t], dk[t][n]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        if (!real[t]) continue;
+        const int key = (wave * KT + t) * 16 + l % 16;
+        const int64_t at = (static_cast<int64_t>(w.it.key_first) + key) * a.kv_heads + head;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+            const int col = n * 16 + g * 4;
+            dk[t][n] *= 1.0f / unit[t];
+            if (w.it.part < 0) {
+                put4<T>(a.dk + at * a.dim, col, a.dim, a.out_whole, dk[t][n] * a.scale);
+                put4<T>(a.dv + at * a.dim, col, a.dim, a.out_whole, dv[t][n] * (1.0f / kProbabilityUnit<T>));
+            } else {
+                float* to = a.parts +
+                            ((static_cast<int64_t>(w.it.part) * a.kv_heads + head) * a.key_tile + key) * (2 * a.dim);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < a.dim) {
+                        to[col + j] = dk[t][n][j];
+                        to[a.dim + col + j] = dv[t][n][j] * (1.0f / kProbabilityUnit<T>);
+                    }
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_attention_dkv_join(Args<T> a) {
+    const AttnJoin j = a.joins[blockIdx.x / a.key_tile];
+    const int key = static_cast<int>(blockIdx.x) % a.key_tile, head = static_cast<int>(blockIdx.y);
+    const int d = static_cast<int>(threadIdx.x);
+    if (key >= j.keys || d >= 2 * a.dim) return;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.key_tile * 2 * a.dim;
+    const float* part = a.parts + ((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.key_tile + key) * (2 * a.dim) + d;
+    float sum = 0.0f;
+    for (int p = 0; p < j.parts; ++p) sum += part[p * step];
+    const int64_t at = ((static_cast<int64_t>(j.key_first) + key) * a.kv_heads + head) * a.dim;
+    if (d < a.dim)
+        a.dk[at + d] = round_to<T>(sum * a.scale);
+    else
+        a.dv[at + d - a.dim] = round_to<T>(sum);
+}
+
+// ---- launches -----------------------------------------------------------------------
+
+template <typename T>
+Args<T> args_of(const relm_mp_attention_plan& p, const AttnOperands& o) {
+    Args<T> a{};
+    a.q = rows_of<T>(o.q);
+    a.k = rows_of<T>(o.k);
+    a.v = rows_of<T>(o.v);
+    a.grad = rows_of<T>(o.grad);
+    a.key_mask = o.key_mask;
+    a.dim = static_cast<int>(o.head_dim);
+    a.heads = p.heads;
+    a.kv_heads = p.kv_heads;
+    a.group = p.heads / p.kv_heads;
+    a.row_tile = p.row_tile;
+    a.key_tile = p.key_tile;
+    a.scale = o.scale;
+    a.num_items = p.num_items;
+    a.items = plan_items(p);
+    a.joins = plan_joins(p);
+    a.out = static_cast<T*>(o.out);
+    a.lse = o.lse;
+    a.delta = o.delta;
+    a.dq = static_cast<T*>(o.dq);
+    a.dk = static_cast<T*>(o.dk);
+    a.dv = static_cast<T*>(o.dv);
+    a.parts = o.parts;
+    a.out_whole = sizeof(T) * o.head_dim % 4 == 0;
+    for (const void* x : {o.out, o.dq, o.dk, o.dv}) a.out_whole = a.out_whole && reinterpret_cast<uintptr_t>(x) % 4 == 0;
+    return a;
+}
+
+// f with the padded head size (32, 64 or 128) and the rows' shape of the plan.
+template <typename F>
+void with_dim(int64_t dim, F&& f) {
+    if (dim <= 32)
+        f(std::integral_constant<int, 32>{});
+    else if (dim <= 64)
+        f(std::integral_constant<int, 64>{});
+    else
+        f(std::integral_constant<int, 128>{});
+}
+template <typename T, int DP, typename F>
+void with_rows(int row_tile, F&& f) {
+    using std::integral_constant;
+    // float rows of 128 values: tiles of 128 keys and of 32 rows to a wave leave it too
+    // few registers
+    constexpr bool kLarge = sizeof(T) * DP >= 512;
+    switch (row_tile) {
+        case 16: f(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
+        case 32: f(integral_constant<int, kLarge ? 1 : 2>{}, integral_constant<int, kLarge ? 2 : 1>{}); break;
+        case 64: f(integral_constant<int, 1>{}, integral_constant<int, 4>{}); break;
+        default: f(integral_constant<int, 2>{}, integral_constant<int, 4>{}); break;
+    }
+}
+
+template <typename T>
+hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
+    const Args<T> a = args_of<T>(p, o);
+    if (p.num_items == 0) return hipSuccess;
+    with_dim(o.head_dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        with_rows<T, DP>(p.row_tile, [&](auto rt, auto wm) {
+            hipLaunchKernelGGL((k_attention<T, DP, decltype(rt)::value, decltype(wm)::value>),
+                               dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
+        });
+        if (p.num_joins > 0)
+            hipLaunchKernelGGL((k_attention_join<T, DP>), dim3(static_cast<unsigned>(p.num_joins) * p.row_tile, p.kv_heads),
+                               dim3(kThreads), 0, st, a);
+    });
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
+    const Args<T> a = args_of<T>(p, o);
+    with_dim(o.head_dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        if (p.num_items > 0)
+            with_rows<T, DP>(p.row_tile, [&](auto rt, auto wm) {
+                hipLaunchKernelGGL((k_attention_dq<T, DP, decltype(rt)::value, decltype(wm)::value>),
+                                   dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
+            });
+        if (p.num_joins > 0)
+            hipLaunchKernelGGL((k_attention_dq_join<T, DP>),
+                               dim3(static_cast<unsigned>(p.num_joins) * p.row_tile, p.kv_heads), dim3(kThreads), 0, st, a);
+        if (p.num_key_items > 0) {
+            Args<T> b = a;
+            b.items = plan_key_items(p);
+            b.joins = plan_key_joins(p);
+            b.num_items = p.num_key_items;
+            // two tiles of keys to a wave halve its reads of the rows; float rows of 128
+            // values leave no registers for the second
+            constexpr int KT = sizeof(T) * DP < 512 ? 2 : 1;
+            const unsigned wgs = static_cast<unsigned>(p.num_key_items) * p.kv_heads;
+            if (p.key_tile == 64 * KT)
+                hipLaunchKernelGGL((k_attention_dkv<T, DP, KT>), dim3(wgs), dim3(kThreads), 0, st, b);
+            else
+                hipLaunchKernelGGL((k_attention_dkv<T, DP, 1>), dim3(wgs * (p.key_tile / 64)), dim3(kThreads), 0, st, b);
+            if (p.num_key_joins > 0)
+                hipLaunchKernelGGL(k_attention_dkv_join<T>,
+                                   dim3(static_cast<unsigned>(p.num_key_joins) * p.key_tile, p.kv_heads), dim3(kThreads), 0,
+                                   st, b);
+        }
+    });
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cross_attention(int dtype, const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
+    hipError_t e = hipErrorInvalidValue;
+    with_value_type(dtype, [&](auto t) { e = forward<decltype(t)>(p, o, st); });
+    return e;
+}
+
+hipError_t launch_cross_attention_backward(int dtype, const relm_mp_attention_plan& p, const AttnOperands& o,
+                                           hipStream_t st) {
+    hipError_t e = hipErrorInvalidValue;
+    with_value_type(dtype, [&](auto t) { e = backward<decltype(t)>(p, o, st); });
+    return e;
+}
+
+}  // namespace relm_mp

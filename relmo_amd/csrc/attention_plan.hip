@@ -1,0 +1,175 @@
+// The plan of a batch's cross attention, on the host: from the lengths of its graphs,
+// which workgroup takes which rows and keys.
+#include <algorithm>
+#include <cstring>
+#include <string>
+#include <vector>
+
+#include "attention.h"
+#include "internal.h"
+
+namespace relm_mp {
+
+namespace {
+
+constexpr int64_t kWorkgroups = 1024;  // of a launch: four to each of 256 CUs
+constexpr int64_t kPartUnit = 128;     // parts end on whole tiles of keys and rows
+constexpr int64_t kLeastKeys = 512;    // of a part: shorter ones cost more to join than to walk
+constexpr int64_t kLeastRows = 256;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int64_t padded(const std::vector<int64_t>& n, int64_t tile) {
+    int64_t sum = 0;
+    for (int64_t v : n) sum += ceil_div(v, tile) * tile;
+    return sum;
+}
+
+struct Layout {
+    std::vector<AttnItem> items, key_items;
+    std::vector<AttnJoin> joins, key_joins;
+    int32_t row_tile = 16, key_tile = 64;
+    int32_t num_parts = 0, num_key_parts = 0;
+};
+
+// Units [0, n) of one item in equal parts of about `share`, each but the last a
+// multiple of kPartUnit: the number of parts and the units of one.
+struct Split {
+    int64_t parts, size;
+};
+Split split(int64_t n, int64_t share) {
+    if (2 * n < 3 * share) return {1, n};
+    const int64_t size = ceil_div(ceil_div(n, ceil_div(n, share)), kPartUnit) * kPartUnit;
+    return {ceil_div(n, size), size};
+}
+
+int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group, int64_t kv_heads, Layout& L) {
+    std::vector<int64_t> rows(graphs), keys(graphs);
+    int64_t most_rows = 0;
+    for (int64_t b = 0; b < graphs; ++b) {
+        rows[b] = (qo[b + 1] - qo[b]) * group;
+        keys[b] = ko[b + 1] - ko[b];
+        most_rows = std::max(most_rows, rows[b]);
+        if (rows[b] > RELM_MP_MAX_ROWS)
+            return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: a graph has too many queries");
+    }
+    // Rows of an item.  Up to 32, its waves take different keys and a row's sums meet at
+    // the end; from there on each wave has rows of its own, 16 or 32.  128 rows read a
+    // key tile half as often as 64, unless the lengths leave a fifth more rows empty.
+    if (most_rows <= 16)
+        L.row_tile = 16;
+    else if (most_rows <= 32)
+        L.row_tile = 32;
+    else
+        L.row_tile = 5 * padded(rows, 128) <= 6 * padded(rows, 64) ? 128 : 64;
+    L.key_tile = 5 * padded(keys, 128) <= 6 * padded(keys, 64) ? 128 : 64;
+
+    // A share is what a workgroup gets when all the work is dealt to kWorkgroups.
+    int64_t row_work = 0, key_work = 0;
+    for (int64_t b = 0; b < graphs; ++b) {
+        row_work += ceil_div(rows[b], L.row_tile) * keys[b] * kv_heads;
+        key_work += ceil_div(keys[b], L.key_tile) * rows[b] * kv_heads;
+    }
+    const int64_t key_share = std::max(kLeastKeys, ceil_div(row_work, kWorkgroups));
+    const int64_t row_share = std::max(kLeastRows, ceil_div(key_work, kWorkgroups));
+
+    constexpr size_t kMost = size_t{1} << 24;  // table records: 512 MB
+    for (int64_t b = 0; b < graphs; ++b) {
+        const Split s = split(keys[b], key_share);
+        for (int64_t r = 0; r < rows[b]; r += L.row_tile) {
+            const int32_t n = static_cast<int32_t>(std::min<int64_t>(L.row_tile, rows[b] - r));
+            if (s.parts > 1)
+                L.joins.push_back({static_cast<int32_t>(qo[b]), static_cast<int32_t>(r), n, 0, 0, L.num_parts,
+                                   static_cast<int32_t>(s.parts), 0});
+            for (int64_t p = 0; p < s.parts; ++p)
+                L.items.push_back({static_cast<int32_t>(qo[b]), static_cast<int32_t>(r), n,
+                                   static_cast<int32_t>(ko[b] + p * s.size),
+                                   static_cast<int32_t>(std::min(s.size, keys[b] - p * s.size)),
+                                   s.parts > 1 ? L.num_parts++ : -1, {0, 0}});
+        }
+        const Split t = split(rows[b], row_share);
+        for (int64_t k = 0; k < keys[b]; k += L.key_tile) {
+            const int32_t n = static_cast<int32_t>(std::min<int64_t>(L.key_tile, keys[b] - k));
+            if (t.parts > 1)
+                L.key_joins.push_back({static_cast<int32_t>(qo[b]), 0, 0, static_cast<int32_t>(ko[b] + k), n,
+                                       L.num_key_parts, static_cast<int32_t>(t.parts), 0});
+            for (int64_t p = 0; p < t.parts; ++p)
+                L.key_items.push_back({static_cast<int32_t>(qo[b]), static_cast<int32_t>(p * t.size),
+                                       static_cast<int32_t>(std::min(t.size, rows[b] - p * t.size)),
+                                       static_cast<int32_t>(ko[b] + k), n, t.parts > 1 ? L.num_key_parts++ : -1, {0, 0}});
+        }
+        if (L.items.size() + L.key_items.size() + L.joins.size() + L.key_joins.size() > kMost)
+            return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: too many queries and keys for one plan");
+    }
+    // The longest first, so that none starts when the others end.
+    std::stable_sort(L.items.begin(), L.items.end(), [](const AttnItem& a, const AttnItem& b) { return a.keys > b.keys; });
+    std::stable_sort(L.key_items.begin(), L.key_items.end(),
+                     [](const AttnItem& a, const AttnItem& b) { return a.rows > b.rows; });
+    return RELM_MP_OK;
+}
+
+int check_offsets(const int64_t* o, int64_t graphs, int64_t rows, const char* name) {
+    const auto bad = [&](const char* what) {
+        return set_error(RELM_MP_ERR_INVALID_ARGUMENT, std::string("relm_mp attention plan: ") + name + what);
+    };
+    if (o[0] != 0 || o[graphs] != rows) return bad(" must run from 0 to the number of rows.");
+    for (int64_t b = 0; b < graphs; ++b)
+        if (o[b + 1] < o[b]) return bad(" must ascend.");
+    return RELM_MP_OK;
+}
+
+}  // namespace
+
+int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t q_rows, int64_t k_rows, int32_t heads,
+                         int32_t kv_heads, void* table, size_t table_bytes, relm_mp_attention_plan* plan) {
+    const auto bad = [](const char* what) {
+        return set_error(RELM_MP_ERR_INVALID_ARGUMENT, std::string("relm_mp attention plan: ") + what);
+    };
+    if (plan == nullptr || graphs < 0 || (qo == nullptr) || (ko == nullptr)) return bad("NULL or negative argument");
+    if (heads < 1 || kv_heads < 1 || heads > 4096 || heads % kv_heads != 0)
+        return bad("heads must be a multiple of kv_heads, both in [1, 4096]");
+    if (q_rows < 0 || k_rows < 0 || q_rows > RELM_MP_MAX_ROWS || k_rows > RELM_MP_MAX_ROWS)
+        return bad("rows must be in [0, 2^31 - 2]");
+    int rc = check_offsets(qo, graphs, q_rows, "q_offsets");
+    if (rc == RELM_MP_OK) rc = check_offsets(ko, graphs, k_rows, "k_offsets");
+    if (rc != RELM_MP_OK) return rc;
+    Layout L;
+    rc = lay_out(qo, ko, graphs, heads / kv_heads, kv_heads, L);
+    if (rc != RELM_MP_OK) return rc;
+    const size_t records = L.items.size() + L.joins.size() + L.key_items.size() + L.key_joins.size();
+    relm_mp_attention_plan p{};
+    p.q_rows = q_rows;
+    p.k_rows = k_rows;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.graphs = graphs;
+    p.table_bytes = static_cast<int64_t>(records * sizeof(AttnItem));
+    p.row_tile = L.row_tile;
+    p.key_tile = L.key_tile;
+    p.num_items = static_cast<int32_t>(L.items.size());
+    p.num_parts = L.num_parts;
+    p.num_joins = static_cast<int32_t>(L.joins.size());
+    p.num_key_items = static_cast<int32_t>(L.key_items.size());
+    p.num_key_parts = L.num_key_parts;
+    p.num_key_joins = static_cast<int32_t>(L.key_joins.size());
+    if (static_cast<int64_t>(std::max(L.items.size(), 2 * L.key_items.size())) * kv_heads > 0x7fffffff ||
+        static_cast<int64_t>(std::max(L.joins.size(), L.key_joins.size())) * 128 > 0x7fffffff || kv_heads > 65535)
+        return bad("too many items for one launch");
+    if (table != nullptr) {
+        if (table_bytes < static_cast<size_t>(p.table_bytes))
+            return set_error(RELM_MP_ERR_WORKSPACE, "relm_mp attention plan: table too small");
+        char* at = static_cast<char*>(table);
+        const auto put = [&](const void* from, size_t n) {
+            if (n > 0) std::memcpy(at, from, n * sizeof(AttnItem));
+            at += n * sizeof(AttnItem);
+        };
+        put(L.items.data(), L.items.size());
+        put(L.joins.data(), L.joins.size());
+        put(L.key_items.data(), L.key_items.size());
+        put(L.key_joins.data(), L.key_joins.size());
+    }
+    *plan = p;
+    return RELM_MP_OK;
+}
+
+}  // namespace relm_mp

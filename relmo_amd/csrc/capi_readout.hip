@@ -1,11 +1,14 @@
 // C ABI of the readout ops (include/relm_mp.h): argument checks, then the kernels
-// of norm_kernels.hip.
+// of norm_kernels.hip and attention_kernels.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <exception>
 #include <string>
 
+#include "attention.h"
 #include "internal.h"
 #include "relm_mp.h"
 
@@ -55,6 +58,23 @@ int norm(int dtype, const void* x, const void* r, const void* w, int64_t rows, i
     return RELM_MP_OK;
 }
 
+// The backward's delta first, then the parts of dq or of dk and dv (one after the other
+// in the same memory).
+size_t delta_bytes(const relm_mp_attention_plan& p) {
+    return align_up(static_cast<size_t>(p.q_rows) * p.heads * sizeof(float), 256);
+}
+
+bool null_rows(const relm_mp_head_rows* r) { return r == nullptr || r->data == nullptr; }
+
+int check_attention(int dtype, const relm_mp_attention_plan* plan, int64_t head_dim, float scale) {
+    if (plan == nullptr) return bad("cross_attention: NULL plan");
+    if (!value_dtype(dtype)) return bad("cross_attention: dtype must be f32, bf16 or f16");
+    if (head_dim < 1 || head_dim > RELM_MP_MAX_HEAD_DIM) return bad("cross_attention: head_dim must be in [1, 128]");
+    if (!(scale > 0.0f) || std::isinf(scale)) return bad("cross_attention: scale must be finite and positive");
+    if (plan->table == nullptr && plan->table_bytes > 0) return bad("cross_attention: the plan has no table");
+    return RELM_MP_OK;
+}
+
 }  // namespace
 
 }  // namespace relm_mp
@@ -89,6 +109,88 @@ int relm_mp_add_rms_norm_backward(int dtype, const void* dy, const void* dh, con
     RELM_HIP(launch_add_rms_norm_backward(dtype, dy, dh, h, w, rstd, rows, width, dx, dw, static_cast<float*>(workspace),
                                           static_cast<hipStream_t>(stream)),
              "relm_mp add_rms_norm backward kernels");
+    return RELM_MP_OK;
+}
+
+int relm_mp_attention_plan_build(const int64_t* q_offsets, const int64_t* k_offsets, int64_t graphs, int64_t q_rows,
+                                 int64_t k_rows, int32_t heads, int32_t kv_heads, void* table, size_t table_bytes,
+                                 relm_mp_attention_plan* plan) {
+    try {
+        return build_attention_plan(q_offsets, k_offsets, graphs, q_rows, k_rows, heads, kv_heads, table, table_bytes, plan);
+    } catch (const std::exception& e) {  // host memory
+        return bad(std::string("attention plan: ") + e.what());
+    }
+}
+
+size_t relm_mp_cross_attention_workspace_size(const relm_mp_attention_plan* plan, int64_t head_dim) {
+    return plan == nullptr ? 0 : attention_part_floats(*plan, head_dim) * sizeof(float);
+}
+
+int relm_mp_cross_attention(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* q,
+                            const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim, const uint8_t* key_mask,
+                            float scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                            relm_mp_stream_t stream) {
+    RELM_TRY(check_attention(dtype, plan, head_dim, scale));
+    if (plan->q_rows == 0) return RELM_MP_OK;
+    if (null_rows(q) || out == nullptr || (plan->k_rows > 0 && (null_rows(k) || null_rows(v))))
+        return bad("cross_attention: NULL array");
+    RELM_TRY(check_workspace(workspace, workspace_bytes, relm_mp_cross_attention_workspace_size(plan, head_dim),
+                             "cross_attention"));
+    AttnOperands o{};
+    o.q = *q;
+    if (plan->k_rows > 0) {
+        o.k = *k;
+        o.v = *v;
+    }
+    o.head_dim = head_dim;
+    o.key_mask = key_mask;
+    o.scale = scale;
+    o.out = out;
+    o.lse = lse;
+    o.parts = static_cast<float*>(workspace);
+    RELM_HIP(launch_cross_attention(dtype, *plan, o, static_cast<hipStream_t>(stream)), "relm_mp cross_attention kernel");
+    return RELM_MP_OK;
+}
+
+size_t relm_mp_cross_attention_backward_workspace_size(const relm_mp_attention_plan* plan, int64_t head_dim) {
+    if (plan == nullptr) return 0;
+    return delta_bytes(*plan) +
+           std::max(attention_part_floats(*plan, head_dim), attention_key_part_floats(*plan, head_dim)) * sizeof(float);
+}
+
+int relm_mp_cross_attention_backward(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* grad,
+                                     const relm_mp_head_rows* q, const relm_mp_head_rows* k, const relm_mp_head_rows* v,
+                                     int64_t head_dim, const uint8_t* key_mask, float scale, const void* out, const float* lse,
+                                     void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                     relm_mp_stream_t stream) {
+    RELM_TRY(check_attention(dtype, plan, head_dim, scale));
+    if (plan->q_rows == 0 && plan->k_rows == 0) return RELM_MP_OK;
+    if ((plan->q_rows > 0 && (null_rows(grad) || null_rows(q) || out == nullptr || lse == nullptr || dq == nullptr)) ||
+        (plan->k_rows > 0 && (null_rows(k) || null_rows(v) || dk == nullptr || dv == nullptr)))
+        return bad("cross_attention_backward: NULL array");
+    RELM_TRY(check_workspace(workspace, workspace_bytes, relm_mp_cross_attention_backward_workspace_size(plan, head_dim),
+                             "cross_attention_backward"));
+    AttnOperands o{};
+    if (plan->q_rows > 0) {
+        o.q = *q;
+        o.grad = *grad;
+    }
+    if (plan->k_rows > 0) {
+        o.k = *k;
+        o.v = *v;
+    }
+    o.head_dim = head_dim;
+    o.key_mask = key_mask;
+    o.scale = scale;
+    o.out = const_cast<void*>(out);  // read only
+    o.lse = const_cast<float*>(lse);
+    o.delta = static_cast<float*>(workspace);
+    o.dq = dq;
+    o.dk = dk;
+    o.dv = dv;
+    o.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(*plan));
+    RELM_HIP(launch_cross_attention_backward(dtype, *plan, o, static_cast<hipStream_t>(stream)),
+             "relm_mp cross_attention backward kernels");
     return RELM_MP_OK;
 }
 

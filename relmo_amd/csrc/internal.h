@@ -226,6 +226,14 @@ hipError_t launch_add_rms_norm_backward(int dtype, const void* dy, const void* d
                                         const float* rstd, int64_t rows, int64_t width, void* dx, void* dw, float* partial,
                                         hipStream_t st);
 
+// ---- cross attention (attention_plan.hip, attention_kernels.hip; attention.h) ----
+struct AttnOperands;
+int build_attention_plan(const int64_t* q_offsets, const int64_t* k_offsets, int64_t graphs, int64_t q_rows, int64_t k_rows,
+                         int32_t heads, int32_t kv_heads, void* table, size_t table_bytes, relm_mp_attention_plan* plan);
+hipError_t launch_cross_attention(int dtype, const relm_mp_attention_plan& plan, const AttnOperands& o, hipStream_t st);
+hipError_t launch_cross_attention_backward(int dtype, const relm_mp_attention_plan& plan, const AttnOperands& o,
+                                           hipStream_t st);
+
 // ---- content comparison (match_kernels.hip) -------------------------------
 constexpr int kMaxMatch = RELM_MP_MAX_MATCH;
 // After the launches mismatch[c] == gen iff the snapshot of plans[c] differs

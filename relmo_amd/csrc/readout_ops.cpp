@@ -130,6 +130,143 @@ std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad_y, const std
     return {dx, dw};
 }
 
+// ---- cross attention -------------------------------------------------------------
+
+// A batch's plan with its table on the device.  The table is copied there before the
+// constructor returns, so any stream may use it; a stream other than the one the
+// memory was allocated on is recorded with the allocator.
+struct AttentionPlan : torch::CustomClassHolder {
+    relm_mp_attention_plan plan{};
+    Tensor table;
+    hipStream_t stream = nullptr;
+
+    void used_on(const c10::hip::HIPStream& s) const {
+        if (table.numel() > 0 && s.stream() != stream)
+            c10::hip::HIPCachingAllocator::recordStream(table.storage().data_ptr(), s);
+    }
+};
+
+c10::intrusive_ptr<AttentionPlan> attention_plan(const Tensor& q_offsets, const Tensor& k_offsets, int64_t heads,
+                                                 int64_t kv_heads) {
+    for (const Tensor* t : {&q_offsets, &k_offsets})
+        TORCH_CHECK(t->dim() == 1 && t->scalar_type() == at::kLong && t->is_cuda() && t->numel() >= 1 &&
+                        t->device() == q_offsets.device() && t->numel() == q_offsets.numel(),
+                    "attention_plan: q_offsets and k_offsets must be int64 [graphs + 1] on one GPU.");
+    TORCH_CHECK(heads >= 1 && heads <= 4096 && kv_heads >= 1 && kv_heads <= 4096,
+                "attention_plan: heads and kv_heads must be in [1, 4096].");
+    c10::OptionalDeviceGuard guard(q_offsets.device());
+    const Tensor host = at::stack({q_offsets, k_offsets}).cpu();  // one copy, waited for
+    const int64_t graphs = q_offsets.numel() - 1;
+    const int64_t* qo = host.const_data_ptr<int64_t>();
+    const int64_t* ko = qo + graphs + 1;
+    auto ref = c10::make_intrusive<AttentionPlan>();
+    const auto build = [&](void* table, size_t bytes) {
+        raise_if(relm_mp_attention_plan_build(qo, ko, graphs, qo[graphs], ko[graphs], static_cast<int32_t>(heads),
+                                              static_cast<int32_t>(kv_heads), table, bytes, &ref->plan));
+    };
+    build(nullptr, 0);
+    Tensor table = at::empty({ref->plan.table_bytes}, at::kByte);
+    if (ref->plan.table_bytes > 0) build(table.data_ptr(), static_cast<size_t>(ref->plan.table_bytes));
+    const auto s = c10::hip::getCurrentHIPStream(q_offsets.get_device());
+    ref->table = table.to(q_offsets.device());
+    ref->stream = s.stream();
+    ref->plan.table = ref->plan.table_bytes > 0 ? ref->table.const_data_ptr() : nullptr;
+    return ref;
+}
+
+namespace {
+
+// [rows, heads, dim] with unit strides of the values, or a copy that has them.
+Tensor with_unit_values(const Tensor& t) { return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous(); }
+
+relm_mp_head_rows head_rows(const Tensor& t) { return {t.const_data_ptr(), t.stride(0), t.stride(1)}; }
+
+struct AttnArgs {
+    int dtype;
+    Tensor q, k, v, mask;
+    int64_t dim;
+    float scale;
+    const uint8_t* mask_ptr() const {
+        return mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr;
+    }
+};
+
+AttnArgs attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionPlan& p,
+                        const std::optional<Tensor>& key_mask, double scale, const char* op) {
+    AttnArgs a;
+    a.dtype = value_dtype(q, op, "q");
+    for (const Tensor* t : {&q, &k, &v}) {
+        TORCH_CHECK(t->dim() == 3, op, ": q, k and v must be [rows, heads, head_dim].");
+        check_like(*t, q, op, "k and v");
+    }
+    a.dim = q.size(2);
+    TORCH_CHECK(a.dim >= 1 && a.dim <= RELM_MP_MAX_HEAD_DIM, op, ": head_dim must be in [1, ", RELM_MP_MAX_HEAD_DIM, "].");
+    TORCH_CHECK(q.size(0) == p.plan.q_rows && q.size(1) == p.plan.heads, op, ": q must be [", p.plan.q_rows, ", ",
+                p.plan.heads, ", head_dim] for this plan.");
+    for (const Tensor* t : {&k, &v})
+        TORCH_CHECK(t->size(0) == p.plan.k_rows && t->size(1) == p.plan.kv_heads && t->size(2) == a.dim, op,
+                    ": k and v must be [", p.plan.k_rows, ", ", p.plan.kv_heads, ", ", a.dim, "] for this plan.");
+    TORCH_CHECK(p.table.device() == q.device(), op, ": the plan is on another device.");
+    a.q = with_unit_values(q);
+    a.k = with_unit_values(k);
+    a.v = with_unit_values(v);
+    if (key_mask.has_value() && key_mask->defined()) {
+        TORCH_CHECK(key_mask->dim() == 1 && key_mask->size(0) == p.plan.k_rows && key_mask->scalar_type() == at::kBool &&
+                        key_mask->device() == q.device(),
+                    op, ": key_mask must be bool [", p.plan.k_rows, "] on the device of q.");
+        a.mask = key_mask->contiguous();
+    }
+    a.scale = static_cast<float>(scale);
+    return a;
+}
+
+}  // namespace
+
+// (out, lse); lse is empty unless `keep`.
+std::tuple<Tensor, Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                           const c10::intrusive_ptr<AttentionPlan>& plan,
+                                           const std::optional<Tensor>& key_mask, double scale, bool keep) {
+    const AttnArgs a = attention_args(q, k, v, *plan, key_mask, scale, "cross_attention");
+    c10::OptionalDeviceGuard guard(q.device());
+    plan->used_on(c10::hip::getCurrentHIPStream(q.get_device()));
+    Tensor out = at::empty(q.sizes(), q.options());
+    Tensor lse = keep ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))
+                      : at::empty({0}, q.options().dtype(at::kFloat));
+    const size_t need = relm_mp_cross_attention_workspace_size(&plan->plan, a.dim);
+    const Tensor ws = need > 0 ? bytes(need, q) : Tensor();
+    const relm_mp_head_rows qr = head_rows(a.q), kr = head_rows(a.k), vr = head_rows(a.v);
+    raise_if(relm_mp_cross_attention(a.dtype, &plan->plan, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale, out.data_ptr(),
+                                     keep ? lse.data_ptr<float>() : nullptr, need > 0 ? ws.data_ptr() : nullptr, need,
+                                     current_stream(q)));
+    return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k,
+                                                            const Tensor& v, const c10::intrusive_ptr<AttentionPlan>& plan,
+                                                            const std::optional<Tensor>& key_mask, double scale,
+                                                            const Tensor& out, const Tensor& lse) {
+    const char* op = "cross_attention_backward";
+    const AttnArgs a = attention_args(q, k, v, *plan, key_mask, scale, op);
+    check_same(grad, q, op, "grad");
+    check_same(out, q, op, "out");
+    TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.dim() == 2 &&
+                    lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
+                op, ": lse must be the forward's, float32 [rows, heads].");
+    c10::OptionalDeviceGuard guard(q.device());
+    plan->used_on(c10::hip::getCurrentHIPStream(q.get_device()));
+    const Tensor g = with_unit_values(grad), o = out.contiguous(), l = lse.contiguous();
+    Tensor dq = at::empty(q.sizes(), q.options());
+    Tensor dk = at::empty(k.sizes(), k.options());
+    Tensor dv = at::empty(v.sizes(), v.options());
+    const size_t need = relm_mp_cross_attention_backward_workspace_size(&plan->plan, a.dim);
+    const Tensor ws = bytes(need, q);
+    const relm_mp_head_rows gr = head_rows(g), qr = head_rows(a.q), kr = head_rows(a.k), vr = head_rows(a.v);
+    raise_if(relm_mp_cross_attention_backward(a.dtype, &plan->plan, &gr, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale,
+                                              o.const_data_ptr(), l.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                                              dv.data_ptr(), ws.data_ptr(), need, current_stream(q)));
+    return {dq, dk, dv};
+}
+
 }  // namespace readout
 }  // namespace relm_amd
 
@@ -137,10 +274,17 @@ TORCH_LIBRARY_FRAGMENT(relm_mp, m) {
     m.def("add_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps, bool keep) -> (Tensor, Tensor, Tensor)");
     m.def("add_rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
     m.def("add_rms_norm_backward(Tensor grad_y, Tensor? grad_h, Tensor h, Tensor weight, Tensor rstd) -> (Tensor, Tensor)");
+    m.class_<relm_amd::readout::AttentionPlan>("AttentionPlan");
+    m.def("attention_plan(Tensor q_offsets, Tensor k_offsets, int heads, int kv_heads) -> __torch__.torch.classes.relm_mp.AttentionPlan");
+    m.def("cross_attention(Tensor q, Tensor k, Tensor v, __torch__.torch.classes.relm_mp.AttentionPlan plan, Tensor? key_mask, float scale, bool keep) -> (Tensor, Tensor)");
+    m.def("cross_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, __torch__.torch.classes.relm_mp.AttentionPlan plan, Tensor? key_mask, float scale, Tensor out, Tensor lse) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(relm_mp, CompositeImplicitAutograd, m) {
     m.impl("add_rms_norm", relm_amd::readout::add_rms_norm);
     m.impl("add_rms_norm_fp8", relm_amd::readout::add_rms_norm_fp8);
     m.impl("add_rms_norm_backward", relm_amd::readout::add_rms_norm_backward);
+    m.impl("attention_plan", relm_amd::readout::attention_plan);
+    m.impl("cross_attention", relm_amd::readout::cross_attention);
+    m.impl("cross_attention_backward", relm_amd::readout::cross_attention_backward);
 }

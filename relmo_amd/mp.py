@@ -243,6 +243,47 @@ def add_rms_norm_fp8(
     return _readout.add_rms_norm_fp8(x, residual, weight, float(eps))
 
 
+def attention_plan(
+    q_offsets: torch.Tensor,
+    k_offsets: torch.Tensor,
+    heads: int,
+    kv_heads: int | None = None,
+) -> _readout.AttentionPlan:
+    """The plan of a batch's :func:`cross_attention`: made once from the lengths of its graphs
+    and kept for every layer and step on that batch.
+
+    Graph ``b`` has the queries ``q_offsets[b]:q_offsets[b + 1]`` and the keys
+    ``k_offsets[b]:k_offsets[b + 1]`` (int64 [graphs + 1], from 0, ascending; both may be
+    empty).  ``kv_heads`` (default ``heads``) divides ``heads``: query head ``h`` reads key
+    head ``h // (heads // kv_heads)``.  The offsets are read back and checked here (the one
+    wait for the device) and copied: later writes to them do not change the plan."""
+
+    require_torch("attention_plan")
+    return _readout.attention_plan(q_offsets, k_offsets, heads, kv_heads)
+
+
+def cross_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    plan: _readout.AttentionPlan,
+    key_mask: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Attention of every graph's queries to that graph's keys: ``softmax(scale * q k^T) v``.
+
+    ``q`` [queries, heads, head_dim], ``k`` and ``v`` [keys, kv_heads, head_dim] of one dtype
+    (float32, bfloat16 or float16 on the GPU; head_dim at most 128), in any strides whose
+    last is 1 (others are copied).  ``key_mask`` (bool [keys]) is False for keys that are
+    left out: whatever they hold, NaN included, does not enter.  A query without a key to
+    attend to gets zeros.  ``scale`` (default ``head_dim ** -0.5``) is positive.  Scores,
+    softmax statistics and sums are float32; the gradients of shared key heads add up over
+    their query heads, in a fixed order.  No counterpart in relmo."""
+
+    require_torch("cross_attention")
+    return _readout.cross_attention(q, k, v, plan, key_mask, scale)
+
+
 @contextlib.contextmanager
 def plan_scope():
     """Trust scope for the library's index plans (no counterpart in relmo).
@@ -280,7 +321,9 @@ __all__ = [
     "add_rms_norm",
     "add_rms_norm_fp8",
     "assert_runtime_compat",
+    "attention_plan",
     "available",
+    "cross_attention",
     "fanin_pack_from_edges",
     "fanin_pack_multi",
     "fanin_reduce",

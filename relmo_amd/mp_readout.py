@@ -1,7 +1,8 @@
 """The readout ops of the facade: what a program runs on the object states.
 
-``add_rms_norm`` (a residual stream's norm, also with an 8-bit output) without a
-counterpart in relmo.  GPU tensors of float32, bfloat16 or float16 run the
+``add_rms_norm`` (a residual stream's norm, also with an 8-bit output) and
+``cross_attention`` (per-graph queries to the graphs' objects), without counterparts
+in relmo.  GPU tensors of float32, bfloat16 or float16 run the
 library's kernels through autograd functions; CPU tensors (and the policy's
 fallback) run the ATen formulations below, which autograd differentiates.
 """
@@ -117,4 +118,108 @@ def add_rms_norm_fp8(x, residual, weight, eps: float):
     return q, scale, x if residual is None else h.to(x.dtype)
 
 
-__all__ = ["add_rms_norm", "add_rms_norm_fp8", "rms_norm"]
+# ---- cross attention ---------------------------------------------------------------
+
+
+class AttentionPlan:
+    """The lengths of a batch's graphs and, on the GPU, how their attention is laid over the device."""
+
+    def __init__(self, q_offsets, k_offsets, heads: int, kv_heads: int, ref=None):
+        self.q_offsets, self.k_offsets = q_offsets, k_offsets
+        self.heads, self.kv_heads, self.ref = heads, kv_heads, ref
+
+
+def attention_plan(q_offsets, k_offsets, heads: int, kv_heads: int | None) -> AttentionPlan:
+    heads = int(heads)
+    kv_heads = heads if kv_heads is None else int(kv_heads)
+    if heads < 1 or kv_heads < 1 or heads % kv_heads != 0:
+        raise ValueError("attention_plan expects heads to be a multiple of kv_heads.")
+    for name, t in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
+        if t.dim() != 1 or t.dtype != torch.int64 or t.numel() < 1 or t.numel() != q_offsets.numel():
+            raise ValueError(f"attention_plan expects {name} to be int64 [graphs + 1].")
+    op = library_op("attention_plan", tensor=q_offsets, gpu_only=True)
+    if op is not None:
+        return AttentionPlan(q_offsets, k_offsets, heads, kv_heads, op(q_offsets, k_offsets, heads, kv_heads))
+    for name, t in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
+        if int(t[0]) != 0 or bool((t[1:] < t[:-1]).any()):
+            raise RuntimeError(f"relm_mp attention plan: {name} must ascend from 0.")
+    return AttentionPlan(q_offsets, k_offsets, heads, kv_heads)
+
+
+def _attention_checks(q, k, v, plan, key_mask, scale: float) -> None:
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.size(2) != k.size(2):
+        raise ValueError("cross_attention expects q [queries, heads, head_dim] and k, v [keys, kv_heads, head_dim].")
+    if q.size(1) != plan.heads or k.size(1) != plan.kv_heads:
+        raise ValueError("cross_attention expects the plan's heads and kv_heads.")
+    for name, t in (("k", k), ("v", v)):
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"cross_attention expects {name} to have the dtype and device of q.")
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != k.shape[:1] or key_mask.device != q.device):
+        raise ValueError("cross_attention expects key_mask to be bool [keys] on the device of q.")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("cross_attention expects a finite, positive scale.")
+
+
+def cross_attention_python(q, k, v, plan, key_mask, scale: float):
+    """Graph by graph in ATen, in at least float32: the facade's formulation for CPU tensors."""
+
+    group, dim = plan.heads // plan.kv_heads, q.size(2)
+    wide = torch.promote_types(q.dtype, torch.float32)
+    qo, ko = plan.q_offsets.tolist(), plan.k_offsets.tolist()
+    if qo[-1] != q.size(0) or ko[-1] != k.size(0):
+        raise ValueError("cross_attention expects the plan's numbers of queries and keys.")
+    outs = [q.new_zeros(0, plan.heads, dim, dtype=wide)]
+    for b in range(len(qo) - 1):
+        n = qo[b + 1] - qo[b]
+        qb = q[qo[b]:qo[b + 1]].to(wide).view(n, plan.kv_heads, group, dim).permute(1, 2, 0, 3)
+        kb, vb = (t[ko[b]:ko[b + 1]] for t in (k, v))
+        if key_mask is not None:
+            kept = key_mask[ko[b]:ko[b + 1]]
+            kb, vb = kb[kept], vb[kept]
+        kb, vb = (t.to(wide).permute(1, 0, 2).unsqueeze(1) for t in (kb, vb))
+        if kb.size(2) == 0:
+            outs.append(q.new_zeros(n, plan.heads, dim, dtype=wide))
+            continue
+        p = torch.softmax(qb.matmul(kb.transpose(2, 3)) * scale, 3)
+        outs.append(p.matmul(vb).permute(2, 0, 1, 3).reshape(n, plan.heads, dim))
+    return torch.cat(outs).to(q.dtype)
+
+
+if torch is not None:
+
+    class _CrossAttentionFunction(torch.autograd.Function):
+        """Keeps the inputs, the output and each row's logarithm of its total; the backward
+        computes the probabilities again."""
+
+        @staticmethod
+        def forward(ctx, q, k, v, plan, key_mask, scale):
+            out, lse = ops_namespace().cross_attention(q, k, v, plan, key_mask, scale, True)
+            ctx.plan, ctx.scale = plan, scale
+            ctx.save_for_backward(q, k, v, key_mask, out, lse)
+            return out
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            q, k, v, key_mask, out, lse = ctx.saved_tensors
+            dq, dk, dv = ops_namespace().cross_attention_backward(grad, q, k, v, ctx.plan, key_mask, ctx.scale, out, lse)
+            return dq, dk, dv, None, None, None
+
+else:  # pragma: no cover - torch missing
+    _CrossAttentionFunction = None
+
+
+def cross_attention(q, k, v, plan, key_mask, scale: float | None):
+    scale = q.size(-1) ** -0.5 if scale is None and q.size(-1) else float(1.0 if scale is None else scale)
+    _attention_checks(q, k, v, plan, key_mask, scale)
+    op = library_op("cross_attention", tensor=q, gpu_only=True)
+    if op is None:
+        return cross_attention_python(q, k, v, plan, key_mask, scale)
+    if plan.ref is None:
+        raise ValueError("cross_attention expects a plan made from offsets on the GPU.")
+    if _wants_grad(q, k, v):
+        return _CrossAttentionFunction.apply(q, k, v, plan.ref, key_mask, scale)
+    return op(q, k, v, plan.ref, key_mask, scale, False)[0]
+
+
+__all__ = ["AttentionPlan", "add_rms_norm", "add_rms_norm_fp8", "attention_plan", "cross_attention", "rms_norm"]
