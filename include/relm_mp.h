@@ -608,6 +608,27 @@ int relm_mp_cross_attention_backward(int dtype, const relm_mp_attention_plan* pl
                                      const void* out, const float* lse, void* dq, void* dk, void* dv,
                                      void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
 
+/* ---- orthogonalised update ----------------------------------------------------
+ * Per matrix: X = in / (|in|_F + eps), then `steps` times A = X X^T, X <- a X + (b A + c
+ * A A) X (on the shorter side), out = X.  Iterates are held in 22 bits and sums in float
+ * whatever dtype is; the result is rounded once.  The polynomial a x + b x^3 + c x^5 must
+ * keep [0, 1] within [-2, 2] over the steps (checked), which bounds every iterate. */
+typedef struct relm_mp_update {
+    const void* in;     /* rows x cols, neighbouring columns side by side */
+    void* out;          /* rows x cols, contiguous; may not overlap an input */
+    int64_t rows;
+    int64_t cols;
+    int64_t row_stride; /* of `in`, in values */
+} relm_mp_update;
+
+#define RELM_MP_MAX_ORTHO_STEPS 64
+#define RELM_MP_MAX_ORTHO_SIDE 65536
+
+/* updates: `count` host descriptors.  workspace: *_workspace_size bytes, 256-byte aligned. */
+size_t relm_mp_orthogonalise_workspace_size(const relm_mp_update* updates, int32_t count);
+int relm_mp_orthogonalise(int dtype, const relm_mp_update* updates, int32_t count, int32_t steps, float a, float b,
+                          float c, float eps, void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

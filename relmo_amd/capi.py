@@ -82,6 +82,8 @@ EXPORTED_SYMBOLS = (
     "relm_mp_cross_attention",
     "relm_mp_cross_attention_backward_workspace_size",
     "relm_mp_cross_attention_backward",
+    "relm_mp_orthogonalise_workspace_size",
+    "relm_mp_orthogonalise",
 )
 
 
@@ -162,6 +164,18 @@ class HeadRows(ctypes.Structure):
     """Mirror of ``struct relm_mp_head_rows``."""
 
     _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Update(ctypes.Structure):
+    """Mirror of ``struct relm_mp_update``."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p),  # `in` of the header
+        ("out", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+    ]
 
 
 _i64 = ctypes.c_int64
@@ -245,6 +259,9 @@ _SIGNATURES = {
     "relm_mp_cross_attention_backward_workspace_size": (_sz, [_AP, _i64]),
     "relm_mp_cross_attention_backward": (
         _int, [_int, _AP, _HR, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "relm_mp_orthogonalise_workspace_size": (_sz, [ctypes.POINTER(Update), ctypes.c_int32]),
+    "relm_mp_orthogonalise": (
+        _int, [_int, ctypes.POINTER(Update), ctypes.c_int32, ctypes.c_int32, _f32, _f32, _f32, _f32, _vp, _sz, _vp]),
     "relm_mp_plan_match": (
         _int,
         [_vp, _vp, _i64, ctypes.POINTER(_PP), ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), _vp,

@@ -27,7 +27,7 @@ ARCH = os.environ.get("RELM_MP_OFFLOAD_ARCH", "gfx950")
 
 HIP_SOURCES = ["plan_kernels.hip", "small_plan_kernels.hip", "reduce_kernels.hip", "pack_kernels.hip", "match_kernels.hip",
                "film_kernels.hip", "norm_kernels.hip",
-               "attention_plan.hip", "attention_kernels.hip",
+               "attention_plan.hip", "attention_kernels.hip", "orthogonal_kernels.hip",
                "capi.hip", "capi_readout.hip"]
 TORCH_SOURCES = ["relm_mp_ops.cpp", "readout_ops.cpp"]
 HIP_LIB = PKG_DIR / "librelm_mp_hip.so"

@@ -1,5 +1,5 @@
 // C ABI of the readout ops (include/relm_mp.h): argument checks, then the kernels
-// of norm_kernels.hip and attention_kernels.hip.
+// of norm_kernels.hip, attention_kernels.hip and orthogonal_kernels.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -10,6 +10,7 @@
 
 #include "attention.h"
 #include "internal.h"
+#include "orthogonal.h"
 #include "relm_mp.h"
 
 namespace relm_mp {
@@ -72,6 +73,39 @@ int check_attention(int dtype, const relm_mp_attention_plan* plan, int64_t head_
     if (head_dim < 1 || head_dim > RELM_MP_MAX_HEAD_DIM) return bad("cross_attention: head_dim must be in [1, 128]");
     if (!(scale > 0.0f) || std::isinf(scale)) return bad("cross_attention: scale must be finite and positive");
     if (plan->table == nullptr && plan->table_bytes > 0) return bad("cross_attention: the plan has no table");
+    return RELM_MP_OK;
+}
+
+// The rule of a polynomial, with the scales that its values need; an error where the
+// iteration leaves [-2, 2] (seen on a grid of starting values).
+int ortho_rule(int32_t steps, float a, float b, float c, float eps, OrthoRule* rule) {
+    if (steps < 1 || steps > RELM_MP_MAX_ORTHO_STEPS) return bad("orthogonalise: steps must be in [1, 64]");
+    if (!(eps >= 0.0f) || std::isinf(eps)) return bad("orthogonalise: eps must be finite and not negative");
+    double most_b = 1e-3;
+    for (int i = 0; i <= 1024; ++i) {
+        double x = i / 1024.0;
+        for (int32_t s = 0; s < steps; ++s) {
+            const double factor = b * x * x + c * x * x * x * x;
+            most_b = std::max(most_b, std::fabs(factor));
+            x = (a + factor) * x;
+            if (!(std::fabs(x) <= 2.0))
+                return bad("orthogonalise: these coefficients take singular values past 2");
+        }
+    }
+    *rule = OrthoRule{a, b, c, eps, 4096.0f, std::ldexp(1.0f, std::max(-10, std::min(13, std::ilogb(30000.0 / most_b)))), steps};
+    return RELM_MP_OK;
+}
+
+int check_updates(const relm_mp_update* updates, int32_t count) {
+    if (count < 0 || (count > 0 && updates == nullptr)) return bad("orthogonalise: NULL or negative argument");
+    for (int32_t i = 0; i < count; ++i) {
+        const relm_mp_update& u = updates[i];
+        if (u.rows < 0 || u.cols < 0 || u.rows > RELM_MP_MAX_ORTHO_SIDE || u.cols > RELM_MP_MAX_ORTHO_SIDE)
+            return bad("orthogonalise: rows and columns must be in [0, 65536]");
+        if (u.rows == 0 || u.cols == 0) continue;
+        if (u.in == nullptr || u.out == nullptr) return bad("orthogonalise: NULL array");
+        if (u.rows > 1 && u.row_stride < u.cols) return bad("orthogonalise: rows overlap");
+    }
     return RELM_MP_OK;
 }
 
@@ -191,6 +225,27 @@ int relm_mp_cross_attention_backward(int dtype, const relm_mp_attention_plan* pl
     o.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(*plan));
     RELM_HIP(launch_cross_attention_backward(dtype, *plan, o, static_cast<hipStream_t>(stream)),
              "relm_mp cross_attention backward kernels");
+    return RELM_MP_OK;
+}
+
+size_t relm_mp_orthogonalise_workspace_size(const relm_mp_update* updates, int32_t count) {
+    if (check_updates(updates, count) != RELM_MP_OK) return 0;
+    return orthogonalise_workspace(updates, count);
+}
+
+int relm_mp_orthogonalise(int dtype, const relm_mp_update* updates, int32_t count, int32_t steps, float a, float b, float c,
+                          float eps, void* workspace, size_t workspace_bytes, relm_mp_stream_t stream) {
+    if (!value_dtype(dtype)) return bad("orthogonalise: dtype must be f32, bf16 or f16");
+    OrthoRule rule;
+    RELM_TRY(ortho_rule(steps, a, b, c, eps, &rule));
+    RELM_TRY(check_updates(updates, count));
+    RELM_TRY(check_workspace(workspace, workspace_bytes, orthogonalise_workspace(updates, count), "orthogonalise"));
+    try {
+        RELM_HIP(launch_orthogonalise(dtype, updates, count, rule, workspace, static_cast<hipStream_t>(stream)),
+                 "relm_mp orthogonalise kernels");
+    } catch (const std::exception& e) {  // host memory
+        return bad(std::string("orthogonalise: ") + e.what());
+    }
     return RELM_MP_OK;
 }
 

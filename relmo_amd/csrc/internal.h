@@ -234,6 +234,12 @@ hipError_t launch_cross_attention(int dtype, const relm_mp_attention_plan& plan,
 hipError_t launch_cross_attention_backward(int dtype, const relm_mp_attention_plan& plan, const AttnOperands& o,
                                            hipStream_t st);
 
+// ---- orthogonalised update (orthogonal_kernels.hip; orthogonal.h) --------------
+struct OrthoRule;
+size_t orthogonalise_workspace(const relm_mp_update* updates, int32_t count);
+hipError_t launch_orthogonalise(int dtype, const relm_mp_update* updates, int32_t count, const OrthoRule& rule, void* ws,
+                                hipStream_t st);
+
 // ---- content comparison (match_kernels.hip) -------------------------------
 constexpr int kMaxMatch = RELM_MP_MAX_MATCH;
 // After the launches mismatch[c] == gen iff the snapshot of plans[c] differs

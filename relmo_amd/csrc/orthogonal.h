@@ -1,0 +1,34 @@
+// What the orthogonalised update's kernels and entry point share.
+#pragma once
+
+#include <cstdint>
+
+#include "relm_mp.h"
+
+namespace relm_mp {
+
+// One update, turned so that m <= n; mp and np are m and n rounded up to 32.
+struct OrthoMatrix {
+    const void* in;
+    void* out;
+    int64_t in_stride;
+    int32_t m, n, mp, np;
+    int32_t tall;      // the update is [n, m]
+    float scale;       // of X's pairs: a power of two
+    int64_t first_tile[2];  // of the symmetric products' and the update's tiles
+    int64_t x, xt[2], a, b, partial;  // bytes into the workspace
+};
+
+// Descriptors travel as kernel arguments (at most 4 KB).
+constexpr int kOrthoBatch = 32;
+constexpr int kNormParts = 256;  // partial sums of squares of a matrix: a wave adds them
+// Lower tiles of 128 x 128 from which on they are taken instead of 64 x 64 ones.
+constexpr int64_t kLargeTiles = 100;
+
+struct OrthoRule {
+    float a, b, c, eps;
+    float scale_a, scale_b;  // of A's and B's pairs: powers of two
+    int32_t steps;
+};
+
+}  // namespace relm_mp

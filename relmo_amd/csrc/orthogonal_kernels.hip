@@ -1,0 +1,640 @@
+// Orthogonalised update by Newton-Schulz products: X = G / (|G|_F + eps), then `steps` times
+//
+//   A = X X^T,   B = b A + c A A,   X <- a X + B X
+//
+// on the shorter side (a taller G is read and written transposed), which drives the
+// singular values towards 1 and keeps the singular vectors.
+//
+// Arithmetic.  The iteration multiplies small singular values by about a per step, and the
+// rounding of what it multiplies with them, so 11 or 8 bits are too few for the iterates.
+// Every iterate is held as two halves, x = hi + lo with hi = half(x), lo = half(x - hi):
+// 22 bits, at scales (powers of two, exact) that keep the halves within their normal
+// range.  A product of two such matrices is three matrix-instruction products, hi hi + hi
+// lo + lo hi, added in float: about float's own accuracy at a third of the 16-bit rate,
+// five times the float instructions' rate.  The Frobenius norm is added in double.
+//
+// A and B are symmetric: of A X^T-like products only the lower tiles are computed and
+// written twice, and both operands of every product are read along their rows.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "device_utils.h"
+#include "internal.h"
+#include "mfma_tiles.h"
+#include "orthogonal.h"
+#include "value_types.h"
+
+namespace relm_mp {
+
+namespace {
+
+using Half8 = Frag<f16>;
+using Half4 = f16 __attribute__((ext_vector_type(4)));
+
+struct Pair {
+    f16 hi, lo;
+};
+__device__ __forceinline__ Pair halves(float x) {
+    const f16 hi = static_cast<f16>(x);
+    return {hi, static_cast<f16>(x - static_cast<float>(hi))};
+}
+__device__ __forceinline__ float whole(f16 hi, f16 lo) { return static_cast<float>(hi) + static_cast<float>(lo); }
+
+// One product of pairs; the small terms first.
+__device__ __forceinline__ f32x4 mma_pairs(Half8 ah, Half8 al, Half8 bh, Half8 bl, f32x4 c) {
+    c = mma<f16>(al, bh, c);
+    c = mma<f16>(ah, bl, c);
+    return mma<f16>(ah, bh, c);
+}
+
+// The contraction values row 4 g + j and 16 + 4 g + j of lds_frag_t, along a row.
+__device__ __forceinline__ Half8 lds_frag_split(const f16* tile, int stride, int row, int col) {
+    const int g = lane_id() / 16;
+    const Half4 a = *reinterpret_cast<const Half4*>(tile + row * stride + col + 4 * g);
+    const Half4 b = *reinterpret_cast<const Half4*>(tile + row * stride + col + 16 + 4 * g);
+    return Half8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// Entry (i, j) of X, the update turned so that it is at least as wide as tall.
+template <typename T>
+__device__ __forceinline__ float entry(const OrthoMatrix& d, int i, int j) {
+    const T* in = static_cast<const T*>(d.in);
+    return static_cast<float>(d.tall ? in[static_cast<int64_t>(j) * d.in_stride + i]
+                                     : in[static_cast<int64_t>(i) * d.in_stride + j]);
+}
+template <typename T>
+__device__ __forceinline__ void put_entry(const OrthoMatrix& d, int i, int j, float x) {
+    T* out = static_cast<T*>(d.out);
+    out[d.tall ? static_cast<int64_t>(j) * d.m + i : static_cast<int64_t>(i) * d.n + j] = round_to<T>(x);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = kWave / 2; o > 0; o /= 2) v += __shfl_xor(v, o);
+    return v;
+}
+
+// ---- one workgroup per matrix, everything in LDS ------------------------------------------
+
+constexpr int kSmallThreads = 512;
+constexpr int kSmallWaves = kSmallThreads / kWave;
+constexpr int kSmallBlocks = 2;  // 32 x 32 blocks of A that a wave keeps: 10 lower blocks of 128 rows on 8 waves
+
+struct OrthoBatch {
+    OrthoMatrix mat[kOrthoBatch];
+};
+
+// Latency bound (a product of 96 x 96 is 27 matrix instructions to a wave): few barriers
+// (4 a step), operands from LDS in blocks of 32 x 32, a step's A kept in the registers
+// of the wave that computed it.
+template <typename T>
+__global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch, OrthoRule rule) {
+    extern __shared__ __align__(16) f16 pool[];
+    __shared__ double partial[kSmallWaves];
+    const OrthoMatrix& d = batch.mat[blockIdx.x];
+    const int m = d.m, n = d.n, mp = d.mp, np = d.np;
+    const int sx = np + 8, sa = mp + 8;  // strides: rows spread over the banks
+    f16 *xh = pool, *xl = xh + mp * sx, *ah = xl + mp * sx, *al = ah + mp * sa;
+    const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave, l = lane_id(), g = l / 16, c16 = l % 16;
+
+    double sum = 0.0;
+    for (int u = tid; u < m * n; u += kSmallThreads) {
+        // along the rows of the update as it lies in memory
+        const int i = d.tall ? u % m : u / n, j = d.tall ? u / m : u % n;
+        const float x = entry<T>(d, i, j);
+        sum += static_cast<double>(x) * static_cast<double>(x);
+    }
+    sum = wave_sum(sum);
+    if (l == 0) partial[wave] = sum;
+    __syncthreads();
+    sum = partial[0];
+#pragma unroll
+    for (int v = 1; v < kSmallWaves; ++v) sum += partial[v];
+    const float scale = static_cast<float>(static_cast<double>(d.scale) / (sqrt(sum) + static_cast<double>(rule.eps)));
+    for (int u = tid; u < mp * np; u += kSmallThreads) {
+        const int i = d.tall ? u % mp : u / np, j = d.tall ? u / mp : u % np;
+        const Pair p = halves(i < m && j < n ? entry<T>(d, i, j) * scale : 0.0f);
+        xh[i * sx + j] = p.hi;
+        xl[i * sx + j] = p.lo;
+    }
+    __syncthreads();
+
+    const int blocks = mp / 32, lower = blocks * (blocks + 1) / 2;
+    const float to_a = rule.scale_a / (d.scale * d.scale), from_b = 1.0f / rule.scale_b;
+    const float b_of_a = rule.b * rule.scale_b / rule.scale_a, b_of_aa = rule.c * rule.scale_b / (rule.scale_a * rule.scale_a);
+    for (int step = 0; step < rule.steps; ++step) {
+        // A, the lower blocks; then A A over the same blocks
+        f32x4 a[kSmallBlocks][2][2];
+        auto product = [&](const f16* ph, const f16* pl, int stride, int depth, int r0, int c0, f32x4 (&acc)[2][2]) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) acc[r][c] = f32x4(0.0f);
+            for (int k = 0; k < depth; k += 32) {
+                Half8 fh[2], fl[2], gh[2], gl[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    fh[r] = lds_frag<f16>(ph, stride, r0 + 16 * r + c16, k + 8 * g);
+                    fl[r] = lds_frag<f16>(pl, stride, r0 + 16 * r + c16, k + 8 * g);
+                    gh[r] = lds_frag<f16>(ph, stride, c0 + 16 * r + c16, k + 8 * g);
+                    gl[r] = lds_frag<f16>(pl, stride, c0 + 16 * r + c16, k + 8 * g);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) acc[r][c] = mma_pairs(fh[r], fl[r], gh[c], gl[c], acc[r][c]);
+            }
+        };
+        auto place = [&](int q, int& r0, int& c0) {  // block q of the lower triangle, row by row
+            int r = 0;
+            while ((r + 1) * (r + 2) / 2 <= q) ++r;
+            r0 = 32 * r;
+            c0 = 32 * (q - r * (r + 1) / 2);
+        };
+        auto put = [&](int r0, int c0, const f32x4 (&v)[2][2]) {  // a block and its mirror image
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    Half4 hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Pair p = halves(v[r][c][i]);
+                        const int row = r0 + 16 * r + 4 * g + i, col = c0 + 16 * c + c16;
+                        hi[i] = p.hi;
+                        lo[i] = p.lo;
+                        if (r0 != c0) {
+                            ah[row * sa + col] = p.hi;
+                            al[row * sa + col] = p.lo;
+                        }
+                    }
+                    const int at = (c0 + 16 * c + c16) * sa + r0 + 16 * r + 4 * g;
+                    *reinterpret_cast<Half4*>(ah + at) = hi;
+                    *reinterpret_cast<Half4*>(al + at) = lo;
+                }
+        };
+#pragma unroll
+        for (int q = 0; q < kSmallBlocks; ++q) {
+            const int block = wave + q * kSmallWaves;
+            if (block >= lower) break;
+            int r0, c0;
+            place(block, r0, c0);
+            product(xh, xl, sx, np, r0, c0, a[q]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) a[q][r][c] *= to_a;
+            put(r0, c0, a[q]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < kSmallBlocks; ++q) {
+            const int block = wave + q * kSmallWaves;
+            if (block >= lower) break;
+            int r0, c0;
+            place(block, r0, c0);
+            f32x4 aa[2][2];
+            product(ah, al, sa, mp, r0, c0, aa);
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) a[q][r][c] = a[q][r][c] * b_of_a + aa[r][c] * b_of_aa;
+        }
+        __syncthreads();  // A has been read: B takes its place
+#pragma unroll
+        for (int q = 0; q < kSmallBlocks; ++q) {
+            const int block = wave + q * kSmallWaves;
+            if (block >= lower) break;
+            int r0, c0;
+            place(block, r0, c0);
+            put(r0, c0, a[q]);
+        }
+        __syncthreads();
+        // X <- a X + B X: 16 columns of X depend on themselves and B alone, so each is one
+        // wave's, in place
+        for (int strip = wave; strip < np / 16; strip += kSmallWaves) {
+            Half8 fh[4], fl[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < blocks) {
+                    fh[k] = lds_frag_t<f16>(xh, sx, 32 * k, 16 * strip);
+                    fl[k] = lds_frag_t<f16>(xl, sx, 32 * k, 16 * strip);
+                }
+            const bool last = step + 1 == rule.steps;
+            for (int r = 0; r < mp / 16; ++r) {
+                f32x4 acc = f32x4(0.0f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k < blocks)
+                        acc = mma_pairs(lds_frag_split(ah, sa, 16 * r + c16, 32 * k), lds_frag_split(al, sa, 16 * r + c16, 32 * k),
+                                        fh[k], fl[k], acc);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 16 * r + 4 * g + i, col = 16 * strip + c16, at = row * sx + col;
+                    const float x = fmaf(rule.a, whole(xh[at], xl[at]), acc[i] * from_b);
+                    if (!last) {
+                        const Pair p = halves(x);
+                        xh[at] = p.hi;
+                        xl[at] = p.lo;
+                    } else if (row < m && col < n) {
+                        put_entry<T>(d, row, col, x / d.scale);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- larger matrices: tiles of all matrices of a launch -------------------------------------
+
+constexpr int kThreads = 256;
+
+// Partial sums of squares, kNormParts to a matrix.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ortho_norm(OrthoBatch batch, void* ws) {
+    __shared__ double lds[kThreads / kWave];
+    const OrthoMatrix& d = batch.mat[blockIdx.y];
+    const int64_t rows = d.tall ? d.n : d.m;
+    const int cols = d.tall ? d.m : d.n;
+    const int wave = static_cast<int>(threadIdx.x) / kWave;
+    double sum = 0.0;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + wave; r < rows;
+         r += kNormParts * (kThreads / kWave)) {
+        const T* in = static_cast<const T*>(d.in) + r * d.in_stride;
+        for (int c = lane_id(); c < cols; c += kWave) {
+            const double x = static_cast<double>(static_cast<float>(in[c]));
+            sum = fma(x, x, sum);
+        }
+    }
+    sum = wave_sum(sum);
+    if (lane_id() == 0) lds[threadIdx.x / kWave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int v = 1; v < kThreads / kWave; ++v) sum += lds[v];
+        reinterpret_cast<double*>(static_cast<char*>(ws) + d.partial)[blockIdx.x] = sum;
+    }
+}
+
+// Planes of a matrix in the workspace: hi, then lo, row-major over a padded width (zeros).
+struct Planes {
+    f16* hi;
+    f16* lo;
+    int64_t stride;
+};
+__device__ __forceinline__ Planes planes(void* ws, int64_t at, int64_t rows, int64_t stride) {
+    f16* hi = reinterpret_cast<f16*>(static_cast<char*>(ws) + at);
+    return {hi, hi + rows * stride, stride};
+}
+__device__ __forceinline__ Planes planes_x(void* ws, const OrthoMatrix& d) { return planes(ws, d.x, d.m, d.np); }
+__device__ __forceinline__ Planes planes_xt(void* ws, const OrthoMatrix& d, int which) {
+    return planes(ws, d.xt[which], d.n, d.mp);
+}
+__device__ __forceinline__ Planes planes_a(void* ws, const OrthoMatrix& d) { return planes(ws, d.a, d.m, d.mp); }
+__device__ __forceinline__ Planes planes_b(void* ws, const OrthoMatrix& d) { return planes(ws, d.b, d.m, d.mp); }
+
+// X and its transpose as pairs, 32 x 32 entries to a workgroup; the padding of every plane.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ortho_split(OrthoBatch batch, OrthoRule rule, void* ws) {
+    __shared__ float tile[32][33];
+    __shared__ double total;
+    const OrthoMatrix& d = batch.mat[blockIdx.z];
+    const int i0 = static_cast<int>(blockIdx.y) * 32, j0 = static_cast<int>(blockIdx.x) * 32;
+    if (i0 >= d.mp || j0 >= d.np) return;
+    const int tx = static_cast<int>(threadIdx.x) % 32, ty = static_cast<int>(threadIdx.x) / 32;
+    if (threadIdx.x < kWave) {
+        const double* part = reinterpret_cast<const double*>(static_cast<const char*>(ws) + d.partial);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kNormParts / kWave; ++i) sum += part[i * kWave + threadIdx.x];
+        sum = wave_sum(sum);
+        if (threadIdx.x == 0) total = sum;
+    }
+    for (int r = ty; r < 32; r += kThreads / 32) {  // along the update's rows
+        const int i = d.tall ? i0 + tx : i0 + r, j = d.tall ? j0 + r : j0 + tx;
+        const float x = i < d.m && j < d.n ? entry<T>(d, i, j) : 0.0f;
+        if (d.tall)
+            tile[tx][r] = x;
+        else
+            tile[r][tx] = x;
+    }
+    __syncthreads();
+    const float scale = static_cast<float>(static_cast<double>(d.scale) / (sqrt(total) + static_cast<double>(rule.eps)));
+    const Planes x = planes_x(ws, d), xt = planes_xt(ws, d, 0), xt1 = planes_xt(ws, d, 1), a = planes_a(ws, d),
+                 b = planes_b(ws, d);
+    for (int r = ty; r < 32; r += kThreads / 32) {
+        if (i0 + r < d.m) {
+            const Pair p = halves(tile[r][tx] * scale);
+            const int64_t at = (i0 + r) * x.stride + j0 + tx;
+            x.hi[at] = p.hi;
+            x.lo[at] = p.lo;
+        }
+        if (j0 + r < d.n) {
+            const Pair p = halves(tile[tx][r] * scale);
+            const int64_t at = (j0 + r) * xt.stride + i0 + tx;
+            xt.hi[at] = p.hi;
+            xt.lo[at] = p.lo;
+            if (i0 + tx >= d.m) xt1.hi[at] = xt1.lo[at] = static_cast<f16>(0.0f);
+        }
+    }
+    // the columns past m of A and B: the workgroups of the last 32 columns of row block
+    // 0 of X hold i0 = 0 only, so each workgroup of column 0 takes its 32 rows
+    if (j0 == 0 && d.mp > d.m)
+        for (int u = static_cast<int>(threadIdx.x); u < 32 * (d.mp - d.m); u += kThreads) {
+            const int row = i0 + u / (d.mp - d.m), col = d.m + u % (d.mp - d.m);
+            if (row < d.m) {
+                const int64_t at = row * a.stride + col;
+                a.hi[at] = a.lo[at] = b.hi[at] = b.lo[at] = static_cast<f16>(0.0f);
+            }
+        }
+}
+
+enum Product { kGram, kSquare, kUpdate };
+
+// A tile of one of the three products of a step: BT x BT entries, 4 waves of (BT / 2)^2,
+// depth 32 at a time through two LDS buffers while the next is on its way in registers.
+// Bound by the matrix instructions: per depth of 32 a wave of the 128-tile runs 48 of
+// them (768 cycles) for 16 LDS reads of 1 KB.
+template <typename T, int PRODUCT, int BT>
+__global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
+    constexpr int MT = BT / 32, ST = 40;  // row of 32 halves and 16 bytes
+    constexpr int kUnits = BT * 4 * 2 * 2 / kThreads;  // 16-byte units of a thread: rows x 4 x planes x operands
+    __shared__ __align__(16) f16 lds[2][2][2][BT * ST];  // [buffer][operand][plane]
+    // the tile's matrix
+    const int64_t flat = xcd_tile(blockIdx.x, gridDim.x);
+    int which = 0;
+    const int first_of = PRODUCT == kUpdate ? 1 : 0;
+    while (which + 1 < count && flat >= batch.mat[which + 1].first_tile[first_of]) ++which;
+    const OrthoMatrix& d = batch.mat[which];
+    const int t = static_cast<int>(flat - d.first_tile[first_of]);
+    int ti, tj;
+    if constexpr (PRODUCT == kUpdate) {
+        const int rows = (d.m + BT - 1) / BT;
+        ti = t % rows;
+        tj = t / rows;
+    } else {  // the lower triangle, row by row
+        ti = static_cast<int>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        while (ti * (ti + 1) / 2 > t) --ti;
+        tj = t - ti * (ti + 1) / 2;
+    }
+    const Planes a = planes_a(ws, d), b = planes_b(ws, d);
+    const Planes xt = planes_xt(ws, d, step & 1);
+    Planes p, q;
+    int depth, q_rows;
+    if constexpr (PRODUCT == kGram) {
+        p = q = planes_x(ws, d);
+        depth = d.np;
+        q_rows = d.m;
+    } else if constexpr (PRODUCT == kSquare) {
+        p = q = a;
+        depth = d.mp;
+        q_rows = d.m;
+    } else {
+        p = b;
+        q = xt;
+        depth = d.mp;
+        q_rows = d.n;
+    }
+    const int r0 = ti * BT, c0 = tj * BT;
+    const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave, l = lane_id(), g = l / 16, c16 = l % 16;
+    const int wr = (wave / 2) * (BT / 2), wc = (wave % 2) * (BT / 2);
+
+    // unit u of the thread: row u / 4 of an operand's plane, values 8 (u % 4) .. + 8
+    const f16* from[kUnits];
+    int to[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int u = i * kThreads + tid;
+        const int row = (u / 4) % BT, col = (u % 4) * 8, plane = (u / (4 * BT)) % 2, operand = u / (8 * BT);
+        const Planes& o = operand == 0 ? p : q;
+        // rows past the matrix read its last one: their results are not stored
+        const int64_t src = operand == 0 ? min(r0 + row, d.m - 1) : min(c0 + row, q_rows - 1);
+        from[i] = (plane == 0 ? o.hi : o.lo) + src * o.stride + col;
+        to[i] = (operand * 2 + plane) * (BT * ST) + row * ST + col;
+    }
+    Half8 next[kUnits];
+    auto fetch = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) next[i] = *reinterpret_cast<const Half8*>(from[i] + k);
+    };
+    auto settle = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) *reinterpret_cast<Half8*>(&lds[buffer][0][0][0] + to[i]) = next[i];
+    };
+    f32x4 acc[MT][MT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int c = 0; c < MT; ++c) acc[r][c] = f32x4(0.0f);
+    fetch(0);
+    settle(0);
+    __syncthreads();
+    for (int k = 0; k < depth; k += 32) {
+        const int buffer = (k / 32) & 1;
+        if (k + 32 < depth) fetch(k + 32);
+        Half8 fh[MT], fl[MT], gh[MT], gl[MT];
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+            fh[r] = lds_frag<f16>(lds[buffer][0][0], ST, wr + 16 * r + c16, 8 * g);
+            fl[r] = lds_frag<f16>(lds[buffer][0][1], ST, wr + 16 * r + c16, 8 * g);
+            gh[r] = lds_frag<f16>(lds[buffer][1][0], ST, wc + 16 * r + c16, 8 * g);
+            gl[r] = lds_frag<f16>(lds[buffer][1][1], ST, wc + 16 * r + c16, 8 * g);
+        }
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+            for (int c = 0; c < MT; ++c) acc[r][c] = mma_pairs(fh[r], fl[r], gh[c], gl[c], acc[r][c]);
+        if (k + 32 < depth) settle(buffer ^ 1);
+        __syncthreads();
+    }
+
+    const float to_a = rule.scale_a / (d.scale * d.scale), from_b = 1.0f / rule.scale_b;
+    const float b_of_a = rule.b * rule.scale_b / rule.scale_a, b_of_aa = rule.c * rule.scale_b / (rule.scale_a * rule.scale_a);
+    const Planes x = planes_x(ws, d), xt_new = planes_xt(ws, d, (step & 1) ^ 1);
+    const bool last = step + 1 == rule.steps;
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int c = 0; c < MT; ++c) {
+            // entries (row0 .. row0 + 3, col)
+            const int row0 = r0 + wr + 16 * r + 4 * g, col = c0 + wc + 16 * c + c16;
+            if (row0 >= d.m || col >= q_rows) continue;
+            f32x4 v = acc[r][c];
+            if constexpr (PRODUCT == kGram) {
+                v *= to_a;
+            } else {
+                const Planes& old = PRODUCT == kSquare ? a : xt;  // A is symmetric
+                const Half4 oh = *reinterpret_cast<const Half4*>(old.hi + col * old.stride + row0);
+                const Half4 ol = *reinterpret_cast<const Half4*>(old.lo + col * old.stride + row0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (PRODUCT == kSquare)
+                        v[i] = whole(oh[i], ol[i]) * b_of_a + v[i] * b_of_aa;
+                    else
+                        v[i] = fmaf(rule.a, whole(oh[i], ol[i]), v[i] * from_b);
+                }
+            }
+            if constexpr (PRODUCT == kUpdate) {
+                if (last) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (row0 + i < d.m) put_entry<T>(d, row0 + i, col, v[i] / d.scale);
+                    continue;
+                }
+            }
+            const Planes& direct = PRODUCT == kGram ? a : PRODUCT == kSquare ? b : x;
+            const Planes& turned = PRODUCT == kGram ? a : PRODUCT == kSquare ? b : xt_new;
+            Half4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const Pair pr = row0 + i < d.m ? halves(v[i]) : Pair{static_cast<f16>(0.0f), static_cast<f16>(0.0f)};
+                hi[i] = pr.hi;
+                lo[i] = pr.lo;
+                // a tile on the diagonal is written once, as its own mirror image
+                if (row0 + i < d.m && (PRODUCT == kUpdate || ti != tj)) {
+                    direct.hi[(row0 + i) * direct.stride + col] = pr.hi;
+                    direct.lo[(row0 + i) * direct.stride + col] = pr.lo;
+                }
+            }
+            // the padded width holds all four (zeros past m)
+            *reinterpret_cast<Half4*>(turned.hi + col * turned.stride + row0) = hi;
+            *reinterpret_cast<Half4*>(turned.lo + col * turned.stride + row0) = lo;
+        }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// LDS of k_ortho_small.
+size_t small_bytes(int64_t mp, int64_t np) { return static_cast<size_t>(2 * mp * (np + 8) + 2 * mp * (mp + 8)) * sizeof(f16); }
+
+constexpr size_t kSmallLds = 160 * 1024 - 256;  // a CU's, less the kernel's own
+
+bool is_small(int64_t mp, int64_t np) { return mp <= 128 && np <= 16384 && small_bytes(mp, np) <= kSmallLds; }
+
+// Sizes of a matrix; its planes from `at` on in the workspace (large ones).
+OrthoMatrix describe(const relm_mp_update& u, size_t& at) {
+    OrthoMatrix d{};
+    d.in = u.in;
+    d.out = u.out;
+    d.in_stride = u.row_stride;
+    d.tall = u.rows > u.cols;
+    d.m = static_cast<int32_t>(std::min(u.rows, u.cols));
+    d.n = static_cast<int32_t>(std::max(u.rows, u.cols));
+    d.mp = static_cast<int32_t>(ceil_div(d.m, 32) * 32);
+    d.np = static_cast<int32_t>(ceil_div(d.n, 32) * 32);
+    // 2^round(log2 sqrt(m n)), at most 2^13: the entries of X are about 1 at first, and
+    // no more than twice the scale throughout
+    const int e = static_cast<int>(std::lround(0.5 * std::log2(static_cast<double>(d.m) * static_cast<double>(d.n))));
+    d.scale = std::ldexp(1.0f, std::min(e, 13));
+    if (is_small(d.mp, d.np)) return d;
+    const auto take = [&](size_t bytes) {
+        const size_t p = at;
+        at = align_up(at + bytes, 256);
+        return static_cast<int64_t>(p);
+    };
+    const size_t m = d.m, n = d.n, mp = d.mp, np = d.np;
+    d.x = take(4 * m * np);
+    d.xt[0] = take(4 * n * mp);
+    d.xt[1] = take(4 * n * mp);
+    d.a = take(4 * m * mp);
+    d.b = take(4 * m * mp);
+    d.partial = take(kNormParts * sizeof(double));
+    return d;
+}
+
+template <typename T, int BT>
+hipError_t large_steps(const OrthoBatch& b, const OrthoRule& rule, int count, int64_t lower, int64_t all, void* ws,
+                       hipStream_t st) {
+    for (int step = 0; step < rule.steps; ++step) {
+        hipLaunchKernelGGL((k_ortho_product<T, kGram, BT>), dim3(static_cast<unsigned>(lower)), dim3(kThreads), 0, st, b, rule,
+                           count, step, ws);
+        hipLaunchKernelGGL((k_ortho_product<T, kSquare, BT>), dim3(static_cast<unsigned>(lower)), dim3(kThreads), 0, st, b,
+                           rule, count, step, ws);
+        hipLaunchKernelGGL((k_ortho_product<T, kUpdate, BT>), dim3(static_cast<unsigned>(all)), dim3(kThreads), 0, st, b, rule,
+                           count, step, ws);
+    }
+    return hipGetLastError();
+}
+
+// Numbers the tiles of a launch's matrices.
+void number_tiles(OrthoBatch& b, int count, int64_t bt, int64_t& lower, int64_t& all) {
+    lower = all = 0;
+    for (int i = 0; i < count; ++i) {
+        OrthoMatrix& d = b.mat[i];
+        d.first_tile[0] = lower;
+        d.first_tile[1] = all;
+        const int64_t r = ceil_div(d.m, bt), c = ceil_div(d.n, bt);
+        lower += r * (r + 1) / 2;
+        all += r * c;
+    }
+}
+
+template <typename T>
+hipError_t run(const std::vector<OrthoMatrix>& small, const std::vector<OrthoMatrix>& large, const OrthoRule& rule, void* ws,
+               hipStream_t st) {
+    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(k_ortho_small<T>),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds);
+    if (!small.empty() && allowed != hipSuccess) return allowed;
+    for (size_t i = 0; i < small.size(); i += kOrthoBatch) {
+        OrthoBatch b{};
+        const size_t count = std::min<size_t>(kOrthoBatch, small.size() - i);
+        size_t lds = 0;
+        for (size_t k = 0; k < count; ++k) {
+            b.mat[k] = small[i + k];
+            lds = std::max(lds, small_bytes(b.mat[k].mp, b.mat[k].np));
+        }
+        hipLaunchKernelGGL(k_ortho_small<T>, dim3(static_cast<unsigned>(count)), dim3(kSmallThreads), lds, st, b, rule);
+    }
+    for (size_t i = 0; i < large.size(); i += kOrthoBatch) {
+        OrthoBatch b{};
+        const int count = static_cast<int>(std::min<size_t>(kOrthoBatch, large.size() - i));
+        int mp = 0, np = 0;
+        for (int k = 0; k < count; ++k) {
+            b.mat[k] = large[i + k];
+            mp = std::max(mp, b.mat[k].mp);
+            np = std::max(np, b.mat[k].np);
+        }
+        hipLaunchKernelGGL(k_ortho_norm<T>, dim3(kNormParts, count), dim3(kThreads), 0, st, b, ws);
+        hipLaunchKernelGGL(k_ortho_split<T>, dim3(np / 32, mp / 32, count), dim3(kThreads), 0, st, b, rule, ws);
+        int64_t lower, all;
+        number_tiles(b, count, 128, lower, all);
+        hipError_t e;
+        if (lower >= kLargeTiles) {
+            e = large_steps<T, 128>(b, rule, count, lower, all, ws, st);
+        } else {
+            number_tiles(b, count, 64, lower, all);
+            e = large_steps<T, 64>(b, rule, count, lower, all, ws, st);
+        }
+        if (e != hipSuccess) return e;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t orthogonalise_workspace(const relm_mp_update* updates, int32_t count) {
+    size_t at = 0;
+    for (int32_t i = 0; i < count; ++i)
+        if (updates[i].rows > 0 && updates[i].cols > 0) describe(updates[i], at);
+    return at;
+}
+
+hipError_t launch_orthogonalise(int dtype, const relm_mp_update* updates, int32_t count, const OrthoRule& rule, void* ws,
+                                hipStream_t st) {
+    std::vector<OrthoMatrix> small, large;
+    size_t at = 0;
+    for (int32_t i = 0; i < count; ++i) {
+        if (updates[i].rows == 0 || updates[i].cols == 0) continue;
+        const OrthoMatrix d = describe(updates[i], at);
+        (is_small(d.mp, d.np) ? small : large).push_back(d);
+    }
+    hipError_t e = hipErrorInvalidValue;
+    with_value_type(dtype, [&](auto t) { e = run<decltype(t)>(small, large, rule, ws, st); });
+    return e;
+}
+
+}  // namespace relm_mp

@@ -10,6 +10,7 @@
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <optional>
 #include <tuple>
@@ -267,6 +268,45 @@ std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor& grad, 
     return {dq, dk, dv};
 }
 
+// ---- orthogonalised update ---------------------------------------------------------
+
+// One result per update; updates of more than two dimensions are stacks of matrices.
+std::vector<Tensor> orthogonalise(at::TensorList updates, int64_t steps, at::ArrayRef<double> coefficients, double eps) {
+    const char* op = "orthogonalise";
+    TORCH_CHECK(coefficients.size() == 3, op, ": three coefficients expected.");
+    std::vector<Tensor> inputs, results;
+    if (updates.empty()) return results;
+    const int dtype = value_dtype(updates[0], op, "every update");
+    std::vector<relm_mp_update> mats;
+    c10::OptionalDeviceGuard guard(updates[0].device());
+    inputs.reserve(updates.size());
+    results.reserve(updates.size());
+    mats.reserve(updates.size());
+    for (const Tensor& u : updates) {
+        check_like(u, updates[0], op, "every update");
+        TORCH_CHECK(u.dim() >= 2, op, ": updates must be matrices or stacks of them.");
+        const int64_t rows = u.size(-2), cols = u.size(-1);
+        const bool rows_apart = u.dim() == 2 && (cols <= 1 || u.stride(1) == 1) && (rows <= 1 || u.stride(0) >= cols);
+        inputs.push_back(rows_apart ? u : u.contiguous());
+        results.push_back(at::empty(u.sizes(), u.options()));
+        const Tensor& in = inputs.back();
+        const int64_t stride = u.dim() == 2 ? std::max(in.stride(0), cols) : cols;
+        const int64_t step = rows * cols * static_cast<int64_t>(u.element_size());
+        for (int64_t i = 0, n = step == 0 ? 0 : u.numel() / (rows * cols); i < n; ++i)
+            mats.push_back({static_cast<const char*>(in.const_data_ptr()) + i * step,
+                            static_cast<char*>(results.back().data_ptr()) + i * step, rows, cols, stride});
+    }
+    TORCH_CHECK(mats.size() <= 1 << 20, op, ": too many matrices.");
+    const int32_t count = static_cast<int32_t>(mats.size());
+    const size_t need = relm_mp_orthogonalise_workspace_size(mats.data(), count);
+    const Tensor ws = need > 0 ? bytes(need, updates[0]) : Tensor();
+    raise_if(relm_mp_orthogonalise(dtype, mats.data(), count, static_cast<int32_t>(std::min<int64_t>(steps, 1 << 30)),
+                                   static_cast<float>(coefficients[0]), static_cast<float>(coefficients[1]),
+                                   static_cast<float>(coefficients[2]), static_cast<float>(eps),
+                                   need > 0 ? ws.data_ptr() : nullptr, need, current_stream(updates[0])));
+    return results;
+}
+
 }  // namespace readout
 }  // namespace relm_amd
 
@@ -278,6 +318,7 @@ TORCH_LIBRARY_FRAGMENT(relm_mp, m) {
     m.def("attention_plan(Tensor q_offsets, Tensor k_offsets, int heads, int kv_heads) -> __torch__.torch.classes.relm_mp.AttentionPlan");
     m.def("cross_attention(Tensor q, Tensor k, Tensor v, __torch__.torch.classes.relm_mp.AttentionPlan plan, Tensor? key_mask, float scale, bool keep) -> (Tensor, Tensor)");
     m.def("cross_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, __torch__.torch.classes.relm_mp.AttentionPlan plan, Tensor? key_mask, float scale, Tensor out, Tensor lse) -> (Tensor, Tensor, Tensor)");
+    m.def("orthogonalise(Tensor[] updates, int steps, float[] coefficients, float eps) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(relm_mp, CompositeImplicitAutograd, m) {
@@ -287,4 +328,5 @@ TORCH_LIBRARY_IMPL(relm_mp, CompositeImplicitAutograd, m) {
     m.impl("attention_plan", relm_amd::readout::attention_plan);
     m.impl("cross_attention", relm_amd::readout::cross_attention);
     m.impl("cross_attention_backward", relm_amd::readout::cross_attention_backward);
+    m.impl("orthogonalise", relm_amd::readout::orthogonalise);
 }

@@ -284,6 +284,27 @@ def cross_attention(
     return _readout.cross_attention(q, k, v, plan, key_mask, scale)
 
 
+def orthogonalise(
+    updates: torch.Tensor | list[torch.Tensor],
+    steps: int = 5,
+    coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315),
+    eps: float = 1e-7,
+):
+    """The nearly orthogonal matrix to each update, by Newton-Schulz products: ``X = G / (|G| +
+    eps)``, then ``steps`` times ``A = X X^T``, ``X <- a X + (b A + c A A) X`` on the shorter
+    side.  Singular vectors stay, singular values go towards 1 (with the default
+    coefficients into 0.7 to 1.2).
+
+    ``updates`` is one tensor or a list of them, as all of a model's (few launches for all
+    together); each a matrix or a stack of matrices, of one dtype (float32, bfloat16 or
+    float16 on the GPU).  Iterates are held in 22 bits and sums in float32 whatever the
+    dtype.  The polynomial must keep [0, 1] within [-2, 2].  No gradient.  No counterpart
+    in relmo."""
+
+    require_torch("orthogonalise")
+    return _readout.orthogonalise(updates, steps, coefficients, eps)
+
+
 @contextlib.contextmanager
 def plan_scope():
     """Trust scope for the library's index plans (no counterpart in relmo).
@@ -331,6 +352,7 @@ __all__ = [
     "fanout_pack_from_edges",
     "fanout_pack_multi",
     "fanout_scatter",
+    "orthogonalise",
     "plan_scope",
     "rms_norm",
 ]

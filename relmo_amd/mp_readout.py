@@ -1,8 +1,8 @@
 """The readout ops of the facade: what a program runs on the object states.
 
-``add_rms_norm`` (a residual stream's norm, also with an 8-bit output) and
-``cross_attention`` (per-graph queries to the graphs' objects), without counterparts
-in relmo.  GPU tensors of float32, bfloat16 or float16 run the
+``add_rms_norm`` (a residual stream's norm, also with an 8-bit output),
+``cross_attention`` (per-graph queries to the graphs' objects) and ``orthogonalise``
+(the weight updates of what they train), without counterparts in relmo.  GPU tensors of float32, bfloat16 or float16 run the
 library's kernels through autograd functions; CPU tensors (and the policy's
 fallback) run the ATen formulations below, which autograd differentiates.
 """
@@ -222,4 +222,40 @@ def cross_attention(q, k, v, plan, key_mask, scale: float | None):
     return op(q, k, v, plan.ref, key_mask, scale, False)[0]
 
 
-__all__ = ["AttentionPlan", "add_rms_norm", "add_rms_norm_fp8", "attention_plan", "cross_attention", "rms_norm"]
+# ---- orthogonalised update ---------------------------------------------------------
+
+
+def _orthogonalise_float(update, steps: int, coefficients, eps: float):
+    a, b, c = coefficients
+    x = update.to(torch.promote_types(update.dtype, torch.float32))
+    tall = x.size(-2) > x.size(-1)
+    x = x.mT if tall else x
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return (x.mT if tall else x).to(update.dtype).contiguous()
+
+
+def orthogonalise(updates, steps: int, coefficients, eps: float):
+    one = torch.is_tensor(updates)
+    parts = [updates] if one else list(updates)
+    coefficients = [float(v) for v in coefficients]
+    if len(coefficients) != 3:
+        raise ValueError("orthogonalise expects three coefficients.")
+    for u in parts:
+        if u.dim() < 2:
+            raise ValueError("orthogonalise expects matrices or stacks of them.")
+        if u.dtype != parts[0].dtype or u.device != parts[0].device:
+            raise ValueError("orthogonalise expects updates of one dtype on one device.")
+    op = library_op("orthogonalise", tensor=parts[0], gpu_only=True) if parts else None
+    with torch.no_grad():
+        if op is not None:
+            results = op(parts, int(steps), coefficients, float(eps))
+        else:
+            results = [_orthogonalise_float(u, int(steps), coefficients, eps) for u in parts]
+    return results[0] if one else results
+
+
+__all__ = ["AttentionPlan", "add_rms_norm", "add_rms_norm_fp8", "attention_plan", "cross_attention",
+           "orthogonalise", "rms_norm"]
