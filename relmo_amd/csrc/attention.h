@@ -47,13 +47,18 @@ inline const AttnJoin* plan_key_joins(const relm_mp_attention_plan& p) {
     return reinterpret_cast<const AttnJoin*>(plan_key_items(p) + p.num_key_items);
 }
 
-// Floats that the parts need: per part, key head and row the sum's head_dim values with
-// its maximum and total (forward), its values (dq), or two rows of values per key (dk, dv).
+// Where the parts' sums go: per part, key head and row (key) of its tile one row of
+// head_dim floats, padded to 16 bytes (dk and dv: two); the forward's maxima and totals
+// follow all rows.
+inline int64_t attention_part_stride(int64_t head_dim) { return (head_dim + 3) / 4 * 4; }
+inline int64_t attention_part_rows(const relm_mp_attention_plan& p) {
+    return static_cast<int64_t>(p.num_parts) * p.kv_heads * p.row_tile;
+}
 inline size_t attention_part_floats(const relm_mp_attention_plan& p, int64_t head_dim) {
-    return static_cast<size_t>(p.num_parts) * p.kv_heads * p.row_tile * (head_dim + 2);
+    return static_cast<size_t>(attention_part_rows(p) * (attention_part_stride(head_dim) + 2));
 }
 inline size_t attention_key_part_floats(const relm_mp_attention_plan& p, int64_t head_dim) {
-    return static_cast<size_t>(p.num_key_parts) * p.kv_heads * p.key_tile * 2 * head_dim;
+    return static_cast<size_t>(p.num_key_parts) * p.kv_heads * p.key_tile * 2 * attention_part_stride(head_dim);
 }
 
 struct AttnOperands {

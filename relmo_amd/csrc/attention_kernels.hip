@@ -103,7 +103,9 @@ struct Args {
     float* lse;
     float* delta;
     T *dq, *dk, *dv;
-    float* parts;
+    float* parts;        // sums of the parts, rows of part_stride floats
+    float* part_stats;   // forward: their maxima and totals
+    int part_stride;
     bool out_whole;  // rows of head_dim values side by side start on dwords
 };
 
@@ -381,13 +383,10 @@ __global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
                 a.lse[p.row * a.heads + p.head] = sum_p == 0.0f ? -kInf : (top + log2f(sum_p)) * kLn2;
         } else {
             const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
-            float* to = a.parts + slot * (a.dim + 2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < a.dim) to[2 + col + j] = sum[j];
+            if (col < a.part_stride) *reinterpret_cast<f32x4*>(a.parts + slot * a.part_stride + col) = sum;
             if (col == 0) {
-                to[0] = top;
-                to[1] = sum_p;
+                a.part_stats[2 * slot] = top;
+                a.part_stats[2 * slot + 1] = sum_p;
             }
         }
     };
@@ -438,46 +437,78 @@ __global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
     }
 }
 
-// Joins the parts of a row: out = sum_p 2^(m_p - m) sum_p / sum_p 2^(m_p - m) total_p.
-// A workgroup per row and key head; its thread groups take every kThreads / DP-th part.
-template <typename T, int DP>
+// Joins the parts of a row: out = sum_p 2^(m_p - m) sum_p / sum_p 2^(m_p - m) total_p, or
+// dq = sum of the parts (DQ).  Thread groups of DP / 4 threads hold a row's sums.  MANY: a
+// workgroup per row and key head, its groups taking every kJoinGroups-th part; else a row
+// to each group.  Latency bound: 512 parts are 32 rounds of loads of a group, four at a time.
+template <int DP>
+constexpr int kJoinGroups = kThreads / (DP / 4);
+
+template <typename T, int DP, bool MANY, bool DQ>
 __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
-    constexpr int G = kThreads / DP;
-    __shared__ float lds_top[kThreads], lds_total[G], lds_sum[G][DP];
-    const AttnJoin j = a.joins[blockIdx.x / a.row_tile];
-    const int row = static_cast<int>(blockIdx.x) % a.row_tile, head = static_cast<int>(blockIdx.y);
-    if (row >= j.rows) return;
-    const int t = static_cast<int>(threadIdx.x), d = t % DP, grp = t / DP;
-    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.row_tile * (a.dim + 2);
-    const float* part = a.parts + ((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.row_tile + row) * (a.dim + 2);
+    constexpr int G = kJoinGroups<DP>, W = DP / 4;
+    __shared__ float lds_top[kThreads / kWave], lds_total[G];
+    __shared__ __align__(16) f32x4 lds_sum[MANY ? G * W : 1];
+    const int t = static_cast<int>(threadIdx.x), col = (t % W) * 4, grp = t / W, head = static_cast<int>(blockIdx.y);
+    const int per = MANY ? a.row_tile : a.row_tile / G;  // workgroups of a join
+    const AttnJoin j = a.joins[blockIdx.x / per];
+    const int row = static_cast<int>(blockIdx.x % per) * (MANY ? 1 : G) + (MANY ? 0 : grp);
+    if (MANY && row >= j.rows) return;
+    const int64_t slot0 = (static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.row_tile + row;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.row_tile;
+    const bool mine = row < j.rows && col < a.part_stride;
     float top = -kInf;
-    for (int p = t; p < j.parts; p += kThreads) top = fmaxf(top, part[p * step]);
-    lds_top[t] = top;
-    __syncthreads();
-    for (int o = kThreads / 2; o > 0; o /= 2) {
-        if (t < o) lds_top[t] = fmaxf(lds_top[t], lds_top[t + o]);
-        __syncthreads();
+    if constexpr (!DQ) {
+        if constexpr (MANY) {
+            for (int p = t; p < j.parts; p += kThreads) top = fmaxf(top, a.part_stats[2 * (slot0 + p * step)]);
+#pragma unroll
+            for (int o = kWave / 2; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+            if (lane_id() == 0) lds_top[t / kWave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kThreads / kWave; ++w) top = fmaxf(top, lds_top[w]);
+        } else if (row < j.rows) {
+            for (int p = 0; p < j.parts; ++p) top = fmaxf(top, a.part_stats[2 * (slot0 + p * step)]);
+        }
     }
-    top = lds_top[0];
     const float base = top == -kInf ? 0.0f : top;
-    float sum = 0.0f, total = 0.0f;
-    const bool mine = d < a.dim;
-    for (int p = grp; p < j.parts; p += G) {
-        const float share = exp2_of(part[p * step] - base);
-        total = fmaf(part[p * step + 1], share, total);
-        if (mine) sum = fmaf(part[p * step + 2 + d], share, sum);
+    f32x4 sum = f32x4(0.0f);
+    float total = 0.0f;
+    if (mine) {
+#pragma unroll 4
+        for (int p = MANY ? grp : 0; p < j.parts; p += MANY ? G : 1) {
+            const int64_t slot = slot0 + p * step;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.parts + slot * a.part_stride + col);
+            if constexpr (DQ) {
+                sum += x;
+            } else {
+                const float share = exp2_of(a.part_stats[2 * slot] - base);
+                total = fmaf(a.part_stats[2 * slot + 1], share, total);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(x[i], share, sum[i]);
+            }
+        }
     }
-    lds_sum[grp][d] = sum;
-    if (d == 0) lds_total[grp] = total;
-    __syncthreads();
-    if (grp != 0 || !mine) return;
-    for (int i = 1; i < G; ++i) {
-        sum += lds_sum[i][d];
-        total += lds_total[i];
+    if constexpr (MANY) {
+        lds_sum[t] = sum;
+        if (col == 0) lds_total[grp] = total;
+        __syncthreads();
+        if (grp != 0) return;
+        for (int i = 1; i < G; ++i) {
+            sum += lds_sum[i * W + t];
+            total += lds_total[i];
+        }
     }
+    if (!mine) return;
     const Place p = place_of(a, j.q_first, head, j.row0 + row);
-    a.out[(p.row * a.heads + p.head) * a.dim + d] = round_to<T>(total == 0.0f ? 0.0f : sum * (1.0f / total));
-    if (d == 0 && a.lse != nullptr) a.lse[p.row * a.heads + p.head] = total == 0.0f ? -kInf : (top + log2f(total)) * kLn2;
+    T* to = (DQ ? a.dq : a.out) + (p.row * a.heads + p.head) * a.dim;
+    if constexpr (DQ) {
+        put4<T>(to, col, a.dim, a.out_whole, sum * a.scale);
+    } else {
+        put4<T>(to, col, a.dim, a.out_whole, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+        if (col == 0 && a.lse != nullptr)
+            a.lse[p.row * a.heads + p.head] = total == 0.0f ? -kInf : (top + log2f(total)) * kLn2;
+    }
 }
 
 // Scores to probabilities and their gradients in place: s becomes p, dp becomes ds.
@@ -626,9 +657,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_dq(Args<T> a) {
             put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * a.scale);
         } else {
             const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < a.dim) a.parts[slot * a.dim + col + j] = sum[j];
+            if (col < a.part_stride) *reinterpret_cast<f32x4*>(a.parts + slot * a.part_stride + col) = sum;
         }
     };
     if constexpr (S::kSharers == 1) {
@@ -656,27 +685,6 @@ __global__ __launch_bounds__(kThreads) void k_attention_dq(Args<T> a) {
             if (col < a.dim) finish(row, place_of(a, w.it.q_first, w.head, w.it.row0 + row), col, sum);
         }
     }
-}
-
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void k_attention_dq_join(Args<T> a) {
-    constexpr int G = kThreads / DP;
-    __shared__ float lds_sum[G][DP];
-    const AttnJoin j = a.joins[blockIdx.x / a.row_tile];
-    const int row = static_cast<int>(blockIdx.x) % a.row_tile, head = static_cast<int>(blockIdx.y);
-    if (row >= j.rows) return;
-    const int t = static_cast<int>(threadIdx.x), d = t % DP, grp = t / DP;
-    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.row_tile * a.dim;
-    const float* part = a.parts + ((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.row_tile + row) * a.dim;
-    float sum = 0.0f;
-    if (d < a.dim)
-        for (int p = grp; p < j.parts; p += G) sum += part[p * step + d];
-    lds_sum[grp][d] = sum;
-    __syncthreads();
-    if (grp != 0 || d >= a.dim) return;
-    for (int i = 1; i < G; ++i) sum += lds_sum[i][d];
-    const Place p = place_of(a, j.q_first, head, j.row0 + row);
-    a.dq[(p.row * a.heads + p.head) * a.dim + d] = round_to<T>(sum * a.scale);
 }
 
 // Half values end at 2^-14 (below, they lose bits): the probabilities of a query with
@@ -808,34 +816,37 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv(Args<T> a) {
                 put4<T>(a.dk + at * a.dim, col, a.dim, a.out_whole, dk[t][n] * a.scale);
                 put4<T>(a.dv + at * a.dim, col, a.dim, a.out_whole, dv[t][n] * (1.0f / kProbabilityUnit<T>));
             } else {
-                float* to = a.parts +
-                            ((static_cast<int64_t>(w.it.part) * a.kv_heads + head) * a.key_tile + key) * (2 * a.dim);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (col + j < a.dim) {
-                        to[col + j] = dk[t][n][j];
-                        to[a.dim + col + j] = dv[t][n][j] * (1.0f / kProbabilityUnit<T>);
-                    }
+                float* to = a.parts + ((static_cast<int64_t>(w.it.part) * a.kv_heads + head) * a.key_tile + key) *
+                                          (2 * a.part_stride) + col;
+                if (col < a.part_stride) {
+                    *reinterpret_cast<f32x4*>(to) = dk[t][n];
+                    *reinterpret_cast<f32x4*>(to + a.part_stride) = dv[t][n] * (1.0f / kProbabilityUnit<T>);
+                }
             }
         }
     }
 }
 
-template <typename T>
+// Joins the parts of a key item: a thread group per key, its dk and dv side by side.
+template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void k_attention_dkv_join(Args<T> a) {
-    const AttnJoin j = a.joins[blockIdx.x / a.key_tile];
-    const int key = static_cast<int>(blockIdx.x) % a.key_tile, head = static_cast<int>(blockIdx.y);
-    const int d = static_cast<int>(threadIdx.x);
-    if (key >= j.keys || d >= 2 * a.dim) return;
-    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.key_tile * 2 * a.dim;
-    const float* part = a.parts + ((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.key_tile + key) * (2 * a.dim) + d;
-    float sum = 0.0f;
-    for (int p = 0; p < j.parts; ++p) sum += part[p * step];
+    constexpr int W = DP / 4, G = kThreads / (2 * W);
+    const int t = static_cast<int>(threadIdx.x), per = a.key_tile / G;
+    const AttnJoin j = a.joins[blockIdx.x / per];
+    const int key = static_cast<int>(blockIdx.x % per) * G + t / (2 * W), head = static_cast<int>(blockIdx.y);
+    const int which = t / W % 2, col = (t % W) * 4;
+    if (key >= j.keys || col >= a.part_stride) return;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.key_tile * 2 * a.part_stride;
+    const float* part = a.parts + (((static_cast<int64_t>(j.part0) * a.kv_heads + head) * a.key_tile + key) * 2 + which) *
+                                      a.part_stride + col;
+    f32x4 sum = f32x4(0.0f);
+#pragma unroll 4
+    for (int p = 0; p < j.parts; ++p) sum += *reinterpret_cast<const f32x4*>(part + p * step);
     const int64_t at = ((static_cast<int64_t>(j.key_first) + key) * a.kv_heads + head) * a.dim;
-    if (d < a.dim)
-        a.dk[at + d] = round_to<T>(sum * a.scale);
+    if (which == 0)
+        put4<T>(a.dk + at, col, a.dim, a.out_whole, sum * a.scale);
     else
-        a.dv[at + d - a.dim] = round_to<T>(sum);
+        put4<T>(a.dv + at, col, a.dim, a.out_whole, sum);
 }
 
 // ---- launches -----------------------------------------------------------------------
@@ -865,6 +876,8 @@ Args<T> args_of(const relm_mp_attention_plan& p, const AttnOperands& o) {
     a.dk = static_cast<T*>(o.dk);
     a.dv = static_cast<T*>(o.dv);
     a.parts = o.parts;
+    a.part_stride = static_cast<int>(attention_part_stride(o.head_dim));
+    a.part_stats = o.parts + attention_part_rows(p) * a.part_stride;
     a.out_whole = sizeof(T) * o.head_dim % 4 == 0;
     for (const void* x : {o.out, o.dq, o.dk, o.dv}) a.out_whole = a.out_whole && reinterpret_cast<uintptr_t>(x) % 4 == 0;
     return a;
@@ -894,6 +907,21 @@ void with_rows(int row_tile, F&& f) {
     }
 }
 
+// Rows of up to kFewParts parts on average are joined a thread group to a row.
+constexpr int kFewParts = 8;
+
+template <typename T, int DP, bool DQ>
+void join_rows(const relm_mp_attention_plan& p, const Args<T>& a, hipStream_t st) {
+    if (p.num_joins == 0) return;
+    if (p.num_parts > kFewParts * p.num_joins || p.row_tile < kJoinGroups<DP>)
+        hipLaunchKernelGGL((k_attention_join<T, DP, true, DQ>),
+                           dim3(static_cast<unsigned>(p.num_joins) * p.row_tile, p.kv_heads), dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_attention_join<T, DP, false, DQ>),
+                           dim3(static_cast<unsigned>(p.num_joins) * (p.row_tile / kJoinGroups<DP>), p.kv_heads),
+                           dim3(kThreads), 0, st, a);
+}
+
 template <typename T>
 hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
     const Args<T> a = args_of<T>(p, o);
@@ -904,9 +932,7 @@ hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipSt
             hipLaunchKernelGGL((k_attention<T, DP, decltype(rt)::value, decltype(wm)::value>),
                                dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
         });
-        if (p.num_joins > 0)
-            hipLaunchKernelGGL((k_attention_join<T, DP>), dim3(static_cast<unsigned>(p.num_joins) * p.row_tile, p.kv_heads),
-                               dim3(kThreads), 0, st, a);
+        join_rows<T, DP, false>(p, a, st);
     });
     return hipGetLastError();
 }
@@ -921,9 +947,7 @@ hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipS
                 hipLaunchKernelGGL((k_attention_dq<T, DP, decltype(rt)::value, decltype(wm)::value>),
                                    dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
             });
-        if (p.num_joins > 0)
-            hipLaunchKernelGGL((k_attention_dq_join<T, DP>),
-                               dim3(static_cast<unsigned>(p.num_joins) * p.row_tile, p.kv_heads), dim3(kThreads), 0, st, a);
+        join_rows<T, DP, true>(p, a, st);
         if (p.num_key_items > 0) {
             Args<T> b = a;
             b.items = plan_key_items(p);
@@ -938,9 +962,9 @@ hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipS
             else
                 hipLaunchKernelGGL((k_attention_dkv<T, DP, 1>), dim3(wgs * (p.key_tile / 64)), dim3(kThreads), 0, st, b);
             if (p.num_key_joins > 0)
-                hipLaunchKernelGGL(k_attention_dkv_join<T>,
-                                   dim3(static_cast<unsigned>(p.num_key_joins) * p.key_tile, p.kv_heads), dim3(kThreads), 0,
-                                   st, b);
+                hipLaunchKernelGGL((k_attention_dkv_join<T, DP>),
+                                   dim3(static_cast<unsigned>(p.num_key_joins) * (p.key_tile / (kThreads / (DP / 2))), p.kv_heads),
+                                   dim3(kThreads), 0, st, b);
         }
     });
     return hipGetLastError();

@@ -12,7 +12,10 @@ namespace relm_mp {
 
 namespace {
 
-constexpr int64_t kWorkgroups = 1024;  // of a launch: four to each of 256 CUs
+// Workgroups of a launch at least, where the lengths allow: four to each of 256 CUs, two of
+// those that keep 64 or more rows (keys: 128) in registers.
+constexpr int64_t kWorkgroups = 1024;
+constexpr int64_t kLargeWorkgroups = 512;
 constexpr int64_t kPartUnit = 128;     // parts end on whole tiles of keys and rows
 constexpr int64_t kLeastKeys = 512;    // of a part: shorter ones cost more to join than to walk
 constexpr int64_t kLeastRows = 256;
@@ -64,14 +67,14 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
         L.row_tile = 5 * padded(rows, 128) <= 6 * padded(rows, 64) ? 128 : 64;
     L.key_tile = 5 * padded(keys, 128) <= 6 * padded(keys, 64) ? 128 : 64;
 
-    // A share is what a workgroup gets when all the work is dealt to kWorkgroups.
+    // A share is what a workgroup gets when all the work is dealt to them.
     int64_t row_work = 0, key_work = 0;
     for (int64_t b = 0; b < graphs; ++b) {
         row_work += ceil_div(rows[b], L.row_tile) * keys[b] * kv_heads;
         key_work += ceil_div(keys[b], L.key_tile) * rows[b] * kv_heads;
     }
-    const int64_t key_share = std::max(kLeastKeys, ceil_div(row_work, kWorkgroups));
-    const int64_t row_share = std::max(kLeastRows, ceil_div(key_work, kWorkgroups));
+    const int64_t key_share = std::max(kLeastKeys, ceil_div(row_work, L.row_tile >= 64 ? kLargeWorkgroups : kWorkgroups));
+    const int64_t row_share = std::max(kLeastRows, ceil_div(key_work, L.key_tile == 128 ? kLargeWorkgroups : kWorkgroups));
 
     constexpr size_t kMost = size_t{1} << 24;  // table records: 512 MB
     for (int64_t b = 0; b < graphs; ++b) {
