@@ -33,43 +33,50 @@ constexpr float kInf = __builtin_inff();
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A row's operand at its place: [rows, heads, head_dim] by strides.  `whole`: every row
-// of every head starts on a dword, so that 16-byte accesses serve; else a value at a time.
+// An operand [rows, heads, head_dim] by its strides.
 template <typename T>
 struct Rows {
     const T* data;
     int64_t row_stride, head_stride;
-    bool whole;
 };
 
 template <typename T>
 Rows<T> rows_of(const relm_mp_head_rows& r) {
-    const auto dword = [](int64_t bytes) { return bytes % 4 == 0; };
-    return {static_cast<const T*>(r.data), r.row_stride, r.head_stride,
-            dword(reinterpret_cast<intptr_t>(r.data)) && dword(r.row_stride * static_cast<int64_t>(sizeof(T))) &&
-                dword(r.head_stride * static_cast<int64_t>(sizeof(T)))};
+    return {static_cast<const T*>(r.data), r.row_stride, r.head_stride};
 }
 
-// Values [col, col + N) of a row of `dim` at p, zero past its end.
+// Whether every row of every head starts on a dword.
+bool on_dwords(const relm_mp_head_rows& r, size_t value) {
+    return reinterpret_cast<uintptr_t>(r.data) % 4 == 0 && r.row_stride * value % 4 == 0 && r.head_stride * value % 4 == 0;
+}
+
+// N values of T of a row of `dim` at p, from column `col` on, zero past its end.  WHOLE: 8
+// divides dim and every row of every operand starts on a dword, so 16-byte accesses serve;
+// else value by value.  Neither way branches: loads on both sides of a branch would wait
+// for one another.
 template <typename T, int N>
-__device__ __forceinline__ T __attribute__((ext_vector_type(N))) take(const T* p, int col, int dim, bool whole) {
-    using Vec = T __attribute__((ext_vector_type(N)));
-    Vec v;
-    if (whole && col + N <= dim) {
-        if constexpr (sizeof(T) * N <= 16) {
-            v = *reinterpret_cast<const ValueVec<T, N>*>(p + col);
-        } else {
-            constexpr int M = 16 / sizeof(T);
+using Values = T __attribute__((ext_vector_type(N)));
+
+template <typename T, int N, bool WHOLE>
+__device__ __forceinline__ Values<T, N> take(const T* p, int col, int dim) {
+    Values<T, N> v;
+    const bool live = col < dim;
+    if constexpr (WHOLE) {
+        const T* at = p + (live ? col : 0);
+        constexpr int M = N * sizeof(T) <= 16 ? N : 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < N / M; ++c) {
-                const ValueVec<T, M> part = *reinterpret_cast<const ValueVec<T, M>*>(p + col + c * M);
+        for (int c = 0; c < N / M; ++c) {
+            const ValueVec<T, M> part = *reinterpret_cast<const ValueVec<T, M>*>(at + c * M);
 #pragma unroll
-                for (int j = 0; j < M; ++j) v[c * M + j] = part[j];
-            }
+            for (int j = 0; j < M; ++j) v[c * M + j] = part[j];
         }
+        if (!live) v = Values<T, N>(static_cast<T>(0.0f));
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = col + j < dim ? p[col + j] : static_cast<T>(0.0f);
+        for (int j = 0; j < N; ++j) v[j] = p[min(col + j, dim - 1)];
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (col + j >= dim) v[j] = static_cast<T>(0.0f);
     }
     return v;
 }
@@ -128,7 +135,7 @@ struct Place {
 };
 template <typename T>
 __device__ __forceinline__ Place place_of(const Args<T>& a, int q_first, int kv_head, int r) {
-    const int q = r / a.group;
+    const int q = a.group == 1 ? r : r / a.group;
     return {static_cast<int64_t>(q_first) + q, kv_head * a.group + (r - q * a.group)};
 }
 
@@ -141,34 +148,30 @@ constexpr int kLdsStride = DP + 16 / static_cast<int>(sizeof(T));
 template <typename T, int DP, int BN>
 struct TileLoad {
     static constexpr int kV = 16 / static_cast<int>(sizeof(T));
-    static constexpr int kUnits = DP / kV;  // of a row
-    static constexpr int kRounds = (BN * kUnits + kThreads - 1) / kThreads;
-    using Vec = T __attribute__((ext_vector_type(kV)));
-    Vec v[kRounds];
+    static constexpr int kUnits = DP / kV;               // of a row
+    static constexpr int kStep = kThreads / kUnits;      // rows of a round
+    static constexpr int kRounds = BN / kStep;
+    static_assert(kThreads % kUnits == 0 && BN % kStep == 0, "whole rounds");
+    Values<T, kV> v[kRounds];
 
-    // place(row) gives the row's pointer, NULL for a row of zeros
-    template <typename F>
-    __device__ __forceinline__ void fetch(F&& place, int dim, bool whole) {
+    static __device__ __forceinline__ int first_row() { return static_cast<int>(threadIdx.x) / kUnits; }
+    static __device__ __forceinline__ int column() { return (static_cast<int>(threadIdx.x) % kUnits) * kV; }
+
+    // place(row): where a row of the tile lies (some row that exists for one that does not)
+    template <bool WHOLE, typename F>
+    __device__ __forceinline__ void fetch(F&& place, int dim) {
 #pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-            const int u = i * kThreads + static_cast<int>(threadIdx.x);
-            const int row = u / kUnits, col = (u % kUnits) * kV;
-            const T* p = u < BN * kUnits ? place(row) : nullptr;
-            if (p != nullptr)
-                v[i] = take<T, kV>(p, col, dim, whole);
-            else
-                v[i] = Vec(static_cast<T>(0.0f));
-        }
+        for (int i = 0; i < kRounds; ++i) v[i] = take<T, kV, WHOLE>(place(first_row() + i * kStep), column(), dim);
     }
-    // keep(row): whether the row's values enter (a row that does not is stored as zeros)
+    // Into LDS; unless `all` rows enter, those that keep(row) leaves out as zeros.
     template <typename F>
-    __device__ __forceinline__ void store(T* tile, F&& keep) const {
+    __device__ __forceinline__ void store(T* tile, bool all, F&& keep) const {
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
-            const int u = i * kThreads + static_cast<int>(threadIdx.x);
-            const int row = u / kUnits, col = (u % kUnits) * kV;
-            if (u < BN * kUnits)
-                *reinterpret_cast<Vec*>(tile + row * kLdsStride<T, DP> + col) = keep(row) ? v[i] : Vec(static_cast<T>(0.0f));
+            const int row = first_row() + i * kStep;
+            Values<T, kV> x = v[i];
+            if (!all && !keep(row)) x = Values<T, kV>(static_cast<T>(0.0f));
+            *reinterpret_cast<Values<T, kV>*>(tile + row * kLdsStride<T, DP> + column()) = x;
         }
     }
 };
@@ -176,69 +179,62 @@ struct TileLoad {
 // Which of a tile's BN keys are kept: bit k of the words.
 template <int BN>
 struct KeyBits {
-    uint8_t byte[BN / 64];
+    uint32_t byte[BN / 64];
     uint64_t bits[BN / 64];
-    // asks for the mask's bytes of keys [first, first + left)
+    // asks for the mask's bytes of keys [first, first + left), left > 0
     __device__ __forceinline__ void fetch(const uint8_t* mask, int64_t first, int left) {
 #pragma unroll
         for (int w = 0; w < BN / 64; ++w) {
             const int k = w * 64 + lane_id();
-            byte[w] = k < left ? (mask != nullptr ? mask[first + k] : 1) : 0;
+            byte[w] = mask != nullptr ? mask[first + min(k, left - 1)] : 1u;
+            byte[w] = k < left ? byte[w] : 0u;
         }
     }
     __device__ __forceinline__ void settle() {
 #pragma unroll
         for (int w = 0; w < BN / 64; ++w) bits[w] = __ballot(byte[w] != 0);
     }
-    __device__ __forceinline__ bool has(int k) const {
-        const uint64_t w = BN == 128 && (k & 64) ? bits[BN / 64 - 1] : bits[0];
-        return (w >> (k % 64)) & 1;
-    }
-    // the 32 keys from k on
-    __device__ __forceinline__ uint32_t chunk(int k) const {
-        const uint64_t w = BN == 128 && (k & 64) ? bits[BN / 64 - 1] : bits[0];
-        return static_cast<uint32_t>(w >> (k % 64));
-    }
+    __device__ __forceinline__ bool all() const { return (bits[0] & bits[BN / 64 - 1]) == ~0ull; }
+    __device__ __forceinline__ uint64_t word(int k) const { return BN == 128 && (k & 64) ? bits[BN / 64 - 1] : bits[0]; }
+    __device__ __forceinline__ bool has(int k) const { return (word(k) >> (k % 64)) & 1; }
 };
 
 // Fragments of 16 rows of q (or grad) that a wave keeps: lane l holds row l % 16.
 template <typename T, int DP>
 struct RowFrags {
     Frag<T> f[DP / 32];
-    __device__ __forceinline__ void fetch(const T* p, int dim, bool whole) {
+    template <bool WHOLE>
+    __device__ __forceinline__ void fetch(const T* p, int dim) {
         const int g = lane_id() / 16;
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-            if (p != nullptr)
-                f[c] = take<T, 8>(p, c * 32 + g * 8, dim, whole);
-            else
-                f[c] = Frag<T>(static_cast<T>(0.0f));
-        }
+        for (int c = 0; c < DP / 32; ++c) f[c] = take<T, 8, WHOLE>(p, c * 32 + g * 8, dim);
     }
 };
 
-// Scores (before scaling) of 32 keys by 16 rows, keys down: two tiles of 16 keys.
-template <typename T, int DP>
-__device__ __forceinline__ void keys_by_rows(const T* keys, int key0, const RowFrags<T, DP>& rows, f32x4 (&s)[2]) {
+// Products of 32 keys (rows of a tile, from key0 on) with RT tiles of 16 rows, keys down:
+// two tiles of 16 keys each, on top of `start`.
+template <typename T, int DP, int RT>
+__device__ __forceinline__ void keys_by_rows(const T* keys, int key0, const RowFrags<T, DP> (&rows)[RT], const f32x4 (&start)[2],
+                                             f32x4 (&s)[RT][2]) {
     const int l = lane_id();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        s[t] = f32x4(0.0f);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
-            s[t] = mma<T>(lds_frag<T>(keys, kLdsStride<T, DP>, key0 + 16 * t + l % 16, c * 32 + (l / 16) * 8), rows.f[c], s[t]);
+        for (int r = 0; r < RT; ++r) s[r][t] = start[t];
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+            const Frag<T> k = lds_frag<T>(keys, kLdsStride<T, DP>, key0 + 16 * t + l % 16, c * 32 + (l / 16) * 8);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s[r][t] = mma<T>(k, rows[r].f[c], s[r][t]);
+        }
     }
 }
 
-// Entries of the lane's keys that are not kept become `value`.
-__device__ __forceinline__ void leave_out(f32x4 (&s)[2], uint32_t kept, float value) {
-    if (kept == 0xffffffffu) return;
-    const uint32_t mine = kept >> (4 * (lane_id() / 16));
+// What the scores of the lane's keys start from: 0, or -inf for a key that is not kept
+// (whose values are zeros in LDS).  The products then need no selection.
+__device__ __forceinline__ void key_starts(const float* starts, int key0, f32x4 (&start)[2]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (!((mine >> (16 * t + i)) & 1)) s[t][i] = value;
+    for (int t = 0; t < 2; ++t) start[t] = *reinterpret_cast<const f32x4*>(starts + key0 + 16 * t + 4 * (lane_id() / 16));
 }
 
 // Over the four lanes that share a query (l, l ^ 16, l ^ 32, l ^ 48).
@@ -250,6 +246,11 @@ __device__ __forceinline__ float lanes_sum(float v) {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
+
+// Two waves to a SIMD with 16-bit values: one's matrix instructions run beside the other's
+// exponentials.  Float rows need the registers of both.
+template <typename T>
+constexpr int kWavesPerSimd = sizeof(T) == 2 ? 2 : 1;
 
 // Shapes of the row kernels: a wave has RT tiles of 16 rows; WM waves have rows of their
 // own and 4 / WM share each row tile, taking different keys of a tile.
@@ -263,13 +264,14 @@ struct RowShape {
 
 // Forward.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with the running maximum m:
 // when a key tile raises it, what has been added up is scaled by exp(m_old - m_new).
-template <typename T, int DP, int RT, int WM>
-__global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
+template <typename T, int DP, int RT, int WM, bool WHOLE>
+__global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T> a) {
     using S = RowShape<RT, WM>;
     constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
     constexpr int kTileBytes = 2 * BN * ST * static_cast<int>(sizeof(T));
     constexpr int kMergeBytes = S::kSharers > 1 ? kWaves * 16 * RT * (DP + 2) * 4 : 0;
     __shared__ __align__(16) char lds[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+    __shared__ __align__(16) float starts[BN];
     T* kt = reinterpret_cast<T*>(lds);
     T* vt = kt + BN * ST;
     const Work w = work_of(a.items, a.num_items, a.kv_heads);
@@ -285,7 +287,8 @@ __global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
         const int row = (row_wave * RT + r) * 16 + l % 16;
         real[r] = row < w.it.rows;
         at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
-        qf[r].fetch(real[r] ? a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride : nullptr, a.dim, a.q.whole);
+        // a row past the item reads its first: a column of the scores, used by no other
+        qf[r].template fetch<WHOLE>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
     }
     f32x4 o[RT][ND];
     float m[RT], total[RT];
@@ -304,41 +307,38 @@ __global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
         const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
         const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
         const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
-        kl.fetch([&](int row) { return row < left ? kp + row * a.k.row_stride : nullptr; }, a.dim, a.k.whole);
-        vl.fetch([&](int row) { return row < left ? vp + row * a.v.row_stride : nullptr; }, a.dim, a.v.whole);
+        kl.template fetch<WHOLE>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
+        vl.template fetch<WHOLE>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         __syncthreads();
-        kl.store(kt, [](int) { return true; });  // scores of keys that are not kept are replaced, not used
-        vl.store(vt, [&](int row) { return a.key_mask == nullptr || bits.has(row); });
+        kl.store(kt, bits.all(), [&](int row) { return bits.has(row); });
+        vl.store(vt, bits.all(), [&](int row) { return bits.has(row); });
+        if (threadIdx.x < BN) starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
         __syncthreads();
-        const KeyBits<BN> now = bits;
         if (k0 + BN < w.it.keys) fetch(k0 + BN);
-        f32x4 s[RT][S::kChunks][2];
-        float top[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) top[r] = -kInf;
+        f32x4 s[S::kChunks][RT][2];
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int key0 = (key_wave * S::kChunks + c) * 32;
-            const uint32_t kept = now.chunk(key0);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                keys_by_rows<T, DP>(kt, key0, qf[r], s[r][c]);
-                leave_out(s[r][c], kept, -kInf);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], s[r][c][t][i]);
-            }
+            f32x4 start[2];
+            key_starts(starts, key0, start);
+            keys_by_rows<T, DP, RT>(kt, key0, qf, start, s[c]);
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             // the maximum of scale * log2(e) * s; the factor is positive
-            const float most = fmaxf(m[r], lanes_max(top[r]) * sl2);
+            float top = -kInf;
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[c][r][t][i]);
+            const float most = fmaxf(m[r], lanes_max(top) * sl2);
             if (__any(most > m[r])) {
                 const float shrink = exp2_of(m[r] - (most == -kInf ? 0.0f : most));
                 total[r] *= shrink;
@@ -353,8 +353,8 @@ __global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = exp2_of(fmaf(s[r][c][t][i], sl2, -base));
-                        s[r][c][t][i] = p;
+                        const float p = exp2_of(fmaf(s[c][r][t][i], sl2, -base));
+                        s[c][r][t][i] = p;
                         total[r] += p;
                     }
         }
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(kThreads) void k_attention(Args<T> a) {
             const int key0 = (key_wave * S::kChunks + c) * 32;
             Frag<T> p[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) p[r] = frag_of<T>(s[r][c][0], s[r][c][1]);
+            for (int r = 0; r < RT; ++r) p[r] = frag_of<T>(s[c][r][0], s[c][r][1]);
 #pragma unroll
             for (int n = 0; n < ND; ++n) {
                 const Frag<T> vf = lds_frag_t<T>(vt, ST, key0, n * 16);
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
 }
 
 // Scores to probabilities and their gradients in place: s becomes p, dp becomes ds.
-__device__ __forceinline__ void backward_scores(f32x4 (&s)[2], f32x4 (&dp)[2], uint32_t kept, float sl2, float lse2, float delta) {
+__device__ __forceinline__ void backward_scores(f32x4 (&s)[2], f32x4 (&dp)[2], float sl2, float lse2, float delta) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -521,8 +521,6 @@ __device__ __forceinline__ void backward_scores(f32x4 (&s)[2], f32x4 (&dp)[2], u
             s[t][i] = p;
             dp[t][i] = p * (dp[t][i] - delta);
         }
-    leave_out(s, kept, 0.0f);
-    leave_out(dp, kept, 0.0f);
 }
 
 // Half values lose bits below 2^-14, where ds of keys with small probabilities lies.  A lane
@@ -563,13 +561,14 @@ __device__ __forceinline__ float lse2_of(float lse) { return lse == -kInf ? kInf
 
 // dq of a row item: like the forward, with the probabilities recomputed from lse.  The
 // item over a row's first keys also leaves its delta for the key kernel.
-template <typename T, int DP, int RT, int WM>
-__global__ __launch_bounds__(kThreads) void k_attention_dq(Args<T> a) {
+template <typename T, int DP, int RT, int WM, bool WHOLE>
+__global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Args<T> a) {
     using S = RowShape<RT, WM>;
     constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
     constexpr int kTileBytes = 2 * BN * ST * static_cast<int>(sizeof(T));
     constexpr int kMergeBytes = S::kSharers > 1 ? kWaves * 16 * RT * DP * 4 : 0;
     __shared__ __align__(16) char lds[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+    __shared__ __align__(16) float starts[BN];
     T* kt = reinterpret_cast<T*>(lds);
     T* vt = kt + BN * ST;
     const Work w = work_of(a.items, a.num_items, a.kv_heads);
@@ -587,18 +586,17 @@ __global__ __launch_bounds__(kThreads) void k_attention_dq(Args<T> a) {
         const int row = (row_wave * RT + r) * 16 + l % 16;
         real[r] = row < w.it.rows;
         at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
-        qf[r].fetch(real[r] ? a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride : nullptr, a.dim, a.q.whole);
-        gf[r].fetch(real[r] ? a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride : nullptr, a.dim,
-                    a.grad.whole);
+        qf[r].template fetch<WHOLE>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
+        gf[r].template fetch<WHOLE>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
         RowFrags<T, DP> of;
-        of.fetch(real[r] ? a.out + (at[r].row * a.heads + at[r].head) * a.dim : nullptr, a.dim, a.out_whole);
+        of.template fetch<WHOLE>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
         float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
         delta[r] = lanes_sum(sum);
-        lse2[r] = real[r] ? lse2_of(a.lse[at[r].row * a.heads + at[r].head]) : kInf;
+        lse2[r] = lse2_of(a.lse[at[r].row * a.heads + at[r].head]);
         unit[r] = kStartUnit<T>;
         if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
 #pragma unroll
@@ -612,32 +610,33 @@ __global__ __launch_bounds__(kThreads) void k_attention_dq(Args<T> a) {
         const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
         const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
         const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
-        kl.fetch([&](int row) { return row < left ? kp + row * a.k.row_stride : nullptr; }, a.dim, a.k.whole);
-        vl.fetch([&](int row) { return row < left ? vp + row * a.v.row_stride : nullptr; }, a.dim, a.v.whole);
+        kl.template fetch<WHOLE>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
+        vl.template fetch<WHOLE>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         __syncthreads();
-        kl.store(kt, [&](int row) { return a.key_mask == nullptr || bits.has(row); });
-        vl.store(vt, [](int) { return true; });
+        kl.store(kt, bits.all(), [&](int row) { return bits.has(row); });
+        vl.store(vt, bits.all(), [&](int row) { return bits.has(row); });
+        if (threadIdx.x < BN) starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
         __syncthreads();
-        const KeyBits<BN> now = bits;
         if (k0 + BN < w.it.keys) fetch(k0 + BN);
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int key0 = (key_wave * S::kChunks + c) * 32;
-            const uint32_t kept = now.chunk(key0);
+            const f32x4 zero[2] = {f32x4(0.0f), f32x4(0.0f)};
+            f32x4 start[2], s[RT][2], dp[RT][2];
+            key_starts(starts, key0, start);
+            keys_by_rows<T, DP, RT>(kt, key0, qf, start, s);
+            keys_by_rows<T, DP, RT>(vt, key0, gf, zero, dp);
             Frag<T> ds[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                f32x4 s[2], dp[2];
-                keys_by_rows<T, DP>(kt, key0, qf[r], s);
-                keys_by_rows<T, DP>(vt, key0, gf[r], dp);
-                backward_scores(s, dp, kept, sl2, lse2[r], delta[r]);
-                into_unit<T>(dp, unit[r], dq[r]);
-                ds[r] = frag_of<T>(dp[0], dp[1]);
+                backward_scores(s[r], dp[r], sl2, lse2[r], delta[r]);
+                into_unit<T>(dp[r], unit[r], dq[r]);
+                ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
             }
 #pragma unroll
             for (int n = 0; n < ND; ++n) {
@@ -696,8 +695,8 @@ constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
 // dk and dv of a key item: a wave keeps KT tiles of 16 keys and walks the graph's rows
 // (rows down, keys across, so that a lane's probabilities are the operand of the products
 // over rows).
-template <typename T, int DP, int KT>
-__global__ __launch_bounds__(kThreads) void k_attention_dkv(Args<T> a) {
+template <typename T, int DP, int KT, bool WHOLE>
+__global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Args<T> a) {
     constexpr int BR = 64, ST = kLdsStride<T, DP>, ND = DP / 16;
     __shared__ __align__(16) T qt[BR * ST];
     __shared__ __align__(16) T gt[BR * ST];
@@ -711,17 +710,24 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv(Args<T> a) {
     const float sl2 = a.scale * kLog2e;
 
     RowFrags<T, DP> kf[KT], vf[KT];
-    bool kept[KT], real[KT];
+    bool real[KT];
     float unit[KT];
+    f32x4 start[KT];  // of the scores: -inf for a key that is not kept
     f32x4 dk[KT][ND], dv[KT][ND];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
         const int key = (wave * KT + t) * 16 + l % 16;
-        const int64_t at = static_cast<int64_t>(w.it.key_first) + key;
+        // a key past the item reads its last: a column of the scores, used by no other
         real[t] = key < w.it.keys;
-        kept[t] = real[t] && (a.key_mask == nullptr || a.key_mask[at] != 0);
-        kf[t].fetch(kept[t] ? a.k.data + at * a.k.row_stride + head * a.k.head_stride : nullptr, a.dim, a.k.whole);
-        vf[t].fetch(kept[t] ? a.v.data + at * a.v.row_stride + head * a.v.head_stride : nullptr, a.dim, a.v.whole);
+        const int64_t at = static_cast<int64_t>(w.it.key_first) + min(key, w.it.keys - 1);
+        const bool kept = real[t] && (a.key_mask == nullptr || a.key_mask[at] != 0);
+        kf[t].template fetch<WHOLE>(a.k.data + at * a.k.row_stride + head * a.k.head_stride, a.dim);
+        vf[t].template fetch<WHOLE>(a.v.data + at * a.v.row_stride + head * a.v.head_stride, a.dim);
+        if (!kept) {
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) kf[t].f[c] = vf[t].f[c] = Frag<T>(static_cast<T>(0.0f));
+        }
+        start[t] = f32x4(kept ? 0.0f : -kInf);
 #pragma unroll
         for (int n = 0; n < ND; ++n) dk[t][n] = dv[t][n] = f32x4(0.0f);
         unit[t] = kStartUnit<T>;
@@ -731,65 +737,73 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv(Args<T> a) {
     float lse_in = 0.0f, delta_in = 0.0f;
     const auto fetch = [&](int r0) {
         const int left = w.it.rows - r0;
-        ql.fetch([&](int row) {
-            const Place p = place_of(a, w.it.q_first, head, w.it.row0 + r0 + row);
-            return row < left ? a.q.data + p.row * a.q.row_stride + p.head * a.q.head_stride : nullptr;
-        }, a.dim, a.q.whole);
-        gl.fetch([&](int row) {
-            const Place p = place_of(a, w.it.q_first, head, w.it.row0 + r0 + row);
-            return row < left ? a.grad.data + p.row * a.grad.row_stride + p.head * a.grad.head_stride : nullptr;
-        }, a.dim, a.grad.whole);
-        const int row = static_cast<int>(threadIdx.x);
-        if (row < BR) {
-            lse_in = kInf;
-            delta_in = 0.0f;
-            if (row < left) {
-                const Place p = place_of(a, w.it.q_first, head, w.it.row0 + r0 + row);
-                lse_in = lse2_of(a.lse[p.row * a.heads + p.head]);
-                delta_in = a.delta[p.row * a.heads + p.head];
-            }
-        }
+        const auto place = [&](int row) { return place_of(a, w.it.q_first, head, w.it.row0 + r0 + min(row, left - 1)); };
+        ql.template fetch<WHOLE>([&](int row) {
+            const Place p = place(row);
+            return a.q.data + p.row * a.q.row_stride + p.head * a.q.head_stride;
+        }, a.dim);
+        gl.template fetch<WHOLE>([&](int row) {
+            const Place p = place(row);
+            return a.grad.data + p.row * a.grad.row_stride + p.head * a.grad.head_stride;
+        }, a.dim);
+        const int row = static_cast<int>(threadIdx.x) % BR;
+        const Place p = place(row);
+        lse_in = lse2_of(a.lse[p.row * a.heads + p.head]);
+        delta_in = a.delta[p.row * a.heads + p.head];
+        if (row >= left) lse_in = kInf;  // probability 0
     };
     if (w.it.rows > 0) fetch(0);
     for (int r0 = 0; r0 < w.it.rows; r0 += BR) {
         __syncthreads();
-        ql.store(qt, [](int) { return true; });
-        gl.store(gt, [](int) { return true; });
+        const int left = w.it.rows - r0;
+        ql.store(qt, left >= BR, [&](int row) { return row < left; });
+        gl.store(gt, left >= BR, [&](int row) { return row < left; });
         if (threadIdx.x < BR) {
             row_lse2[threadIdx.x] = lse_in;
             row_delta[threadIdx.x] = delta_in;
         }
         __syncthreads();
-        const int left = w.it.rows - r0;
         if (left > BR) fetch(r0 + BR);
 #pragma unroll
         for (int c = 0; c < BR / 32; ++c) {
             if (c * 32 >= left) break;
+            f32x4 s[KT][2], dp[KT][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = c * 32 + h * 16;
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    s[t][h] = start[t];
+                    dp[t][h] = f32x4(0.0f);
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) {
+                    const Frag<T> qr = lds_frag<T>(qt, ST, row + l % 16, i * 32 + g * 8);
+                    const Frag<T> gr = lds_frag<T>(gt, ST, row + l % 16, i * 32 + g * 8);
+#pragma unroll
+                    for (int t = 0; t < KT; ++t) {
+                        s[t][h] = mma<T>(qr, kf[t].f[i], s[t][h]);
+                        dp[t][h] = mma<T>(gr, vf[t].f[i], dp[t][h]);
+                    }
+                }
+            }
             Frag<T> pf[KT], dsf[KT];
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
-                f32x4 s[2], dp[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int row = c * 32 + h * 16;
-                    s[h] = dp[h] = f32x4(0.0f);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) {
-                        s[h] = mma<T>(lds_frag<T>(qt, ST, row + l % 16, i * 32 + g * 8), kf[t].f[i], s[h]);
-                        dp[h] = mma<T>(lds_frag<T>(gt, ST, row + l % 16, i * 32 + g * 8), vf[t].f[i], dp[h]);
-                    }
-                    const f32x4 lse2 = *reinterpret_cast<const f32x4*>(row_lse2 + row + g * 4);
-                    const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + row + g * 4);
+                    const f32x4 lse2 = *reinterpret_cast<const f32x4*>(row_lse2 + c * 32 + h * 16 + g * 4);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + c * 32 + h * 16 + g * 4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = kept[t] ? exp2_of(fmaf(s[h][i], sl2, -lse2[i])) : 0.0f;
-                        s[h][i] = p;
-                        dp[h][i] = kept[t] ? p * (dp[h][i] - delta[i]) : 0.0f;
+                        const float p = exp2_of(fmaf(s[t][h][i], sl2, -lse2[i]));
+                        s[t][h][i] = p;
+                        dp[t][h][i] = p * (dp[t][h][i] - delta[i]);
                     }
                 }
-                pf[t] = frag_of<T>(s[0] * kProbabilityUnit<T>, s[1] * kProbabilityUnit<T>);
-                into_unit<T>(dp, unit[t], dk[t]);
-                dsf[t] = frag_of<T>(dp[0], dp[1]);
+                pf[t] = frag_of<T>(s[t][0] * kProbabilityUnit<T>, s[t][1] * kProbabilityUnit<T>);
+                into_unit<T>(dp[t], unit[t], dk[t]);
+                dsf[t] = frag_of<T>(dp[t][0], dp[t][1]);
             }
 #pragma unroll
             for (int n = 0; n < ND; ++n) {
@@ -883,22 +897,34 @@ Args<T> args_of(const relm_mp_attention_plan& p, const AttnOperands& o) {
     return a;
 }
 
-// f with the padded head size (32, 64 or 128) and the rows' shape of the plan.
+// The WHOLE of the kernels.
+bool whole_rows(const AttnOperands& o, size_t value) {
+    return o.head_dim % 8 == 0 && reinterpret_cast<uintptr_t>(o.out) % 4 == 0 && on_dwords(o.q, value) &&
+           on_dwords(o.k, value) && on_dwords(o.v, value) && on_dwords(o.grad, value);
+}
+
+// f with the padded head size (32, 64 or 128), WHOLE, and the rows' shape of the plan.
 template <typename F>
-void with_dim(int64_t dim, F&& f) {
+void with_dim(int64_t dim, bool whole, F&& f) {
+    const auto with = [&](auto dp) {
+        if (whole)
+            f(dp, std::true_type{});
+        else
+            f(dp, std::false_type{});
+    };
     if (dim <= 32)
-        f(std::integral_constant<int, 32>{});
+        with(std::integral_constant<int, 32>{});
     else if (dim <= 64)
-        f(std::integral_constant<int, 64>{});
+        with(std::integral_constant<int, 64>{});
     else
-        f(std::integral_constant<int, 128>{});
+        with(std::integral_constant<int, 128>{});
 }
 template <typename T, int DP, typename F>
 void with_rows(int row_tile, F&& f) {
     using std::integral_constant;
-    // float rows of 128 values: tiles of 128 keys and of 32 rows to a wave leave it too
-    // few registers
-    constexpr bool kLarge = sizeof(T) * DP >= 512;
+    // rows of 128 values: tiles of 128 keys and of 32 rows to a wave leave it too few
+    // registers
+    constexpr bool kLarge = DP == 128;
     switch (row_tile) {
         case 16: f(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
         case 32: f(integral_constant<int, kLarge ? 1 : 2>{}, integral_constant<int, kLarge ? 2 : 1>{}); break;
@@ -926,10 +952,11 @@ template <typename T>
 hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
     const Args<T> a = args_of<T>(p, o);
     if (p.num_items == 0) return hipSuccess;
-    with_dim(o.head_dim, [&](auto dp) {
+    with_dim(o.head_dim, whole_rows(o, sizeof(T)), [&](auto dp, auto whole) {
         constexpr int DP = decltype(dp)::value;
+        constexpr bool W = decltype(whole)::value;
         with_rows<T, DP>(p.row_tile, [&](auto rt, auto wm) {
-            hipLaunchKernelGGL((k_attention<T, DP, decltype(rt)::value, decltype(wm)::value>),
+            hipLaunchKernelGGL((k_attention<T, DP, decltype(rt)::value, decltype(wm)::value, W>),
                                dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
         });
         join_rows<T, DP, false>(p, a, st);
@@ -940,11 +967,12 @@ hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipSt
 template <typename T>
 hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
     const Args<T> a = args_of<T>(p, o);
-    with_dim(o.head_dim, [&](auto dp) {
+    with_dim(o.head_dim, whole_rows(o, sizeof(T)), [&](auto dp, auto whole) {
         constexpr int DP = decltype(dp)::value;
+        constexpr bool W = decltype(whole)::value;
         if (p.num_items > 0)
             with_rows<T, DP>(p.row_tile, [&](auto rt, auto wm) {
-                hipLaunchKernelGGL((k_attention_dq<T, DP, decltype(rt)::value, decltype(wm)::value>),
+                hipLaunchKernelGGL((k_attention_dq<T, DP, decltype(rt)::value, decltype(wm)::value, W>),
                                    dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
             });
         join_rows<T, DP, true>(p, a, st);
@@ -953,14 +981,14 @@ hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipS
             b.items = plan_key_items(p);
             b.joins = plan_key_joins(p);
             b.num_items = p.num_key_items;
-            // two tiles of keys to a wave halve its reads of the rows; float rows of 128
-            // values leave no registers for the second
-            constexpr int KT = sizeof(T) * DP < 512 ? 2 : 1;
+            // two tiles of keys to a wave halve its reads of the rows; rows of 128 values
+            // leave no registers for the second
+            constexpr int KT = DP < 128 ? 2 : 1;
             const unsigned wgs = static_cast<unsigned>(p.num_key_items) * p.kv_heads;
             if (p.key_tile == 64 * KT)
-                hipLaunchKernelGGL((k_attention_dkv<T, DP, KT>), dim3(wgs), dim3(kThreads), 0, st, b);
+                hipLaunchKernelGGL((k_attention_dkv<T, DP, KT, W>), dim3(wgs), dim3(kThreads), 0, st, b);
             else
-                hipLaunchKernelGGL((k_attention_dkv<T, DP, 1>), dim3(wgs * (p.key_tile / 64)), dim3(kThreads), 0, st, b);
+                hipLaunchKernelGGL((k_attention_dkv<T, DP, 1, W>), dim3(wgs * (p.key_tile / 64)), dim3(kThreads), 0, st, b);
             if (p.num_key_joins > 0)
                 hipLaunchKernelGGL((k_attention_dkv_join<T, DP>),
                                    dim3(static_cast<unsigned>(p.num_key_joins) * (p.key_tile / (kThreads / (DP / 2))), p.kv_heads),
