@@ -156,6 +156,8 @@ class AttentionPlan(ctypes.Structure):
         ("num_key_items", ctypes.c_int32),
         ("num_key_parts", ctypes.c_int32),
         ("num_key_joins", ctypes.c_int32),
+        ("num_idle_items", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
         ("table", ctypes.c_void_p),
     ]
 

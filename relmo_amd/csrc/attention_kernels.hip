@@ -863,6 +863,226 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv_join(Args<T> a) {
         put4<T>(a.dv + at, col, a.dim, a.out_whole, sum);
 }
 
+// The whole backward of a batch whose graphs have at most 32 rows: a workgroup has all of a
+// graph's rows, so a key tile's dk and dv are complete when it has been walked, dq when
+// all have, and keys and values are read once.  A wave takes 32 keys of a tile.  dq sums over
+// keys and wants them down (as in the forward), dk and dv over rows and want those down: the
+// scores are computed both ways, from the same fragments with the operands exchanged, and
+// their exponentials twice, which beside the reads they overlap costs little.
+template <typename T, int DP>
+struct FewRows {
+    static constexpr int kKeys = 128, kStride = kLdsStride<T, DP>;
+    // float rows of 128 values leave LDS for 16 rows
+    static constexpr int kRows = sizeof(T) * DP < 512 ? 32 : 16;
+    __align__(16) T k[kKeys * kStride];
+    __align__(16) T v[kKeys * kStride];
+    __align__(16) T q[kRows * kStride];
+    __align__(16) T g[kRows * kStride];
+    __align__(16) float starts[kKeys];
+    __align__(16) float lse2[32];
+    __align__(16) float delta[32];
+};
+
+template <typename T, int DP, int RT, bool WHOLE>
+__device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& w, FewRows<T, DP>& m) {
+    using M = FewRows<T, DP>;
+    constexpr int BN = M::kKeys, ST = M::kStride, ND = DP / 16;
+    const int l = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, g = l / 16;
+    const float sl2 = a.scale * kLog2e;
+
+    TileLoad<T, DP, BN> kl, vl;
+    KeyBits<BN> bits;
+    const auto fetch = [&](int k0) {
+        const int left = w.it.keys - k0;
+        const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
+        const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
+        const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
+        kl.template fetch<WHOLE>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
+        vl.template fetch<WHOLE>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
+        bits.fetch(a.key_mask, first, left);
+    };
+    if (w.it.keys > 0) fetch(0);
+
+    RowFrags<T, DP> qf[RT], gf[RT];
+    Place at[RT];
+    bool real[RT];
+    float lse2[RT], delta[RT], unit[RT];
+    f32x4 dq[RT][ND];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = r * 16 + l % 16;
+        real[r] = row < w.it.rows;
+        at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
+        qf[r].template fetch<WHOLE>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
+        gf[r].template fetch<WHOLE>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
+        RowFrags<T, DP> of;
+        of.template fetch<WHOLE>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
+        delta[r] = lanes_sum(sum);
+        lse2[r] = lse2_of(a.lse[at[r].row * a.heads + at[r].head]);
+        if (!real[r]) {  // a sum over rows must not see it
+            lse2[r] = kInf;
+            delta[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) qf[r].f[c] = gf[r].f[c] = Frag<T>(static_cast<T>(0.0f));
+        }
+        unit[r] = kStartUnit<T>;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) dq[r][n] = f32x4(0.0f);
+        if (wave == 0) {
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                lds_put<T>(m.q + row * ST + c * 32 + g * 8, qf[r].f[c]);
+                lds_put<T>(m.g + row * ST + c * 32 + g * 8, gf[r].f[c]);
+            }
+            if (g == 0) {
+                m.lse2[row] = lse2[r];
+                m.delta[row] = delta[r];
+            }
+        }
+    }
+
+    for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
+        bits.settle();
+        __syncthreads();
+        kl.store(m.k, bits.all(), [&](int row) { return bits.has(row); });
+        vl.store(m.v, bits.all(), [&](int row) { return bits.has(row); });
+        if (threadIdx.x < BN) m.starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
+        __syncthreads();
+        if (k0 + BN < w.it.keys) fetch(k0 + BN);
+        const int key0 = wave * 32;
+        if (k0 + key0 >= w.it.keys) continue;
+
+        // [key tile][row tile]: keys down, for dq; and rows down, for dk and dv
+        f32x4 s[2][RT], dp[2][RT], s2[2][RT], dp2[2][RT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const f32x4 down = *reinterpret_cast<const f32x4*>(m.starts + key0 + 16 * t + 4 * g);
+            const f32x4 across = f32x4(m.starts[key0 + 16 * t + l % 16]);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                s[t][r] = down;
+                s2[t][r] = across;
+                dp[t][r] = dp2[t][r] = f32x4(0.0f);
+            }
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const Frag<T> k = lds_frag<T>(m.k, ST, key0 + 16 * t + l % 16, c * 32 + g * 8);
+                const Frag<T> v = lds_frag<T>(m.v, ST, key0 + 16 * t + l % 16, c * 32 + g * 8);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    s[t][r] = mma<T>(k, qf[r].f[c], s[t][r]);
+                    dp[t][r] = mma<T>(v, gf[r].f[c], dp[t][r]);
+                    s2[t][r] = mma<T>(qf[r].f[c], k, s2[t][r]);
+                    dp2[t][r] = mma<T>(gf[r].f[c], v, dp2[t][r]);
+                }
+            }
+        }
+        Frag<T> ds[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            f32x4 sr[2] = {s[0][r], s[1][r]}, dr[2] = {dp[0][r], dp[1][r]};
+            backward_scores(sr, dr, sl2, lse2[r], delta[r]);
+            into_unit<T>(dr, unit[r], dq[r]);
+            ds[r] = frag_of<T>(dr[0], dr[1]);
+        }
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+            const Frag<T> kf = lds_frag_t<T>(m.k, ST, key0, n * 16);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) dq[r][n] = mma<T>(kf, ds[r], dq[r][n]);
+        }
+        Frag<T> pf[2], dsf[2];
+        float unit2[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 pr[2] = {f32x4(0.0f), f32x4(0.0f)}, dr[2] = {f32x4(0.0f), f32x4(0.0f)}, none[1] = {f32x4(0.0f)};
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const f32x4 row_lse2 = *reinterpret_cast<const f32x4*>(m.lse2 + r * 16 + g * 4);
+                const f32x4 row_delta = *reinterpret_cast<const f32x4*>(m.delta + r * 16 + g * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    pr[r][i] = exp2_of(fmaf(s2[t][r][i], sl2, -row_lse2[i]));
+                    dr[r][i] = pr[r][i] * (dp2[t][r][i] - row_delta[i]);
+                }
+            }
+            pf[t] = frag_of<T>(pr[0] * kProbabilityUnit<T>, pr[1] * kProbabilityUnit<T>);
+            unit2[t] = kStartUnit<T>;
+            into_unit<T>(dr, unit2[t], none);
+            dsf[t] = frag_of<T>(dr[0], dr[1]);
+        }
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+            const Frag<T> gt = rows_frag_t<T, RT>(m.g, ST, n * 16);
+            const Frag<T> qt = rows_frag_t<T, RT>(m.q, ST, n * 16);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 dv = mma<T>(gt, pf[t], f32x4(0.0f));
+                const f32x4 dk = mma<T>(qt, dsf[t], f32x4(0.0f));
+                const int key = k0 + key0 + 16 * t + l % 16;
+                if (key < w.it.keys) {
+                    const int64_t to = ((static_cast<int64_t>(w.it.key_first) + key) * a.kv_heads + w.head) * a.dim;
+                    put4<T>(a.dk + to, n * 16 + g * 4, a.dim, a.out_whole, dk * (a.scale / unit2[t]));
+                    put4<T>(a.dv + to, n * 16 + g * 4, a.dim, a.out_whole, dv * (1.0f / kProbabilityUnit<T>));
+                }
+            }
+        }
+    }
+
+    // the waves' shares of dq meet in LDS
+    constexpr int R = 16 * RT;
+    static_assert(sizeof(m.k) + sizeof(m.v) >= sizeof(float) * kWaves * R * DP, "room for the shares");
+    float* sums = reinterpret_cast<float*>(m.k);  // [kWaves][R][DP]
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+            *reinterpret_cast<f32x4*>(sums + (wave * R + r * 16 + l % 16) * DP + n * 16 + g * 4) = dq[r][n] * (1.0f / unit[r]);
+    __syncthreads();
+    for (int u = static_cast<int>(threadIdx.x); u < w.it.rows * (DP / 4); u += kThreads) {
+        const int row = u / (DP / 4), col = (u % (DP / 4)) * 4;
+        f32x4 sum = *reinterpret_cast<const f32x4*>(sums + row * DP + col);
+#pragma unroll
+        for (int v = 1; v < kWaves; ++v) sum += *reinterpret_cast<const f32x4*>(sums + (v * R + row) * DP + col);
+        if (w.it.part < 0) {
+            const Place p = place_of(a, w.it.q_first, w.head, w.it.row0 + row);
+            put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * a.scale);
+        } else if (col < a.part_stride) {
+            const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
+            *reinterpret_cast<f32x4*>(a.parts + slot * a.part_stride + col) = sum;
+        }
+    }
+}
+
+// Items of graphs without queries have no rows: their keys get zeros.
+template <typename T, int DP, bool WHOLE>
+__global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_few_rows_backward(Args<T> a) {
+    __shared__ FewRows<T, DP> m;
+    const Work w = work_of(a.items, a.num_items, a.kv_heads);
+    if (w.it.rows == 0) {
+        for (int u = static_cast<int>(threadIdx.x); u < w.it.keys * (DP / 4); u += kThreads) {
+            const int col = (u % (DP / 4)) * 4;
+            const int64_t to = ((static_cast<int64_t>(w.it.key_first) + u / (DP / 4)) * a.kv_heads + w.head) * a.dim;
+            put4<T>(a.dk + to, col, a.dim, a.out_whole, f32x4(0.0f));
+            put4<T>(a.dv + to, col, a.dim, a.out_whole, f32x4(0.0f));
+        }
+        return;
+    }
+    if constexpr (FewRows<T, DP>::kRows == 32) {
+        if (w.it.rows > 16) {
+            few_rows_backward<T, DP, 2, WHOLE>(a, w, m);
+            return;
+        }
+    }
+    few_rows_backward<T, DP, 1, WHOLE>(a, w, m);
+}
+
 // ---- launches -----------------------------------------------------------------------
 
 template <typename T>
@@ -966,10 +1186,18 @@ hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipSt
 
 template <typename T>
 hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
-    const Args<T> a = args_of<T>(p, o);
+    Args<T> a = args_of<T>(p, o);
     with_dim(o.head_dim, whole_rows(o, sizeof(T)), [&](auto dp, auto whole) {
         constexpr int DP = decltype(dp)::value;
         constexpr bool W = decltype(whole)::value;
+        if (p.row_tile <= FewRows<T, DP>::kRows) {
+            a.num_items = p.num_items + p.num_idle_items;
+            if (a.num_items > 0)
+                hipLaunchKernelGGL((k_attention_few_rows_backward<T, DP, W>),
+                                   dim3(static_cast<unsigned>(a.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
+            join_rows<T, DP, true>(p, a, st);
+            return;
+        }
         if (p.num_items > 0)
             with_rows<T, DP>(p.row_tile, [&](auto rt, auto wm) {
                 hipLaunchKernelGGL((k_attention_dq<T, DP, decltype(rt)::value, decltype(wm)::value, W>),

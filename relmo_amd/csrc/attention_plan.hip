@@ -29,7 +29,7 @@ int64_t padded(const std::vector<int64_t>& n, int64_t tile) {
 }
 
 struct Layout {
-    std::vector<AttnItem> items, key_items;
+    std::vector<AttnItem> items, idle, key_items;
     std::vector<AttnJoin> joins, key_joins;
     int32_t row_tile = 16, key_tile = 64;
     int32_t num_parts = 0, num_key_parts = 0;
@@ -90,6 +90,9 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
                                    static_cast<int32_t>(std::min(s.size, keys[b] - p * s.size)),
                                    s.parts > 1 ? L.num_parts++ : -1, {0, 0}});
         }
+        if (rows[b] == 0 && keys[b] > 0)
+            L.idle.push_back({static_cast<int32_t>(qo[b]), 0, 0, static_cast<int32_t>(ko[b]), static_cast<int32_t>(keys[b]), -1,
+                              {0, 0}});
         const Split t = split(rows[b], row_share);
         for (int64_t k = 0; k < keys[b]; k += L.key_tile) {
             const int32_t n = static_cast<int32_t>(std::min<int64_t>(L.key_tile, keys[b] - k));
@@ -101,7 +104,7 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
                                        static_cast<int32_t>(std::min(t.size, rows[b] - p * t.size)),
                                        static_cast<int32_t>(ko[b] + k), n, t.parts > 1 ? L.num_key_parts++ : -1, {0, 0}});
         }
-        if (L.items.size() + L.key_items.size() + L.joins.size() + L.key_joins.size() > kMost)
+        if (L.items.size() + L.idle.size() + L.key_items.size() + L.joins.size() + L.key_joins.size() > kMost)
             return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: too many queries and keys for one plan");
     }
     // The longest first, so that none starts when the others end.
@@ -139,7 +142,7 @@ int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, i
     Layout L;
     rc = lay_out(qo, ko, graphs, heads / kv_heads, kv_heads, L);
     if (rc != RELM_MP_OK) return rc;
-    const size_t records = L.items.size() + L.joins.size() + L.key_items.size() + L.key_joins.size();
+    const size_t records = L.items.size() + L.idle.size() + L.joins.size() + L.key_items.size() + L.key_joins.size();
     relm_mp_attention_plan p{};
     p.q_rows = q_rows;
     p.k_rows = k_rows;
@@ -155,7 +158,8 @@ int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, i
     p.num_key_items = static_cast<int32_t>(L.key_items.size());
     p.num_key_parts = L.num_key_parts;
     p.num_key_joins = static_cast<int32_t>(L.key_joins.size());
-    if (static_cast<int64_t>(std::max(L.items.size(), 2 * L.key_items.size())) * kv_heads > 0x7fffffff ||
+    p.num_idle_items = static_cast<int32_t>(L.idle.size());
+    if (static_cast<int64_t>(std::max(L.items.size() + L.idle.size(), 2 * L.key_items.size())) * kv_heads > 0x7fffffff ||
         static_cast<int64_t>(std::max(L.joins.size(), L.key_joins.size())) * 128 > 0x7fffffff || kv_heads > 65535)
         return bad("too many items for one launch");
     if (table != nullptr) {
@@ -167,6 +171,7 @@ int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, i
             at += n * sizeof(AttnItem);
         };
         put(L.items.data(), L.items.size());
+        put(L.idle.data(), L.idle.size());
         put(L.joins.data(), L.joins.size());
         put(L.key_items.data(), L.key_items.size());
         put(L.key_joins.data(), L.key_joins.size());

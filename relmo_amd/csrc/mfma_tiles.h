@@ -88,6 +88,31 @@ __device__ __forceinline__ Frag<T> lds_frag_t(const T* tile, int stride, int row
     return f;
 }
 
+// lds_frag_t of the first 16 RT rows of a tile (RT = 1: the other 16 are zeros).
+template <typename T, int RT>
+__device__ __forceinline__ Frag<T> rows_frag_t(const T* tile, int stride, int col0) {
+    if constexpr (RT == 2) return lds_frag_t<T>(tile, stride, 0, col0);
+    const int l = static_cast<int>(threadIdx.x) & 63, g = l / 16, i = l % 16;
+    Frag<T> f = Frag<T>(static_cast<T>(0.0f));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = tile[(4 * g + j) * stride + col0 + i];
+    return f;
+}
+
+// 8 values to LDS, 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void lds_put(T* to, const Frag<T>& f) {
+    using Part = T __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int p = 0; p < 8 / N; ++p) {
+        Part x;
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = f[p * N + j];
+        *reinterpret_cast<Part*>(to + p * N) = x;
+    }
+}
+
 // Two results of neighbouring 16-row tiles as the fragment that pairs with
 // lds_frag_t, rounded to T.
 template <typename T>

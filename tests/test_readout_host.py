@@ -144,7 +144,7 @@ def _build(capi, queries, keys, heads, kv_heads):
     table = (ctypes.c_int32 * max(plan.table_bytes // 4, 1))()
     capi.check(capi.lib().relm_mp_attention_plan_build(*args, table, plan.table_bytes, ctypes.byref(plan)))
     records = [tuple(table[i:i + 8]) for i in range(0, plan.table_bytes // 4, 8)]
-    cut = [plan.num_items, plan.num_joins, plan.num_key_items, plan.num_key_joins]
+    cut = [plan.num_items, plan.num_idle_items, plan.num_joins, plan.num_key_items, plan.num_key_joins]
     parts, at = [], 0
     for n in cut:
         parts.append(records[at:at + n])
@@ -161,7 +161,7 @@ def test_plan_covers_every_pair_once(capi, queries, keys, heads, kv_heads) -> No
     """Every (row, key) of every graph lies in exactly one row item and one key item, parts are numbered once and
     joined completely, and nothing reaches past its graph."""
 
-    plan, (items, joins, key_items, key_joins) = _build(capi, queries, keys, heads, kv_heads)
+    plan, (items, idle, joins, key_items, key_joins) = _build(capi, queries, keys, heads, kv_heads)
     group = heads // kv_heads
     qo, ko = _offsets(queries), _offsets(keys)
     graph_of = {}
@@ -188,7 +188,9 @@ def test_plan_covers_every_pair_once(capi, queries, keys, heads, kv_heads) -> No
     big = 1 << 30
     assert check(items, plan.row_tile, big) == plan.num_parts == sum(j[6] for j in joins)
     assert check(key_items, big, plan.key_tile) == plan.num_key_parts == sum(j[6] for j in key_joins)
-    # every row is written and every key
+    # every row is written and every key; keys that no query reads are listed apart
+    assert {(r[3], r[4]) for r in idle} == {(ko[b], k) for b, k in enumerate(keys) if k and not queries[b]}
+    assert all(r[2] == 0 and r[5] < 0 for r in idle)
     rows_whole = sum(r[2] for r in items if r[5] < 0) + sum(j[2] for j in joins)
     assert rows_whole == sum(queries) * group
     keys_whole = sum(r[4] for r in key_items if r[5] < 0) + sum(j[4] for j in key_joins)
