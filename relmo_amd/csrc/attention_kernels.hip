@@ -957,38 +957,18 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         const int key0 = wave * 32;
         if (k0 + key0 >= w.it.keys) continue;
 
-        // [key tile][row tile]: keys down, for dq; and rows down, for dk and dv
-        f32x4 s[2][RT], dp[2][RT], s2[2][RT], dp2[2][RT];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const f32x4 down = *reinterpret_cast<const f32x4*>(m.starts + key0 + 16 * t + 4 * g);
-            const f32x4 across = f32x4(m.starts[key0 + 16 * t + l % 16]);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                s[t][r] = down;
-                s2[t][r] = across;
-                dp[t][r] = dp2[t][r] = f32x4(0.0f);
-            }
-#pragma unroll
-            for (int c = 0; c < DP / 32; ++c) {
-                const Frag<T> k = lds_frag<T>(m.k, ST, key0 + 16 * t + l % 16, c * 32 + g * 8);
-                const Frag<T> v = lds_frag<T>(m.v, ST, key0 + 16 * t + l % 16, c * 32 + g * 8);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    s[t][r] = mma<T>(k, qf[r].f[c], s[t][r]);
-                    dp[t][r] = mma<T>(v, gf[r].f[c], dp[t][r]);
-                    s2[t][r] = mma<T>(qf[r].f[c], k, s2[t][r]);
-                    dp2[t][r] = mma<T>(gf[r].f[c], v, dp2[t][r]);
-                }
-            }
-        }
+        // keys down, for dq
+        f32x4 start[2], s[RT][2], dp[RT][2];
+        const f32x4 zero[2] = {f32x4(0.0f), f32x4(0.0f)};
+        key_starts(m.starts, key0, start);
+        keys_by_rows<T, DP, RT>(m.k, key0, qf, start, s);
+        keys_by_rows<T, DP, RT>(m.v, key0, gf, zero, dp);
         Frag<T> ds[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            f32x4 sr[2] = {s[0][r], s[1][r]}, dr[2] = {dp[0][r], dp[1][r]};
-            backward_scores(sr, dr, sl2, lse2[r], delta[r]);
-            into_unit<T>(dr, unit[r], dq[r]);
-            ds[r] = frag_of<T>(dr[0], dr[1]);
+            backward_scores(s[r], dp[r], sl2, lse2[r], delta[r]);
+            into_unit<T>(dp[r], unit[r], dq[r]);
+            ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
         }
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
@@ -996,10 +976,27 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
 #pragma unroll
             for (int r = 0; r < RT; ++r) dq[r][n] = mma<T>(kf, ds[r], dq[r][n]);
         }
+        // rows down, for dk and dv
         Frag<T> pf[2], dsf[2];
         float unit2[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            f32x4 s2[RT], dp2[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                s2[r] = f32x4(m.starts[key0 + 16 * t + l % 16]);
+                dp2[r] = f32x4(0.0f);
+            }
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const Frag<T> k = lds_frag<T>(m.k, ST, key0 + 16 * t + l % 16, c * 32 + g * 8);
+                const Frag<T> v = lds_frag<T>(m.v, ST, key0 + 16 * t + l % 16, c * 32 + g * 8);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    s2[r] = mma<T>(qf[r].f[c], k, s2[r]);
+                    dp2[r] = mma<T>(gf[r].f[c], v, dp2[r]);
+                }
+            }
             f32x4 pr[2] = {f32x4(0.0f), f32x4(0.0f)}, dr[2] = {f32x4(0.0f), f32x4(0.0f)}, none[1] = {f32x4(0.0f)};
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
@@ -1007,8 +1004,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 const f32x4 row_delta = *reinterpret_cast<const f32x4*>(m.delta + r * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    pr[r][i] = exp2_of(fmaf(s2[t][r][i], sl2, -row_lse2[i]));
-                    dr[r][i] = pr[r][i] * (dp2[t][r][i] - row_delta[i]);
+                    pr[r][i] = exp2_of(fmaf(s2[r][i], sl2, -row_lse2[i]));
+                    dr[r][i] = pr[r][i] * (dp2[r][i] - row_delta[i]);
                 }
             }
             pf[t] = frag_of<T>(pr[0] * kProbabilityUnit<T>, pr[1] * kProbabilityUnit<T>);
@@ -1060,9 +1057,13 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
     }
 }
 
+// Waves to a SIMD that the kernel's registers are held to.
+template <typename T, int DP>
+constexpr int kFewRowsWaves = sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 ? 2 : 1) : (DP == 32 ? 2 : 1);
+
 // Items of graphs without queries have no rows: their keys get zeros.
 template <typename T, int DP, bool WHOLE>
-__global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_few_rows_backward(Args<T> a) {
+__global__ __launch_bounds__(kThreads, (kFewRowsWaves<T, DP>)) void k_attention_few_rows_backward(Args<T> a) {
     __shared__ FewRows<T, DP> m;
     const Work w = work_of(a.items, a.num_items, a.kv_heads);
     if (w.it.rows == 0) {

@@ -46,6 +46,29 @@ Split split(int64_t n, int64_t share) {
     return {ceil_div(n, size), size};
 }
 
+// The order of items of unequal length: each XCD runs through an eighth of the list
+// (work_of), so the items are dealt to eight parts of about the same total, and each part
+// starts with its longest, so that none starts when the others end.  Items of one length
+// stay in their graphs' order: neighbours read the same keys.
+template <typename F>
+void deal(std::vector<AttnItem>& items, F&& length) {
+    const auto longer = [&](const AttnItem& a, const AttnItem& b) { return length(a) > length(b); };
+    if (items.empty()) return;
+    const auto [least, most] = std::minmax_element(items.begin(), items.end(),
+                                                   [&](const AttnItem& a, const AttnItem& b) { return length(a) < length(b); });
+    if (length(*least) == length(*most)) return;
+    std::stable_sort(items.begin(), items.end(), longer);
+    constexpr size_t kParts = 8;
+    std::vector<AttnItem> dealt;
+    dealt.reserve(items.size());
+    for (size_t part = 0; part < kParts; ++part)
+        for (size_t round = 0; round * kParts < items.size(); ++round) {  // there and back
+            const size_t i = round * kParts + (round % 2 == 0 ? part : kParts - 1 - part);
+            if (i < items.size()) dealt.push_back(items[i]);
+        }
+    items.swap(dealt);
+}
+
 int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group, int64_t kv_heads, Layout& L) {
     std::vector<int64_t> rows(graphs), keys(graphs);
     int64_t most_rows = 0;
@@ -107,10 +130,8 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
         if (L.items.size() + L.idle.size() + L.key_items.size() + L.joins.size() + L.key_joins.size() > kMost)
             return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: too many queries and keys for one plan");
     }
-    // The longest first, so that none starts when the others end.
-    std::stable_sort(L.items.begin(), L.items.end(), [](const AttnItem& a, const AttnItem& b) { return a.keys > b.keys; });
-    std::stable_sort(L.key_items.begin(), L.key_items.end(),
-                     [](const AttnItem& a, const AttnItem& b) { return a.rows > b.rows; });
+    deal(L.items, [](const AttnItem& i) { return i.keys; });
+    deal(L.key_items, [](const AttnItem& i) { return i.rows; });
     return RELM_MP_OK;
 }
 
