@@ -1,19 +1,26 @@
 // Torch binding of the readout ops (the relm_mp namespace's second part; the
 // message-passing ops are in relm_mp_ops.cpp).  No reference counterpart: what a
 // program runs on the object states that the message passing leaves.  GPU tensors
-// of float32, bfloat16 or float16; the facade runs ATen formulations for CPU
-// tensors and holds the autograd functions.
+// of float32, bfloat16 or float16 (the facade runs ATen formulations for CPU
+// tensors).  The ops that have gradients make their autograd nodes here: a call's
+// host time counts beside kernels of a few microseconds.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <limits>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <tuple>
+#include <unordered_map>
 #include <vector>
 
 #include "relm_mp.h"
@@ -22,8 +29,29 @@ namespace relm_amd {
 namespace readout {
 
 using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 namespace {
+
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// Gradients that are themselves not differentiated: with create_graph, differentiating
+// them raises.
+variable_list once(variable_list grads, const char* op) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto stop = std::make_shared<torch::autograd::DelayedError>(
+        std::string("trying to differentiate twice the backward of ") + op + ", which has no second derivative",
+        static_cast<int64_t>(grads.size()));
+    variable_list in;
+    for (Tensor& g : grads) in.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+    return (*stop)(std::move(in));
+}
 
 void raise_if(int rc) { TORCH_CHECK(rc == RELM_MP_OK, relm_mp_last_error()); }
 
@@ -40,13 +68,13 @@ int value_dtype(const Tensor& t, const char* op, const char* name) {
 }
 
 void check_like(const Tensor& t, const Tensor& like, const char* op, const char* name) {
-    TORCH_CHECK(t.scalar_type() == like.scalar_type() && t.device() == like.device(), op, ": ", name,
-                " must have the dtype and device of the first argument.");
+    TORCH_CHECK_VALUE(t.scalar_type() == like.scalar_type() && t.device() == like.device(), op, ": ", name,
+                " must have the dtype and the device of the first argument.");
 }
 
 void check_same(const Tensor& t, const Tensor& like, const char* op, const char* name) {
     check_like(t, like, op, name);
-    TORCH_CHECK(t.sizes() == like.sizes(), op, ": ", name, " must have the shape of the first argument.");
+    TORCH_CHECK_VALUE(t.sizes() == like.sizes(), op, ": ", name, " must have the shape of the first argument.");
 }
 
 Tensor bytes(size_t n, const Tensor& like) {
@@ -65,11 +93,11 @@ struct NormArgs {
 
 NormArgs norm_args(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, const char* op) {
     NormArgs a{value_dtype(x, op, "x"), x.contiguous(), Tensor(), weight.contiguous(), 0, 0};
-    TORCH_CHECK(x.dim() >= 1, op, ": x must have at least one dimension.");
+    TORCH_CHECK_VALUE(x.dim() >= 1, op, ": x must have at least one dimension.");
     a.width = x.size(-1);
     a.rows = a.width == 0 ? 0 : x.numel() / a.width;
     check_like(weight, x, op, "weight");
-    TORCH_CHECK(weight.dim() == 1 && weight.size(0) == a.width, op, ": weight must be [", a.width, "].");
+    TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == a.width, op, ": weight must be [", a.width, "].");
     if (residual.has_value() && residual->defined()) {
         check_same(*residual, x, op, "residual");
         a.r = residual->contiguous();
@@ -77,22 +105,86 @@ NormArgs norm_args(const Tensor& x, const std::optional<Tensor>& residual, const
     return a;
 }
 
-}  // namespace
+struct NormResult {
+    Tensor y, h, rstd;  // h: only with a residual (else it is x); rstd: only if kept
+};
 
-// (y, h, rstd): h is empty without a residual (it would be x), rstd unless `keep`.
-std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight,
-                                                double eps, bool keep) {
+NormResult norm_forward(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double eps, bool keep) {
     const NormArgs a = norm_args(x, residual, weight, "add_rms_norm");
     c10::OptionalDeviceGuard guard(x.device());
-    Tensor y = at::empty(x.sizes(), a.x.options());
-    Tensor h = a.r.defined() ? at::empty(x.sizes(), a.x.options()) : at::empty({0}, a.x.options());
-    Tensor rstd = at::empty({keep ? a.rows : 0}, a.x.options().dtype(at::kFloat));
+    NormResult o;
+    o.y = at::empty(x.sizes(), a.x.options());
+    if (a.r.defined()) o.h = at::empty(x.sizes(), a.x.options());
+    if (keep) o.rstd = at::empty({a.rows}, a.x.options().dtype(at::kFloat));
     raise_if(relm_mp_add_rms_norm(a.dtype, a.x.const_data_ptr(), opt_ptr(a.r), a.w.const_data_ptr(), a.rows, a.width,
-                                  static_cast<float>(eps), y.data_ptr(), a.r.defined() ? h.data_ptr() : nullptr,
-                                  keep ? rstd.data_ptr<float>() : nullptr, current_stream(x)));
-    return {y, h, rstd};
+                                  static_cast<float>(eps), o.y.data_ptr(), a.r.defined() ? o.h.data_ptr() : nullptr,
+                                  keep ? o.rstd.data_ptr<float>() : nullptr, current_stream(x)));
+    return o;
 }
 
+// (dx, dweight) from the gradients of y and, where defined, of h.
+std::tuple<Tensor, Tensor> norm_backward(const Tensor& grad_y, const Tensor& grad_h, const Tensor& h, const Tensor& weight,
+                                         const Tensor& rstd) {
+    const NormArgs a = norm_args(h, std::nullopt, weight, "add_rms_norm backward");
+    const Tensor gy = grad_y.contiguous(), gh = grad_h.defined() ? grad_h.contiguous() : Tensor();
+    c10::OptionalDeviceGuard guard(h.device());
+    Tensor dx = at::empty(h.sizes(), a.x.options());
+    Tensor dw = at::empty(weight.sizes(), a.x.options());
+    const size_t need = relm_mp_add_rms_norm_backward_workspace_size(a.dtype, a.rows, a.width);
+    const Tensor ws = bytes(need, h);
+    raise_if(relm_mp_add_rms_norm_backward(a.dtype, gy.const_data_ptr(), opt_ptr(gh), a.x.const_data_ptr(),
+                                           a.w.const_data_ptr(), rstd.const_data_ptr<float>(), a.rows, a.width, dx.data_ptr(),
+                                           dw.data_ptr(), ws.data_ptr(), need, current_stream(h)));
+    return {dx, dw};
+}
+
+// (y, h); the backward reads h, rounded as it was stored, and the rows' 1 / root.
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight,
+                                 double eps) {
+        const NormResult o = norm_forward(x, residual, weight, eps, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({o.h, weight, o.rstd});
+        return {o.y, o.h};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {grads[1], grads[1], Tensor(), Tensor()};
+        const auto [dx, dw] = norm_backward(grads[0], grads[1], saved[0], saved[1], saved[2]);
+        return once({dx, dx, dw, Tensor()}, "add_rms_norm");
+    }
+};
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, double eps) {
+        const NormResult o = norm_forward(x, std::nullopt, weight, eps, true);
+        ctx->save_for_backward({x, weight, o.rstd});
+        return o.y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const auto [dx, dw] = norm_backward(grads[0], Tensor(), saved[0], saved[1], saved[2]);
+        return once({dx, dw, Tensor()}, "rms_norm");
+    }
+};
+
+}  // namespace
+
+std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+    if (wants_grad({&x, &residual, &weight})) {
+        const variable_list o = AddRmsNorm::apply(x, residual, weight, eps);
+        return {o[0], o[1]};
+    }
+    const NormResult o = norm_forward(x, residual, weight, eps, false);
+    return {o.y, o.h};
+}
+
+Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
+    if (wants_grad({&x, &weight})) return RmsNorm::apply(x, weight, eps);
+    return norm_forward(x, std::nullopt, weight, eps, false).y;
+}
+
+// (q, scale, h); without a residual h is empty (it would be x).
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& residual,
                                                     const Tensor& weight, double eps) {
     const NormArgs a = norm_args(x, residual, weight, "add_rms_norm_fp8");
@@ -107,39 +199,24 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& x, const std::
     return {q, scale, h};
 }
 
-std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad_y, const std::optional<Tensor>& grad_h, const Tensor& h,
-                                                 const Tensor& weight, const Tensor& rstd) {
-    const char* op = "add_rms_norm_backward";
-    const NormArgs a = norm_args(h, std::nullopt, weight, op);
-    check_same(grad_y, h, op, "grad_y");
-    TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.device() == h.device() && rstd.numel() == a.rows, op,
-                ": rstd must be the forward's, float32 [rows].");
-    const Tensor gy = grad_y.contiguous(), rs = rstd.contiguous();
-    Tensor gh;
-    if (grad_h.has_value() && grad_h->defined()) {
-        check_same(*grad_h, h, op, "grad_h");
-        gh = grad_h->contiguous();
-    }
-    c10::OptionalDeviceGuard guard(h.device());
-    Tensor dx = at::empty(h.sizes(), a.x.options());
-    Tensor dw = at::empty(weight.sizes(), a.x.options());
-    const size_t need = relm_mp_add_rms_norm_backward_workspace_size(a.dtype, a.rows, a.width);
-    const Tensor ws = bytes(need, h);
-    raise_if(relm_mp_add_rms_norm_backward(a.dtype, gy.const_data_ptr(), opt_ptr(gh), a.x.const_data_ptr(),
-                                           a.w.const_data_ptr(), rs.const_data_ptr<float>(), a.rows, a.width, dx.data_ptr(),
-                                           dw.data_ptr(), ws.data_ptr(), need, current_stream(h)));
-    return {dx, dw};
-}
-
 // ---- cross attention -------------------------------------------------------------
 
 // A batch's plan with its table on the device.  The table is copied there before the
 // constructor returns, so any stream may use it; a stream other than the one the
 // memory was allocated on is recorded with the allocator.
+//
+// Ops take a plan by its number: an argument of a class would send every call through
+// Python's dispatch of such arguments (8 us).  The list holds no plan alive; a number
+// whose plan is gone, or that never was, is refused.
+void forget_plan(int64_t number);
+
 struct AttentionPlan : torch::CustomClassHolder {
     relm_mp_attention_plan plan{};
     Tensor table;
     hipStream_t stream = nullptr;
+    int64_t number = 0;
+
+    void release_resources() override { forget_plan(number); }
 
     void used_on(const c10::hip::HIPStream& s) const {
         if (table.numel() > 0 && s.stream() != stream)
@@ -147,8 +224,33 @@ struct AttentionPlan : torch::CustomClassHolder {
     }
 };
 
-c10::intrusive_ptr<AttentionPlan> attention_plan(const Tensor& q_offsets, const Tensor& k_offsets, int64_t heads,
-                                                 int64_t kv_heads) {
+struct PlanList {
+    std::mutex lock;
+    std::unordered_map<int64_t, c10::weak_intrusive_ptr<AttentionPlan>> plans;
+    int64_t next = 1;
+};
+PlanList& plan_list() {
+    static PlanList* list = new PlanList;  // outlives plans that Python frees at exit
+    return *list;
+}
+
+void forget_plan(int64_t number) {
+    PlanList& list = plan_list();
+    const std::lock_guard<std::mutex> hold(list.lock);
+    list.plans.erase(number);
+}
+
+c10::intrusive_ptr<AttentionPlan> plan_of(int64_t number, const char* op) {
+    PlanList& list = plan_list();
+    const std::lock_guard<std::mutex> hold(list.lock);
+    const auto at = list.plans.find(number);
+    auto plan = at == list.plans.end() ? c10::intrusive_ptr<AttentionPlan>() : at->second.lock();
+    TORCH_CHECK_VALUE(plan, op, ": the plan no longer exists.");
+    return plan;
+}
+
+std::tuple<c10::intrusive_ptr<AttentionPlan>, int64_t> attention_plan(const Tensor& q_offsets, const Tensor& k_offsets,
+                                                                      int64_t heads, int64_t kv_heads) {
     for (const Tensor* t : {&q_offsets, &k_offsets})
         TORCH_CHECK(t->dim() == 1 && t->scalar_type() == at::kLong && t->is_cuda() && t->numel() >= 1 &&
                         t->device() == q_offsets.device() && t->numel() == q_offsets.numel(),
@@ -172,7 +274,11 @@ c10::intrusive_ptr<AttentionPlan> attention_plan(const Tensor& q_offsets, const 
     ref->table = table.to(q_offsets.device());
     ref->stream = s.stream();
     ref->plan.table = ref->plan.table_bytes > 0 ? ref->table.const_data_ptr() : nullptr;
-    return ref;
+    PlanList& list = plan_list();
+    const std::lock_guard<std::mutex> hold(list.lock);
+    ref->number = list.next++;
+    list.plans.emplace(ref->number, c10::weak_intrusive_ptr<AttentionPlan>(ref));
+    return {ref, ref->number};
 }
 
 namespace {
@@ -192,80 +298,107 @@ struct AttnArgs {
     }
 };
 
-AttnArgs attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionPlan& p,
-                        const std::optional<Tensor>& key_mask, double scale, const char* op) {
+AttnArgs attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionPlan& p, const Tensor& key_mask,
+                        double scale) {
+    const char* op = "cross_attention";
     AttnArgs a;
     a.dtype = value_dtype(q, op, "q");
     for (const Tensor* t : {&q, &k, &v}) {
-        TORCH_CHECK(t->dim() == 3, op, ": q, k and v must be [rows, heads, head_dim].");
+        TORCH_CHECK_VALUE(t->dim() == 3, op, ": q, k and v must be [rows, heads, head_dim].");
         check_like(*t, q, op, "k and v");
     }
     a.dim = q.size(2);
-    TORCH_CHECK(a.dim >= 1 && a.dim <= RELM_MP_MAX_HEAD_DIM, op, ": head_dim must be in [1, ", RELM_MP_MAX_HEAD_DIM, "].");
-    TORCH_CHECK(q.size(0) == p.plan.q_rows && q.size(1) == p.plan.heads, op, ": q must be [", p.plan.q_rows, ", ",
-                p.plan.heads, ", head_dim] for this plan.");
+    TORCH_CHECK_VALUE(a.dim >= 1 && a.dim <= RELM_MP_MAX_HEAD_DIM, op, ": head_dim must be in [1, ", RELM_MP_MAX_HEAD_DIM,
+                      "].");
+    TORCH_CHECK_VALUE(q.size(0) == p.plan.q_rows && q.size(1) == p.plan.heads, op, ": q must be [", p.plan.q_rows, ", ",
+                      p.plan.heads, ", head_dim] for this plan.");
     for (const Tensor* t : {&k, &v})
-        TORCH_CHECK(t->size(0) == p.plan.k_rows && t->size(1) == p.plan.kv_heads && t->size(2) == a.dim, op,
-                    ": k and v must be [", p.plan.k_rows, ", ", p.plan.kv_heads, ", ", a.dim, "] for this plan.");
-    TORCH_CHECK(p.table.device() == q.device(), op, ": the plan is on another device.");
+        TORCH_CHECK_VALUE(t->size(0) == p.plan.k_rows && t->size(1) == p.plan.kv_heads && t->size(2) == a.dim, op,
+                          ": k and v must be [", p.plan.k_rows, ", ", p.plan.kv_heads, ", ", a.dim, "] for this plan.");
+    TORCH_CHECK_VALUE(p.table.device() == q.device(), op, ": the plan is on another device.");
     a.q = with_unit_values(q);
     a.k = with_unit_values(k);
     a.v = with_unit_values(v);
-    if (key_mask.has_value() && key_mask->defined()) {
-        TORCH_CHECK(key_mask->dim() == 1 && key_mask->size(0) == p.plan.k_rows && key_mask->scalar_type() == at::kBool &&
-                        key_mask->device() == q.device(),
-                    op, ": key_mask must be bool [", p.plan.k_rows, "] on the device of q.");
-        a.mask = key_mask->contiguous();
+    if (key_mask.defined()) {
+        TORCH_CHECK_VALUE(key_mask.dim() == 1 && key_mask.size(0) == p.plan.k_rows && key_mask.scalar_type() == at::kBool &&
+                              key_mask.device() == q.device(),
+                          op, ": key_mask must be bool [", p.plan.k_rows, "] on the device of q.");
+        a.mask = key_mask.contiguous();
     }
     a.scale = static_cast<float>(scale);
+    TORCH_CHECK_VALUE(a.scale > 0.0f && a.scale < std::numeric_limits<float>::infinity(), op,
+                      ": scale must be finite and positive.");
     return a;
 }
 
-}  // namespace
-
-// (out, lse); lse is empty unless `keep`.
-std::tuple<Tensor, Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
-                                           const c10::intrusive_ptr<AttentionPlan>& plan,
-                                           const std::optional<Tensor>& key_mask, double scale, bool keep) {
-    const AttnArgs a = attention_args(q, k, v, *plan, key_mask, scale, "cross_attention");
+// (out, lse); lse only if kept.
+std::tuple<Tensor, Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionPlan& plan,
+                                             const Tensor& key_mask, double scale, bool keep) {
+    const AttnArgs a = attention_args(q, k, v, plan, key_mask, scale);
     c10::OptionalDeviceGuard guard(q.device());
-    plan->used_on(c10::hip::getCurrentHIPStream(q.get_device()));
-    Tensor out = at::empty(q.sizes(), q.options());
-    Tensor lse = keep ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))
-                      : at::empty({0}, q.options().dtype(at::kFloat));
-    const size_t need = relm_mp_cross_attention_workspace_size(&plan->plan, a.dim);
+    const auto stream = c10::hip::getCurrentHIPStream(q.get_device());
+    plan.used_on(stream);
+    Tensor out = at::empty(q.sizes(), q.options()), lse;
+    if (keep) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    const size_t need = relm_mp_cross_attention_workspace_size(&plan.plan, a.dim);
     const Tensor ws = need > 0 ? bytes(need, q) : Tensor();
     const relm_mp_head_rows qr = head_rows(a.q), kr = head_rows(a.k), vr = head_rows(a.v);
-    raise_if(relm_mp_cross_attention(a.dtype, &plan->plan, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale, out.data_ptr(),
+    raise_if(relm_mp_cross_attention(a.dtype, &plan.plan, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale, out.data_ptr(),
                                      keep ? lse.data_ptr<float>() : nullptr, need > 0 ? ws.data_ptr() : nullptr, need,
-                                     current_stream(q)));
+                                     stream.stream()));
     return {out, lse};
 }
 
-std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k,
-                                                            const Tensor& v, const c10::intrusive_ptr<AttentionPlan>& plan,
-                                                            const std::optional<Tensor>& key_mask, double scale,
-                                                            const Tensor& out, const Tensor& lse) {
-    const char* op = "cross_attention_backward";
-    const AttnArgs a = attention_args(q, k, v, *plan, key_mask, scale, op);
-    check_same(grad, q, op, "grad");
-    check_same(out, q, op, "out");
-    TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.dim() == 2 &&
-                    lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
-                op, ": lse must be the forward's, float32 [rows, heads].");
+std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v,
+                                                      const AttentionPlan& plan, const Tensor& key_mask, double scale,
+                                                      const Tensor& out, const Tensor& lse) {
+    const AttnArgs a = attention_args(q, k, v, plan, key_mask, scale);
+    check_same(grad, q, "cross_attention", "its gradient");
     c10::OptionalDeviceGuard guard(q.device());
-    plan->used_on(c10::hip::getCurrentHIPStream(q.get_device()));
-    const Tensor g = with_unit_values(grad), o = out.contiguous(), l = lse.contiguous();
+    const auto stream = c10::hip::getCurrentHIPStream(q.get_device());
+    plan.used_on(stream);
+    const Tensor g = with_unit_values(grad);
     Tensor dq = at::empty(q.sizes(), q.options());
     Tensor dk = at::empty(k.sizes(), k.options());
     Tensor dv = at::empty(v.sizes(), v.options());
-    const size_t need = relm_mp_cross_attention_backward_workspace_size(&plan->plan, a.dim);
+    const size_t need = relm_mp_cross_attention_backward_workspace_size(&plan.plan, a.dim);
     const Tensor ws = bytes(need, q);
     const relm_mp_head_rows gr = head_rows(g), qr = head_rows(a.q), kr = head_rows(a.k), vr = head_rows(a.v);
-    raise_if(relm_mp_cross_attention_backward(a.dtype, &plan->plan, &gr, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale,
-                                              o.const_data_ptr(), l.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
-                                              dv.data_ptr(), ws.data_ptr(), need, current_stream(q)));
+    raise_if(relm_mp_cross_attention_backward(a.dtype, &plan.plan, &gr, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale,
+                                              out.const_data_ptr(), lse.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                                              dv.data_ptr(), ws.data_ptr(), need, stream.stream()));
     return {dq, dk, dv};
+}
+
+// Keeps the inputs, the output and each row's logarithm of its total; the backward
+// computes the probabilities again.
+struct CrossAttention : torch::autograd::Function<CrossAttention> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                          const std::optional<Tensor>& key_mask, const c10::intrusive_ptr<AttentionPlan>& plan,
+                          double scale) {
+        const Tensor mask = key_mask.value_or(Tensor());
+        const auto [out, lse] = attention_forward(q, k, v, *plan, mask, scale, true);
+        ctx->save_for_backward({q, k, v, mask, out, lse});
+        ctx->saved_data["plan"] = plan;
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const auto plan = ctx->saved_data["plan"].toCustomClass<AttentionPlan>();
+        const auto [dq, dk, dv] = attention_backward(grads[0], s[0], s[1], s[2], *plan, s[3],
+                                                     ctx->saved_data["scale"].toDouble(), s[4], s[5]);
+        return once({dq, dk, dv, Tensor(), Tensor(), Tensor()}, "cross_attention");
+    }
+};
+
+}  // namespace
+
+Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t plan, const std::optional<Tensor>& key_mask,
+                       double scale) {
+    const auto p = plan_of(plan, "cross_attention");
+    if (wants_grad({&q, &k, &v})) return CrossAttention::apply(q, k, v, key_mask, p, scale);
+    return std::get<0>(attention_forward(q, k, v, *p, key_mask.value_or(Tensor()), scale, false));
 }
 
 // ---- orthogonalised update ---------------------------------------------------------
@@ -273,7 +406,7 @@ std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(const Tensor& grad, 
 // One result per update; updates of more than two dimensions are stacks of matrices.
 std::vector<Tensor> orthogonalise(at::TensorList updates, int64_t steps, at::ArrayRef<double> coefficients, double eps) {
     const char* op = "orthogonalise";
-    TORCH_CHECK(coefficients.size() == 3, op, ": three coefficients expected.");
+    TORCH_CHECK_VALUE(coefficients.size() == 3, op, ": three coefficients expected.");
     std::vector<Tensor> inputs, results;
     if (updates.empty()) return results;
     const int dtype = value_dtype(updates[0], op, "every update");
@@ -284,7 +417,7 @@ std::vector<Tensor> orthogonalise(at::TensorList updates, int64_t steps, at::Arr
     mats.reserve(updates.size());
     for (const Tensor& u : updates) {
         check_like(u, updates[0], op, "every update");
-        TORCH_CHECK(u.dim() >= 2, op, ": updates must be matrices or stacks of them.");
+        TORCH_CHECK_VALUE(u.dim() >= 2, op, ": updates must be matrices or stacks of them.");
         const int64_t rows = u.size(-2), cols = u.size(-1);
         const bool rows_apart = u.dim() == 2 && (cols <= 1 || u.stride(1) == 1) && (rows <= 1 || u.stride(0) >= cols);
         inputs.push_back(rows_apart ? u : u.contiguous());
@@ -311,22 +444,20 @@ std::vector<Tensor> orthogonalise(at::TensorList updates, int64_t steps, at::Arr
 }  // namespace relm_amd
 
 TORCH_LIBRARY_FRAGMENT(relm_mp, m) {
-    m.def("add_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps, bool keep) -> (Tensor, Tensor, Tensor)");
+    m.def("add_rms_norm(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor)");
+    m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");
     m.def("add_rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
-    m.def("add_rms_norm_backward(Tensor grad_y, Tensor? grad_h, Tensor h, Tensor weight, Tensor rstd) -> (Tensor, Tensor)");
     m.class_<relm_amd::readout::AttentionPlan>("AttentionPlan");
-    m.def("attention_plan(Tensor q_offsets, Tensor k_offsets, int heads, int kv_heads) -> __torch__.torch.classes.relm_mp.AttentionPlan");
-    m.def("cross_attention(Tensor q, Tensor k, Tensor v, __torch__.torch.classes.relm_mp.AttentionPlan plan, Tensor? key_mask, float scale, bool keep) -> (Tensor, Tensor)");
-    m.def("cross_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, __torch__.torch.classes.relm_mp.AttentionPlan plan, Tensor? key_mask, float scale, Tensor out, Tensor lse) -> (Tensor, Tensor, Tensor)");
+    m.def("attention_plan(Tensor q_offsets, Tensor k_offsets, int heads, int kv_heads) -> (__torch__.torch.classes.relm_mp.AttentionPlan, int)");
+    m.def("cross_attention(Tensor q, Tensor k, Tensor v, int plan, Tensor? key_mask, float scale) -> Tensor");
     m.def("orthogonalise(Tensor[] updates, int steps, float[] coefficients, float eps) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(relm_mp, CompositeImplicitAutograd, m) {
     m.impl("add_rms_norm", relm_amd::readout::add_rms_norm);
+    m.impl("rms_norm", relm_amd::readout::rms_norm);
     m.impl("add_rms_norm_fp8", relm_amd::readout::add_rms_norm_fp8);
-    m.impl("add_rms_norm_backward", relm_amd::readout::add_rms_norm_backward);
     m.impl("attention_plan", relm_amd::readout::attention_plan);
     m.impl("cross_attention", relm_amd::readout::cross_attention);
-    m.impl("cross_attention_backward", relm_amd::readout::cross_attention_backward);
     m.impl("orthogonalise", relm_amd::readout::orthogonalise);
 }

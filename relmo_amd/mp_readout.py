@@ -2,15 +2,15 @@
 
 ``add_rms_norm`` (a residual stream's norm, also with an 8-bit output),
 ``cross_attention`` (per-graph queries to the graphs' objects) and ``orthogonalise``
-(the weight updates of what they train), without counterparts in relmo.  GPU tensors of float32, bfloat16 or float16 run the
-library's kernels through autograd functions; CPU tensors (and the policy's
-fallback) run the ATen formulations below, which autograd differentiates.
+(the weight updates of what they train), without counterparts in relmo.  GPU tensors of float32, bfloat16 or float16 run the library's ops, which check
+their arguments and make their own autograd nodes; CPU tensors (and the policy's fallback)
+run the ATen formulations below, which autograd differentiates.
 """
 
 from __future__ import annotations
 
 from .mp_dispatch import library_op
-from .mp_runtime import ops_namespace, torch
+from .mp_runtime import torch
 
 FP8_MAX = 448.0
 
@@ -40,77 +40,33 @@ def _norm_float(x, residual, weight, eps: float):
     return h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * weight.to(wide), h
 
 
-if torch is not None:
-
-    class _AddRmsNormFunction(torch.autograd.Function):
-        """(y, h); the backward reads h, rounded as it was stored, and the rows' 1 / root."""
-
-        @staticmethod
-        def forward(ctx, x, residual, weight, eps):
-            y, h, rstd = ops_namespace().add_rms_norm(x, residual, weight, eps, True)
-            ctx.set_materialize_grads(False)
-            ctx.save_for_backward(h, weight, rstd)
-            return y, h
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, grad_y, grad_h):
-            h, weight, rstd = ctx.saved_tensors
-            if grad_y is None:
-                return grad_h, grad_h, None, None
-            dx, dw = ops_namespace().add_rms_norm_backward(grad_y, grad_h, h, weight, rstd)
-            return dx, dx, dw, None
-
-    class _RmsNormFunction(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, weight, eps):
-            y, _h, rstd = ops_namespace().add_rms_norm(x, None, weight, eps, True)
-            ctx.save_for_backward(x, weight, rstd)
-            return y
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, grad_y):
-            x, weight, rstd = ctx.saved_tensors
-            dx, dw = ops_namespace().add_rms_norm_backward(grad_y, None, x, weight, rstd)
-            return dx, dw, None
-
-else:  # pragma: no cover - torch missing
-    _AddRmsNormFunction = _RmsNormFunction = None
-
-
 def add_rms_norm(x, residual, weight, eps: float):
     if residual is None:
         return rms_norm(x, weight, eps), x
-    _norm_checks("add_rms_norm", x, residual, weight)
     op = library_op("add_rms_norm", tensor=x, gpu_only=True)
-    if op is None:
-        y, h = _norm_float(x, residual, weight, eps)
-        return y.to(x.dtype), h.to(x.dtype)
-    if _wants_grad(x, residual, weight):
-        return _AddRmsNormFunction.apply(x, residual, weight, float(eps))
-    y, h, _rstd = op(x, residual, weight, float(eps), False)
-    return y, h
+    if op is not None:
+        return op(x, residual, weight, eps)
+    _norm_checks("add_rms_norm", x, residual, weight)
+    y, h = _norm_float(x, residual, weight, eps)
+    return y.to(x.dtype), h.to(x.dtype)
 
 
 def rms_norm(x, weight, eps: float):
+    op = library_op("rms_norm", tensor=x, gpu_only=True)
+    if op is not None:
+        return op(x, weight, eps)
     _norm_checks("rms_norm", x, None, weight)
-    op = library_op("add_rms_norm", tensor=x, gpu_only=True)
-    if op is None:
-        return _norm_float(x, None, weight, eps)[0].to(x.dtype)
-    if _wants_grad(x, weight):
-        return _RmsNormFunction.apply(x, weight, float(eps))
-    return op(x, None, weight, float(eps), False)[0]
+    return _norm_float(x, None, weight, eps)[0].to(x.dtype)
 
 
 def add_rms_norm_fp8(x, residual, weight, eps: float):
-    _norm_checks("add_rms_norm_fp8", x, residual, weight)
     if _wants_grad(x, residual, weight):
         raise RuntimeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad(), or add_rms_norm to train.")
     op = library_op("add_rms_norm_fp8", tensor=x, gpu_only=True)
     if op is not None:
-        q, scale, h = op(x, residual, weight, float(eps))
+        q, scale, h = op(x, residual, weight, eps)
         return q, scale, x if residual is None else h
+    _norm_checks("add_rms_norm_fp8", x, residual, weight)
     y, h = _norm_float(x, residual, weight, eps)
     scale = (y.abs().amax(-1) if x.size(-1) else y.new_zeros(x.shape[:-1])) / FP8_MAX
     scale = torch.where(scale == 0, torch.ones_like(scale), scale).to(torch.float32)
@@ -124,9 +80,11 @@ def add_rms_norm_fp8(x, residual, weight, eps: float):
 class AttentionPlan:
     """The lengths of a batch's graphs and, on the GPU, how their attention is laid over the device."""
 
-    def __init__(self, q_offsets, k_offsets, heads: int, kv_heads: int, ref=None):
+    def __init__(self, q_offsets, k_offsets, heads: int, kv_heads: int, ref=None, number: int | None = None):
         self.q_offsets, self.k_offsets = q_offsets, k_offsets
-        self.heads, self.kv_heads, self.ref = heads, kv_heads, ref
+        self.heads, self.kv_heads = heads, kv_heads
+        self._ref = ref        # keeps the library's plan, which the op finds by its number
+        self.number = number
 
 
 def attention_plan(q_offsets, k_offsets, heads: int, kv_heads: int | None) -> AttentionPlan:
@@ -139,7 +97,7 @@ def attention_plan(q_offsets, k_offsets, heads: int, kv_heads: int | None) -> At
             raise ValueError(f"attention_plan expects {name} to be int64 [graphs + 1].")
     op = library_op("attention_plan", tensor=q_offsets, gpu_only=True)
     if op is not None:
-        return AttentionPlan(q_offsets, k_offsets, heads, kv_heads, op(q_offsets, k_offsets, heads, kv_heads))
+        return AttentionPlan(q_offsets, k_offsets, heads, kv_heads, *op(q_offsets, k_offsets, heads, kv_heads))
     for name, t in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
         if int(t[0]) != 0 or bool((t[1:] < t[:-1]).any()):
             raise RuntimeError(f"relm_mp attention plan: {name} must ascend from 0.")
@@ -185,41 +143,16 @@ def cross_attention_python(q, k, v, plan, key_mask, scale: float):
     return torch.cat(outs).to(q.dtype)
 
 
-if torch is not None:
-
-    class _CrossAttentionFunction(torch.autograd.Function):
-        """Keeps the inputs, the output and each row's logarithm of its total; the backward
-        computes the probabilities again."""
-
-        @staticmethod
-        def forward(ctx, q, k, v, plan, key_mask, scale):
-            out, lse = ops_namespace().cross_attention(q, k, v, plan, key_mask, scale, True)
-            ctx.plan, ctx.scale = plan, scale
-            ctx.save_for_backward(q, k, v, key_mask, out, lse)
-            return out
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, grad):
-            q, k, v, key_mask, out, lse = ctx.saved_tensors
-            dq, dk, dv = ops_namespace().cross_attention_backward(grad, q, k, v, ctx.plan, key_mask, ctx.scale, out, lse)
-            return dq, dk, dv, None, None, None
-
-else:  # pragma: no cover - torch missing
-    _CrossAttentionFunction = None
-
-
 def cross_attention(q, k, v, plan, key_mask, scale: float | None):
-    scale = q.size(-1) ** -0.5 if scale is None and q.size(-1) else float(1.0 if scale is None else scale)
-    _attention_checks(q, k, v, plan, key_mask, scale)
+    if scale is None:
+        scale = max(q.size(-1), 1) ** -0.5
     op = library_op("cross_attention", tensor=q, gpu_only=True)
     if op is None:
+        _attention_checks(q, k, v, plan, key_mask, scale)
         return cross_attention_python(q, k, v, plan, key_mask, scale)
-    if plan.ref is None:
+    if plan.number is None:
         raise ValueError("cross_attention expects a plan made from offsets on the GPU.")
-    if _wants_grad(q, k, v):
-        return _CrossAttentionFunction.apply(q, k, v, plan.ref, key_mask, scale)
-    return op(q, k, v, plan.ref, key_mask, scale, False)[0]
+    return op(q, k, v, plan.number, key_mask, scale)
 
 
 # ---- orthogonalised update ---------------------------------------------------------

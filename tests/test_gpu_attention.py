@@ -324,6 +324,21 @@ def test_plan_keeps_its_own_lengths_and_serves_other_streams() -> None:
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_the_plan_lives_as_long_as_its_graph_and_second_derivatives_raise() -> None:
+    from relmo_amd import mp
+
+    q, k, v, grad, _ = _make([3], [40], 1, 1, 16, torch.float32)
+    plan = mp.attention_plan(_offsets([3]), _offsets([40]), 1)
+    want = _run(q, k, v, grad, plan, None)
+    x = q.detach().requires_grad_(True)
+    out = mp.cross_attention(x, k, v, plan)
+    del plan
+    (gx,) = torch.autograd.grad(out, x, grad, create_graph=True)
+    assert torch.equal(gx, want[1])
+    with pytest.raises(RuntimeError, match="twice"):
+        gx.sum().backward()
+
+
 def test_empty_batches() -> None:
     from relmo_amd import mp
 
@@ -347,9 +362,9 @@ def test_refusals() -> None:
         mp.attention_plan(o, o, 4, 3)
     plan = mp.attention_plan(o, o, 2)
     x = torch.ones(8, 2, 16, device=DEV)
-    with pytest.raises(RuntimeError, match="q must be"):
+    with pytest.raises(ValueError, match="q must be"):
         mp.cross_attention(x[:7], x, x, plan)
-    with pytest.raises(RuntimeError, match="k and v must be"):
+    with pytest.raises(ValueError, match="k and v must be"):
         mp.cross_attention(x, x[:7], x[:7], plan)
     with pytest.raises(ValueError, match="dtype"):
         mp.cross_attention(x, x.bfloat16(), x, plan)
@@ -361,9 +376,13 @@ def test_refusals() -> None:
         with pytest.raises(ValueError, match="scale"):
             mp.cross_attention(x, x, x, plan, scale=scale)
     big = torch.ones(8, 2, 129, device=DEV)
-    with pytest.raises(RuntimeError, match="head_dim"):
+    with pytest.raises(ValueError, match="head_dim"):
         mp.cross_attention(big, big, big, plan)
     with pytest.raises(ValueError, match="GPU"):
         mp.cross_attention(x, x, x, mp.attention_plan(o.cpu(), o.cpu(), 2))
+    number = plan.number
+    del plan
+    with pytest.raises(ValueError, match="no longer exists"):
+        torch.ops.relm_mp.cross_attention(x, x, x, number, None, 1.0)
     rc = capi.lib().relm_mp_cross_attention(capi.F32, None, None, None, None, 16, None, 1.0, None, None, None, 0, None)
     assert rc == capi.ERR_INVALID_ARGUMENT and "plan" in capi.last_error()
