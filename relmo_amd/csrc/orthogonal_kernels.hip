@@ -354,15 +354,19 @@ __global__ __launch_bounds__(kThreads) void k_ortho_split(OrthoBatch batch, Orth
 
 enum Product { kGram, kSquare, kUpdate };
 
-// A tile of one of the three products of a step: BT x BT entries, 4 waves of (BT / 2)^2,
-// depth 32 at a time through two LDS buffers while the next is on its way in registers.
-// Bound by the matrix instructions: per depth of 32 a wave of the 128-tile runs 48 of
-// them (768 cycles) for 16 LDS reads of 1 KB.
+// A tile of one of the three products of a step: BT x BT entries, 4 waves of (BT / 2)^2, a
+// stage of depth 32 at a time.  While a stage is multiplied from registers, the next one's
+// fragments come from LDS, the one after it goes from registers to LDS and the third is on
+// its way from memory: one barrier a stage.  Bound by the matrix instructions: a wave of the
+// 128-tile runs 48 of them (768 cycles) a stage beside 16 LDS reads and 8 writes of 1 KB.
 template <typename T, int PRODUCT, int BT>
 __global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
-    constexpr int MT = BT / 32, ST = 40;  // row of 32 halves and 16 bytes
-    constexpr int kUnits = BT * 4 * 2 * 2 / kThreads;  // 16-byte units of a thread: rows x 4 x planes x operands
-    __shared__ __align__(16) f16 lds[2][2][2][BT * ST];  // [buffer][operand][plane]
+    constexpr int MT = BT / 32;
+    constexpr int kRounds = BT * 4 / kThreads;  // 16-byte units of a thread per operand and plane
+    // [buffer][operand][plane]: rows of 32 halves, their four 16-byte units exchanged by row
+    // (unit u of row r lies at u ^ (r / 2 % 4)): eight neighbouring lanes then read or write
+    // all banks once, along a row and down the rows
+    __shared__ __align__(16) f16 lds[2][2][2][BT * 32];
     // the tile's matrix
     const int64_t flat = xcd_tile(blockIdx.x, gridDim.x);
     int which = 0;
@@ -403,54 +407,103 @@ __global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, Or
     const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave, l = lane_id(), g = l / 16, c16 = l % 16;
     const int wr = (wave / 2) * (BT / 2), wc = (wave % 2) * (BT / 2);
 
-    // unit u of the thread: row u / 4 of an operand's plane, values 8 (u % 4) .. + 8
-    const f16* from[kUnits];
-    int to[kUnits];
+    // rows past the matrix read its last one: their results are not stored
+    const f16* const from[2][2] = {{p.hi + r0 * p.stride, p.lo + r0 * p.stride}, {q.hi + c0 * q.stride, q.lo + c0 * q.stride}};
+    uint32_t offset[2][kRounds];
+    int to[kRounds];
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        const int u = i * kThreads + tid;
-        const int row = (u / 4) % BT, col = (u % 4) * 8, plane = (u / (4 * BT)) % 2, operand = u / (8 * BT);
-        const Planes& o = operand == 0 ? p : q;
-        // rows past the matrix read its last one: their results are not stored
-        const int64_t src = operand == 0 ? min(r0 + row, d.m - 1) : min(c0 + row, q_rows - 1);
-        from[i] = (plane == 0 ? o.hi : o.lo) + src * o.stride + col;
-        to[i] = (operand * 2 + plane) * (BT * ST) + row * ST + col;
+    for (int i = 0; i < kRounds; ++i) {
+        const int row = (i * kThreads + tid) / 4, unit = tid % 4;
+        offset[0][i] = static_cast<uint32_t>(min(row, d.m - 1 - r0) * p.stride + unit * 8);
+        offset[1][i] = static_cast<uint32_t>(min(row, q_rows - 1 - c0) * q.stride + unit * 8);
+        to[i] = row * 32 + (unit ^ (row / 2 % 4)) * 8;
     }
-    Half8 next[kUnits];
+    Half8 next[2][2][kRounds];
     auto fetch = [&](int k) {
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) next[i] = *reinterpret_cast<const Half8*>(from[i] + k);
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < kRounds; ++i)
+                    next[o][h][i] = *reinterpret_cast<const Half8*>(from[o][h] + k + offset[o][i]);
     };
     auto settle = [&](int buffer) {
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) *reinterpret_cast<Half8*>(&lds[buffer][0][0][0] + to[i]) = next[i];
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < kRounds; ++i) *reinterpret_cast<Half8*>(&lds[buffer][o][h][to[i]]) = next[o][h][i];
     };
     f32x4 acc[MT][MT];
 #pragma unroll
     for (int r = 0; r < MT; ++r)
 #pragma unroll
         for (int c = 0; c < MT; ++c) acc[r][c] = f32x4(0.0f);
-    fetch(0);
-    settle(0);
-    __syncthreads();
-    for (int k = 0; k < depth; k += 32) {
-        const int buffer = (k / 32) & 1;
-        if (k + 32 < depth) fetch(k + 32);
+    struct Stage {
         Half8 fh[MT], fl[MT], gh[MT], gl[MT];
+    } even, odd;
+    const int at = c16 * 32 + (g ^ (c16 / 2 % 4)) * 8;  // of the lane's unit within 16 rows
+    auto read = [&](Stage& f, int buffer) {
 #pragma unroll
         for (int r = 0; r < MT; ++r) {
-            fh[r] = lds_frag<f16>(lds[buffer][0][0], ST, wr + 16 * r + c16, 8 * g);
-            fl[r] = lds_frag<f16>(lds[buffer][0][1], ST, wr + 16 * r + c16, 8 * g);
-            gh[r] = lds_frag<f16>(lds[buffer][1][0], ST, wc + 16 * r + c16, 8 * g);
-            gl[r] = lds_frag<f16>(lds[buffer][1][1], ST, wc + 16 * r + c16, 8 * g);
+            f.fh[r] = *reinterpret_cast<const Half8*>(&lds[buffer][0][0][(wr + 16 * r) * 32 + at]);
+            f.fl[r] = *reinterpret_cast<const Half8*>(&lds[buffer][0][1][(wr + 16 * r) * 32 + at]);
+            f.gh[r] = *reinterpret_cast<const Half8*>(&lds[buffer][1][0][(wc + 16 * r) * 32 + at]);
+            f.gl[r] = *reinterpret_cast<const Half8*>(&lds[buffer][1][1][(wc + 16 * r) * 32 + at]);
         }
+    };
+    auto multiply = [&](const Stage& f) {  // the small terms first
 #pragma unroll
         for (int r = 0; r < MT; ++r)
 #pragma unroll
-            for (int c = 0; c < MT; ++c) acc[r][c] = mma_pairs(fh[r], fl[r], gh[c], gl[c], acc[r][c]);
-        if (k + 32 < depth) settle(buffer ^ 1);
+            for (int c = 0; c < MT; ++c) acc[r][c] = mma<f16>(f.fl[r], f.gh[c], acc[r][c]);
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+            for (int c = 0; c < MT; ++c) acc[r][c] = mma<f16>(f.fh[r], f.gl[c], acc[r][c]);
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+            for (int c = 0; c < MT; ++c) acc[r][c] = mma<f16>(f.fh[r], f.gh[c], acc[r][c]);
+    };
+    const int stages = depth / 32;
+    // Stage s, whose fragments are in `now`.  Past the last stage the reads, writes and loads
+    // repeat it, unused, so that a pass has no branch and its instructions mix: one LDS or
+    // memory access to every two matrix instructions, in this order.
+    auto pass = [&](int s, const Stage& now, Stage& next_stage) {
+        read(next_stage, (s + 1) & 1);
+        multiply(now);
+        settle(s & 1);  // the buffer of stage s, which all have read
+        fetch(32 * min(s + 3, stages - 1));
+#pragma unroll
+        for (int i = 0; i < 4 * MT; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       // LDS read
+            __builtin_amdgcn_sched_group_barrier(0x008, MT / 2, 0);  // matrix instructions
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * kRounds; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // LDS write
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // load
+            __builtin_amdgcn_sched_group_barrier(0x008, MT * MT * 3 / (4 * kRounds) - MT * MT / (2 * kRounds), 0);
+        }
         __syncthreads();
+    };
+    fetch(0);
+    settle(0);
+    fetch(32 * min(1, stages - 1));
+    __syncthreads();
+    read(even, 0);
+    settle(1);
+    fetch(32 * min(2, stages - 1));
+    __syncthreads();
+    int s = 0;
+    for (; s + 1 < stages; s += 2) {
+        pass(s, even, odd);
+        pass(s + 1, odd, even);
     }
+    if (s < stages) multiply(even);
 
     const float to_a = rule.scale_a / (d.scale * d.scale), from_b = 1.0f / rule.scale_b;
     const float b_of_a = rule.b * rule.scale_b / rule.scale_a, b_of_aa = rule.c * rule.scale_b / (rule.scale_a * rule.scale_a);
