@@ -15,15 +15,17 @@ struct OrthoMatrix {
     int32_t m, n, mp, np;
     int32_t tall;      // the update is [n, m]
     float scale;       // of X's pairs: a power of two
+    uint64_t inv_cols;      // 2^40 / columns of the update, rounded up: divides indices below 2^21
     int64_t first_tile[2];  // of the symmetric products' and the update's tiles
     int64_t x, xt[2], a, b, partial;  // bytes into the workspace
 };
 
 // Descriptors travel as kernel arguments (at most 4 KB).
-constexpr int kOrthoBatch = 32;
+constexpr int kOrthoBatch = 28;
 constexpr int kNormParts = 256;  // partial sums of squares of a matrix: a wave adds them
-// Lower tiles of 128 x 128 from which on they are taken instead of 64 x 64 ones.
-constexpr int64_t kLargeTiles = 100;
+// Tiles of 128 x 128 from which on they are taken instead of 64 x 64 ones: of the symmetric
+// products, of the update.
+constexpr int64_t kLargeTiles[2] = {100, 128};
 
 struct OrthoRule {
     float a, b, c, eps;

@@ -58,13 +58,7 @@ __device__ __forceinline__ Half8 lds_frag_split(const f16* tile, int stride, int
     return Half8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// Entry (i, j) of X, the update turned so that it is at least as wide as tall.
-template <typename T>
-__device__ __forceinline__ float entry(const OrthoMatrix& d, int i, int j) {
-    const T* in = static_cast<const T*>(d.in);
-    return static_cast<float>(d.tall ? in[static_cast<int64_t>(j) * d.in_stride + i]
-                                     : in[static_cast<int64_t>(i) * d.in_stride + j]);
-}
+// Entry (i, j) of the result; X is the update turned so that it is at least as wide as tall.
 template <typename T>
 __device__ __forceinline__ void put_entry(const OrthoMatrix& d, int i, int j, float x) {
     T* out = static_cast<T*>(d.out);
@@ -100,13 +94,31 @@ __global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch,
     f16 *xh = pool, *xl = xh + mp * sx, *ah = xl + mp * sx, *al = ah + mp * sa;
     const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave, l = lane_id(), g = l / 16, c16 = l % 16;
 
+    // X starts as zeros: its padding stays
+    for (int u = tid; u < mp * sx / 4; u += kSmallThreads)  // both planes, 8 halves at a time
+        *reinterpret_cast<Half8*>(xh + 8 * u) = Half8(static_cast<f16>(0.0f));
+    // the update twice, kBatch values of a thread in flight: its norm, then its entries
+    constexpr int kBatch = 8;
+    const int cols = d.tall ? m : n, total = m * n;
+    const T* in = static_cast<const T*>(d.in);
+    auto every = [&](auto&& use) {
+        for (int u0 = tid; u0 < total; u0 += kBatch * kSmallThreads) {
+            float x[kBatch];
+            int row[kBatch], col[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int u = min(u0 + k * kSmallThreads, total - 1);
+                row[k] = static_cast<int>((static_cast<uint64_t>(u) * d.inv_cols) >> 40);
+                col[k] = u - row[k] * cols;
+                x[k] = static_cast<float>(in[row[k] * d.in_stride + col[k]]);
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k)
+                if (u0 + k * kSmallThreads < total) use(row[k], col[k], x[k]);
+        }
+    };
     double sum = 0.0;
-    for (int u = tid; u < m * n; u += kSmallThreads) {
-        // along the rows of the update as it lies in memory
-        const int i = d.tall ? u % m : u / n, j = d.tall ? u / m : u % n;
-        const float x = entry<T>(d, i, j);
-        sum += static_cast<double>(x) * static_cast<double>(x);
-    }
+    every([&](int, int, float x) { sum = fma(static_cast<double>(x), static_cast<double>(x), sum); });
     sum = wave_sum(sum);
     if (l == 0) partial[wave] = sum;
     __syncthreads();
@@ -114,12 +126,12 @@ __global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch,
 #pragma unroll
     for (int v = 1; v < kSmallWaves; ++v) sum += partial[v];
     const float scale = static_cast<float>(static_cast<double>(d.scale) / (sqrt(sum) + static_cast<double>(rule.eps)));
-    for (int u = tid; u < mp * np; u += kSmallThreads) {
-        const int i = d.tall ? u % mp : u / np, j = d.tall ? u / mp : u % np;
-        const Pair p = halves(i < m && j < n ? entry<T>(d, i, j) * scale : 0.0f);
-        xh[i * sx + j] = p.hi;
-        xl[i * sx + j] = p.lo;
-    }
+    every([&](int row, int col, float x) {
+        const Pair p = halves(x * scale);
+        const int at = d.tall ? col * sx + row : row * sx + col;
+        xh[at] = p.hi;
+        xl[at] = p.lo;
+    });
     __syncthreads();
 
     const int blocks = mp / 32, lower = blocks * (blocks + 1) / 2;
@@ -261,13 +273,25 @@ __global__ __launch_bounds__(kThreads) void k_ortho_norm(OrthoBatch batch, void*
     const int64_t rows = d.tall ? d.n : d.m;
     const int cols = d.tall ? d.m : d.n;
     const int wave = static_cast<int>(threadIdx.x) / kWave;
+    // rows on dwords are read in 16-byte units, the last one's values past the row as zeros
+    constexpr int V = kLaneValues<T>;
+    const bool whole = reinterpret_cast<uintptr_t>(d.in) % 4 == 0 && d.in_stride * sizeof(T) % 4 == 0;
     double sum = 0.0;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + wave; r < rows;
          r += kNormParts * (kThreads / kWave)) {
         const T* in = static_cast<const T*>(d.in) + r * d.in_stride;
-        for (int c = lane_id(); c < cols; c += kWave) {
-            const double x = static_cast<double>(static_cast<float>(in[c]));
-            sum = fma(x, x, sum);
+        if (whole) {
+#pragma unroll 4
+            for (int c = lane_id() * V; c < cols; c += kWave * V) {
+                const FloatVec<V> x = load_values<T, V>(in, c, cols);
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum);
+            }
+        } else {
+            for (int c = lane_id(); c < cols; c += kWave) {
+                const double x = static_cast<double>(static_cast<float>(in[c]));
+                sum = fma(x, x, sum);
+            }
         }
     }
     sum = wave_sum(sum);
@@ -315,7 +339,9 @@ __global__ __launch_bounds__(kThreads) void k_ortho_split(OrthoBatch batch, Orth
     }
     for (int r = ty; r < 32; r += kThreads / 32) {  // along the update's rows
         const int i = d.tall ? i0 + tx : i0 + r, j = d.tall ? j0 + r : j0 + tx;
-        const float x = i < d.m && j < d.n ? entry<T>(d, i, j) : 0.0f;
+        const T* in = static_cast<const T*>(d.in);
+        const float x = i >= d.m || j >= d.n ? 0.0f
+                                             : static_cast<float>(d.tall ? in[j * d.in_stride + i] : in[i * d.in_stride + j]);
         if (d.tall)
             tile[tx][r] = x;
         else
@@ -360,7 +386,7 @@ enum Product { kGram, kSquare, kUpdate };
 // its way from memory: one barrier a stage.  Bound by the matrix instructions: a wave of the
 // 128-tile runs 48 of them (768 cycles) a stage beside 16 LDS reads and 8 writes of 1 KB.
 template <typename T, int PRODUCT, int BT>
-__global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
+__global__ __launch_bounds__(kThreads, 2) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
     constexpr int MT = BT / 32;
     constexpr int kRounds = BT * 4 / kThreads;  // 16-byte units of a thread per operand and plane
     // [buffer][operand][plane]: rows of 32 halves, their four 16-byte units exchanged by row
@@ -376,9 +402,13 @@ __global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, Or
     const int t = static_cast<int>(flat - d.first_tile[first_of]);
     int ti, tj;
     if constexpr (PRODUCT == kUpdate) {
-        const int rows = (d.m + BT - 1) / BT;
-        ti = t % rows;
-        tj = t / rows;
+        // eight tile rows at a time: the 32 tiles that an XCD has on its CUs then read 8 + 4
+        // operand strips, not 16 + 2
+        constexpr int kStrip = 8;
+        const int rows = (d.m + BT - 1) / BT, cols = (d.n + BT - 1) / BT;
+        const int strip = t / (kStrip * cols), in = t - strip * kStrip * cols, high = min(kStrip, rows - strip * kStrip);
+        tj = in / high;
+        ti = strip * kStrip + in - tj * high;
     } else {  // the lower triangle, row by row
         ti = static_cast<int>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
         while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
@@ -418,23 +448,27 @@ __global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, Or
         offset[1][i] = static_cast<uint32_t>(min(row, q_rows - 1 - c0) * q.stride + unit * 8);
         to[i] = row * 32 + (unit ^ (row / 2 % 4)) * 8;
     }
-    Half8 next[2][2][kRounds];
-    auto fetch = [&](int k) {
+    // stages on their way: two of the small tile's, whose stage is over before a load arrives
+    constexpr int kFlights = BT == 64 ? 2 : 1;
+    struct Flight {
+        Half8 v[2][2][kRounds];
+    } flight[kFlights];
+    auto fetch = [&](Flight& f, int k) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < kRounds; ++i)
-                    next[o][h][i] = *reinterpret_cast<const Half8*>(from[o][h] + k + offset[o][i]);
+                    f.v[o][h][i] = *reinterpret_cast<const Half8*>(from[o][h] + k + offset[o][i]);
     };
-    auto settle = [&](int buffer) {
+    auto settle = [&](const Flight& f, int buffer) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < kRounds; ++i) *reinterpret_cast<Half8*>(&lds[buffer][o][h][to[i]]) = next[o][h][i];
+                for (int i = 0; i < kRounds; ++i) *reinterpret_cast<Half8*>(&lds[buffer][o][h][to[i]]) = f.v[o][h][i];
     };
     f32x4 acc[MT][MT];
 #pragma unroll
@@ -472,11 +506,11 @@ __global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, Or
     // Stage s, whose fragments are in `now`.  Past the last stage the reads, writes and loads
     // repeat it, unused, so that a pass has no branch and its instructions mix: one LDS or
     // memory access to every two matrix instructions, in this order.
-    auto pass = [&](int s, const Stage& now, Stage& next_stage) {
+    auto pass = [&](int s, const Stage& now, Stage& next_stage, Flight& f) {
         read(next_stage, (s + 1) & 1);
         multiply(now);
-        settle(s & 1);  // the buffer of stage s, which all have read
-        fetch(32 * min(s + 3, stages - 1));
+        settle(f, s & 1);  // stage s + 2 into the buffer of stage s, which all have read
+        fetch(f, 32 * min(s + 2 + kFlights, stages - 1));
 #pragma unroll
         for (int i = 0; i < 4 * MT; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       // LDS read
@@ -490,18 +524,20 @@ __global__ __launch_bounds__(kThreads) void k_ortho_product(OrthoBatch batch, Or
         }
         __syncthreads();
     };
-    fetch(0);
-    settle(0);
-    fetch(32 * min(1, stages - 1));
+    Flight &first = flight[0], &second = flight[kFlights - 1];
+    fetch(first, 0);
+    settle(first, 0);
+    fetch(second, 32 * min(1, stages - 1));
+    if constexpr (kFlights == 2) fetch(first, 32 * min(2, stages - 1));
     __syncthreads();
     read(even, 0);
-    settle(1);
-    fetch(32 * min(2, stages - 1));
+    settle(second, 1);
+    fetch(second, 32 * min(1 + kFlights, stages - 1));
     __syncthreads();
     int s = 0;
     for (; s + 1 < stages; s += 2) {
-        pass(s, even, odd);
-        pass(s + 1, odd, even);
+        pass(s, even, odd, first);
+        pass(s + 1, odd, even, second);
     }
     if (s < stages) multiply(even);
 
@@ -583,6 +619,7 @@ OrthoMatrix describe(const relm_mp_update& u, size_t& at) {
     // no more than twice the scale throughout
     const int e = static_cast<int>(std::lround(0.5 * std::log2(static_cast<double>(d.m) * static_cast<double>(d.n))));
     d.scale = std::ldexp(1.0f, std::min(e, 13));
+    d.inv_cols = ((uint64_t{1} << 40) + u.cols - 1) / u.cols;
     if (is_small(d.mp, d.np)) return d;
     const auto take = [&](size_t bytes) {
         const size_t p = at;
@@ -599,31 +636,24 @@ OrthoMatrix describe(const relm_mp_update& u, size_t& at) {
     return d;
 }
 
-template <typename T, int BT>
-hipError_t large_steps(const OrthoBatch& b, const OrthoRule& rule, int count, int64_t lower, int64_t all, void* ws,
-                       hipStream_t st) {
-    for (int step = 0; step < rule.steps; ++step) {
-        hipLaunchKernelGGL((k_ortho_product<T, kGram, BT>), dim3(static_cast<unsigned>(lower)), dim3(kThreads), 0, st, b, rule,
-                           count, step, ws);
-        hipLaunchKernelGGL((k_ortho_product<T, kSquare, BT>), dim3(static_cast<unsigned>(lower)), dim3(kThreads), 0, st, b,
-                           rule, count, step, ws);
-        hipLaunchKernelGGL((k_ortho_product<T, kUpdate, BT>), dim3(static_cast<unsigned>(all)), dim3(kThreads), 0, st, b, rule,
-                           count, step, ws);
-    }
-    return hipGetLastError();
-}
-
-// Numbers the tiles of a launch's matrices.
-void number_tiles(OrthoBatch& b, int count, int64_t bt, int64_t& lower, int64_t& all) {
-    lower = all = 0;
+// Numbers the tiles of one kind (0: the lower ones of a symmetric product, 1: the update's)
+// of a launch's matrices; their count.
+int64_t number_tiles(OrthoBatch& b, int count, int64_t bt, int kind) {
+    int64_t at = 0;
     for (int i = 0; i < count; ++i) {
         OrthoMatrix& d = b.mat[i];
-        d.first_tile[0] = lower;
-        d.first_tile[1] = all;
+        d.first_tile[kind] = at;
         const int64_t r = ceil_div(d.m, bt), c = ceil_div(d.n, bt);
-        lower += r * (r + 1) / 2;
-        all += r * c;
+        at += kind == 0 ? r * (r + 1) / 2 : r * c;
     }
+    return at;
+}
+
+template <typename T, int PRODUCT>
+void product(const OrthoBatch& b, const OrthoRule& rule, int count, int step, bool large, int64_t tiles, void* ws,
+             hipStream_t st) {
+    const auto kernel = large ? k_ortho_product<T, PRODUCT, 128> : k_ortho_product<T, PRODUCT, 64>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, st, b, rule, count, step, ws);
 }
 
 template <typename T>
@@ -653,16 +683,18 @@ hipError_t run(const std::vector<OrthoMatrix>& small, const std::vector<OrthoMat
         }
         hipLaunchKernelGGL(k_ortho_norm<T>, dim3(kNormParts, count), dim3(kThreads), 0, st, b, ws);
         hipLaunchKernelGGL(k_ortho_split<T>, dim3(np / 32, mp / 32, count), dim3(kThreads), 0, st, b, rule, ws);
-        int64_t lower, all;
-        number_tiles(b, count, 128, lower, all);
-        hipError_t e;
-        if (lower >= kLargeTiles) {
-            e = large_steps<T, 128>(b, rule, count, lower, all, ws, st);
-        } else {
-            number_tiles(b, count, 64, lower, all);
-            e = large_steps<T, 64>(b, rule, count, lower, all, ws, st);
+        int64_t tiles[2];
+        bool wide[2];
+        for (int kind = 0; kind < 2; ++kind) {
+            tiles[kind] = number_tiles(b, count, 128, kind);
+            wide[kind] = tiles[kind] >= kLargeTiles[kind];
+            if (!wide[kind]) tiles[kind] = number_tiles(b, count, 64, kind);
         }
-        if (e != hipSuccess) return e;
+        for (int step = 0; step < rule.steps; ++step) {
+            product<T, kGram>(b, rule, count, step, wide[0], tiles[0], ws, st);
+            product<T, kSquare>(b, rule, count, step, wide[0], tiles[0], ws, st);
+            product<T, kUpdate>(b, rule, count, step, wide[1], tiles[1], ws, st);
+        }
     }
     return hipGetLastError();
 }
