@@ -92,7 +92,8 @@ __global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch,
     const int m = d.m, n = d.n, mp = d.mp, np = d.np;
     const int sx = np + 8, sa = mp + 8;  // strides: rows spread over the banks
     f16 *xh = pool, *xl = xh + mp * sx, *ah = xl + mp * sx, *al = ah + mp * sa;
-    const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave, l = lane_id(), g = l / 16, c16 = l % 16;
+    const int tid = static_cast<int>(threadIdx.x), l = lane_id(), g = l / 16, c16 = l % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
 
     // X starts as zeros: its padding stays
     for (int u = tid; u < mp * sx / 4; u += kSmallThreads)  // both planes, 8 halves at a time
@@ -226,34 +227,53 @@ __global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch,
         }
         __syncthreads();
         // X <- a X + B X: 16 columns of X depend on themselves and B alone, so each is one
-        // wave's, in place
+        // wave's, in place: all products, then all entries.  The products are transposed (X's
+        // columns down), so that a lane holds four neighbours of a row of X.
+        const bool last = step + 1 == rule.steps;
         for (int strip = wave; strip < np / 16; strip += kSmallWaves) {
-            Half8 fh[4], fl[4];
+            f32x4 acc[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k < blocks) {
-                    fh[k] = lds_frag_t<f16>(xh, sx, 32 * k, 16 * strip);
-                    fl[k] = lds_frag_t<f16>(xl, sx, 32 * k, 16 * strip);
+            for (int r = 0; r < 8; ++r) acc[r] = f32x4(0.0f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (k >= blocks) break;
+                const Half8 fh = lds_frag_t<f16>(xh, sx, 32 * k, 16 * strip), fl = lds_frag_t<f16>(xl, sx, 32 * k, 16 * strip);
+#pragma unroll
+                for (int r = 0; r < 8; r += 2) {
+                    if (r >= 2 * blocks) break;
+                    const Half8 bh0 = lds_frag_split(ah, sa, 16 * r + c16, 32 * k), bl0 = lds_frag_split(al, sa, 16 * r + c16, 32 * k);
+                    const Half8 bh1 = lds_frag_split(ah, sa, 16 * r + 16 + c16, 32 * k),
+                                bl1 = lds_frag_split(al, sa, 16 * r + 16 + c16, 32 * k);
+                    acc[r] = mma<f16>(fl, bh0, acc[r]);
+                    acc[r + 1] = mma<f16>(fl, bh1, acc[r + 1]);
+                    acc[r] = mma<f16>(fh, bl0, acc[r]);
+                    acc[r + 1] = mma<f16>(fh, bl1, acc[r + 1]);
+                    acc[r] = mma<f16>(fh, bh0, acc[r]);
+                    acc[r + 1] = mma<f16>(fh, bh1, acc[r + 1]);
                 }
-            const bool last = step + 1 == rule.steps;
-            for (int r = 0; r < mp / 16; ++r) {
-                f32x4 acc = f32x4(0.0f);
+            }
+            const int col = 16 * strip + 4 * g;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k < blocks)
-                        acc = mma_pairs(lds_frag_split(ah, sa, 16 * r + c16, 32 * k), lds_frag_split(al, sa, 16 * r + c16, 32 * k),
-                                        fh[k], fl[k], acc);
+            for (int r = 0; r < 8; ++r) {
+                if (r >= 2 * blocks) break;
+                const int row = 16 * r + c16;
+                f16 *to_h = xh + row * sx + col, *to_l = xl + row * sx + col;
+                Half4 hi = *reinterpret_cast<const Half4*>(to_h), lo = *reinterpret_cast<const Half4*>(to_l);
+                f32x4 y;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = 16 * r + 4 * g + i, col = 16 * strip + c16, at = row * sx + col;
-                    const float x = fmaf(rule.a, whole(xh[at], xl[at]), acc[i] * from_b);
-                    if (!last) {
-                        const Pair p = halves(x);
-                        xh[at] = p.hi;
-                        xl[at] = p.lo;
-                    } else if (row < m && col < n) {
-                        put_entry<T>(d, row, col, x / d.scale);
-                    }
+                    y[i] = fmaf(rule.a, whole(hi[i], lo[i]), acc[r][i] * from_b);
+                    const Pair p = halves(y[i]);
+                    hi[i] = p.hi;
+                    lo[i] = p.lo;
+                }
+                if (!last) {
+                    *reinterpret_cast<Half4*>(to_h) = hi;
+                    *reinterpret_cast<Half4*>(to_l) = lo;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (row < m && col + i < n) put_entry<T>(d, row, col + i, y[i] / d.scale);
                 }
             }
         }
@@ -602,10 +622,23 @@ size_t small_bytes(int64_t mp, int64_t np) { return static_cast<size_t>(2 * mp *
 
 constexpr size_t kSmallLds = 160 * 1024 - 256;  // a CU's, less the kernel's own
 
-bool is_small(int64_t mp, int64_t np) { return mp <= 128 && np <= 16384 && small_bytes(mp, np) <= kSmallLds; }
+bool is_small(const relm_mp_update& u) {
+    const int64_t mp = ceil_div(std::min(u.rows, u.cols), 32) * 32, np = ceil_div(std::max(u.rows, u.cols), 32) * 32;
+    return mp <= 128 && np <= 16384 && small_bytes(mp, np) <= kSmallLds;
+}
 
-// Sizes of a matrix; its planes from `at` on in the workspace (large ones).
-OrthoMatrix describe(const relm_mp_update& u, size_t& at) {
+// Whether matrices that would fit a workgroup go with the larger ones: where there are some
+// and one launch holds them all, their tiles cost nothing beside the others', and the launch
+// of their own is saved (two of 398 x 11 beside four of up to 398 x 387: 48 of 190 us).
+bool small_join(const relm_mp_update* updates, int32_t count) {
+    if (count > kOrthoBatch) return false;
+    for (int32_t i = 0; i < count; ++i)
+        if (updates[i].rows > 0 && updates[i].cols > 0 && !is_small(updates[i])) return true;
+    return false;
+}
+
+// Sizes of a matrix; its planes from `at` on in the workspace unless it is `small`.
+OrthoMatrix describe(const relm_mp_update& u, bool small, size_t& at) {
     OrthoMatrix d{};
     d.in = u.in;
     d.out = u.out;
@@ -620,7 +653,7 @@ OrthoMatrix describe(const relm_mp_update& u, size_t& at) {
     const int e = static_cast<int>(std::lround(0.5 * std::log2(static_cast<double>(d.m) * static_cast<double>(d.n))));
     d.scale = std::ldexp(1.0f, std::min(e, 13));
     d.inv_cols = ((uint64_t{1} << 40) + u.cols - 1) / u.cols;
-    if (is_small(d.mp, d.np)) return d;
+    if (small) return d;
     const auto take = [&](size_t bytes) {
         const size_t p = at;
         at = align_up(at + bytes, 256);
@@ -703,8 +736,9 @@ hipError_t run(const std::vector<OrthoMatrix>& small, const std::vector<OrthoMat
 
 size_t orthogonalise_workspace(const relm_mp_update* updates, int32_t count) {
     size_t at = 0;
+    const bool join = small_join(updates, count);
     for (int32_t i = 0; i < count; ++i)
-        if (updates[i].rows > 0 && updates[i].cols > 0) describe(updates[i], at);
+        if (updates[i].rows > 0 && updates[i].cols > 0) describe(updates[i], !join && is_small(updates[i]), at);
     return at;
 }
 
@@ -712,10 +746,11 @@ hipError_t launch_orthogonalise(int dtype, const relm_mp_update* updates, int32_
                                 hipStream_t st) {
     std::vector<OrthoMatrix> small, large;
     size_t at = 0;
+    const bool join = small_join(updates, count);
     for (int32_t i = 0; i < count; ++i) {
         if (updates[i].rows == 0 || updates[i].cols == 0) continue;
-        const OrthoMatrix d = describe(updates[i], at);
-        (is_small(d.mp, d.np) ? small : large).push_back(d);
+        const bool fits = !join && is_small(updates[i]);
+        (fits ? small : large).push_back(describe(updates[i], fits, at));
     }
     hipError_t e = hipErrorInvalidValue;
     with_value_type(dtype, [&](auto t) { e = run<decltype(t)>(small, large, rule, ws, st); });

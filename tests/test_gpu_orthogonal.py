@@ -108,10 +108,21 @@ def test_lists_of_many_shapes_equal_single_calls() -> None:
     shapes = SHAPES[:-1] + [(n, 2 * n) for n in range(1, 45)] + [(130 + n, 140) for n in range(35)]
     updates = [torch.randn(*s, device=DEV, generator=g) for s in shapes]
     for got, u in zip(mp.orthogonalise(updates), updates):
-        # tile sizes go by the launch's matrices: equal up to the sums' order
+        # tiles go by the launch's matrices: equal up to the sums' order
         alone = mp.orthogonalise(u)
         assert float((got - alone).norm()) <= 2 * _allowed(u.shape) * float(alone.norm())
-        assert u.size(0) > 128 or u.size(1) > 128 or torch.equal(got, alone)
+
+
+def test_small_matrices_beside_a_large_one() -> None:
+    """They go through the tiles of the large one's launches, stay apart from it, and come out as alone up to the
+    sums' order."""
+    from relmo_amd import mp
+
+    g = _gen(11)
+    shapes = [(398, 387), (398, 11), (1, 1), (5, 300), (128, 128), (31, 33), (96, 96)]
+    updates = [torch.randn(*s, device=DEV, generator=g) for s in shapes]
+    for got, u in zip(mp.orthogonalise(updates), updates):
+        _check(got, u)
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e15, 3e30])
