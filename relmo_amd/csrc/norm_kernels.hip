@@ -27,10 +27,30 @@ constexpr int kThreads = 256;
 constexpr float kFp8Max = 448.0f;  // largest finite e4m3 value
 
 // A row belongs to a group of L lanes (part of a wave up to 64, else the
-// workgroup); each lane holds NV units of V neighbouring values, unit i of lane l
-// at column (i * L + l) * V, so a group reads L * 16 bytes side by side.  NV = 0:
-// rows of any width, walked in units that are read again for the second pass
-// (from the caches: the first pass has just read them).
+// workgroup); each lane holds NV units of V neighbouring values, V a divisor of the
+// width, unit i of lane l at column (i * L + l) * V, so a group reads L * V values side
+// by side.  Lanes past the row read its first unit as zeros: a load under a branch
+// would wait for the one before it.  NV = 0: rows of any width, walked in units that
+// are read again for the second pass (from the caches: the first pass has just read
+// them).
+template <typename T, int V>
+__device__ __forceinline__ FloatVec<V> load_unit(const T* __restrict__ row, int64_t col, int64_t width) {
+    const bool live = col < width;
+    const ValueVec<T, V> v = *reinterpret_cast<const ValueVec<T, V>*>(row + (live ? col : 0));
+    FloatVec<V> x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = live ? static_cast<float>(v[i]) : 0.0f;
+    return x;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_unit(T* __restrict__ row, int64_t col, int64_t width, FloatVec<V> x) {
+    ValueVec<T, V> v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = round_to<T>(x[i]);
+    if (col < width) *reinterpret_cast<ValueVec<T, V>*>(row + col) = v;
+}
+
 template <int L>
 constexpr int kGroups = kThreads / L;
 
@@ -74,29 +94,28 @@ __device__ __forceinline__ float square_sum(FloatVec<V> v, float sum) {
     return sum;
 }
 
-// V values rounded to e4m3 (nearest even; the row's scale keeps them within range).
+// V values rounded to e4m3 (nearest even; the row's scale keeps them within range).  A
+// row's bytes start anywhere: units of 4 and 8 are stored whole where they lie on dwords.
 template <int V>
 __device__ __forceinline__ void store_fp8(uint8_t* row, int64_t col, int64_t width, FloatVec<V> v) {
+    if (col >= width) return;
     if constexpr (V % 4 == 0) {
-        if (col + V <= width) {
-            uint32_t word[V / 4];
+        uint32_t word[V / 4];
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) {
-                int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0, false);
-                w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3], w, true);
-                word[j] = static_cast<uint32_t>(w);
-            }
-            if (((reinterpret_cast<uintptr_t>(row) + col) & 3) == 0) {
+        for (int j = 0; j < V / 4; ++j) {
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3], w, true);
+            word[j] = static_cast<uint32_t>(w);
+        }
+        if (((reinterpret_cast<uintptr_t>(row) + col) & 3) == 0) {
 #pragma unroll
-                for (int j = 0; j < V / 4; ++j) reinterpret_cast<uint32_t*>(row + col)[j] = word[j];
-                return;
-            }
+            for (int j = 0; j < V / 4; ++j) reinterpret_cast<uint32_t*>(row + col)[j] = word[j];
+            return;
         }
     }
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        if (col + j < width)
-            row[col + j] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[j], 0.0f, 0, false) & 0xff);
+        row[col + j] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[j], 0.0f, 0, false) & 0xff);
 }
 
 struct NormArgs {
@@ -114,7 +133,7 @@ struct NormArgs {
 
 // Bound by memory: x, r, y and h move once (the weight stays in registers over
 // the rows of a group).
-template <typename T, int V, int NV, int L, bool FP8>
+template <typename T, int V, int NV, int L, bool FP8, bool RESIDUAL>
 __global__ __launch_bounds__(kThreads) void k_norm(NormArgs a) {
     __shared__ float lds[kThreads / kWave];
     constexpr int NR = NV == 0 ? 1 : NV;
@@ -126,19 +145,19 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs a) {
     FloatVec<V> wv[NR];
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) wv[i] = load_values<T, V>(w, static_cast<int64_t>(i * L + lane) * V, a.width);
+        for (int i = 0; i < NV; ++i) wv[i] = load_unit<T, V>(w, static_cast<int64_t>(i * L + lane) * V, a.width);
     }
     // groups of a workgroup walk the same number of rows: the barriers inside the
     // sums of whole-workgroup groups (L == kThreads: one group) stay together
     for (int64_t row = group; row < a.rows; row += step) {
         const T* x = static_cast<const T*>(a.x) + row * a.width;
-        const T* r = a.r != nullptr ? static_cast<const T*>(a.r) + row * a.width : nullptr;
+        const T* r = static_cast<const T*>(a.r) + (RESIDUAL ? row * a.width : 0);
         T* h = a.h != nullptr ? static_cast<T*>(a.h) + row * a.width : nullptr;
         FloatVec<V> v[NR];
         float sum = 0.0f;
         auto take = [&](int64_t col) {
-            FloatVec<V> s = load_values<T, V>(x, col, a.width);
-            if (r != nullptr) s += load_values<T, V>(r, col, a.width);
+            FloatVec<V> s = load_unit<T, V>(x, col, a.width);
+            if constexpr (RESIDUAL) s += load_unit<T, V>(r, col, a.width);
             return s;
         };
         if constexpr (NV > 0) {
@@ -146,14 +165,14 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs a) {
             for (int i = 0; i < NV; ++i) v[i] = take(static_cast<int64_t>(i * L + lane) * V);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                if (h != nullptr) store_values<T, V>(h, static_cast<int64_t>(i * L + lane) * V, a.width, v[i]);
+                if (h != nullptr) store_unit<T, V>(h, static_cast<int64_t>(i * L + lane) * V, a.width, v[i]);
                 sum = square_sum<V>(v[i], sum);
             }
         } else {
             for (int64_t i = 0; i < units; ++i) {
                 const int64_t col = (i * L + lane) * V;
                 const FloatVec<V> s = take(col);
-                if (h != nullptr) store_values<T, V>(h, col, a.width, s);
+                if (h != nullptr) store_unit<T, V>(h, col, a.width, s);
                 sum = square_sum<V>(s, sum);
             }
         }
@@ -163,16 +182,16 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs a) {
         auto result = [&](int64_t i) {  // unit i of y
             const int64_t col = (i * L + lane) * V;
             if constexpr (NV > 0) return v[i] * rstd * wv[i];
-            return take(col) * rstd * load_values<T, V>(w, col, a.width);
+            return take(col) * rstd * load_unit<T, V>(w, col, a.width);
         };
         if constexpr (!FP8) {
             T* y = static_cast<T*>(a.y) + row * a.width;
             if constexpr (NV > 0) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    store_values<T, V>(y, static_cast<int64_t>(i * L + lane) * V, a.width, result(i));
+                    store_unit<T, V>(y, static_cast<int64_t>(i * L + lane) * V, a.width, result(i));
             } else {
-                for (int64_t i = 0; i < units; ++i) store_values<T, V>(y, (i * L + lane) * V, a.width, result(i));
+                for (int64_t i = 0; i < units; ++i) store_unit<T, V>(y, (i * L + lane) * V, a.width, result(i));
             }
         } else {
             uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.width;
@@ -231,7 +250,7 @@ struct NormBackwardArgs {
 // the weight gradient over the rows of its group in registers; the groups of a
 // workgroup add theirs through LDS in group order, the workgroups in
 // k_norm_fold: no atomics, the same result every time.
-template <typename T, int V, int NV, int L>
+template <typename T, int V, int NV, int L, bool DH>
 __global__ __launch_bounds__(kThreads) void k_norm_backward(NormBackwardArgs a) {
     __shared__ float lds[kThreads / kWave];
     constexpr int NR = NV == 0 ? 1 : NV;
@@ -245,13 +264,13 @@ __global__ __launch_bounds__(kThreads) void k_norm_backward(NormBackwardArgs a) 
     if constexpr (NV > 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            wv[i] = load_values<T, V>(w, static_cast<int64_t>(i * L + lane) * V, a.width);
+            wv[i] = load_unit<T, V>(w, static_cast<int64_t>(i * L + lane) * V, a.width);
             sum_w[i] = FloatVec<V>(0.0f);
         }
     }
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups<L> + group; row < a.rows; row += step) {
         const T* dy = static_cast<const T*>(a.dy) + row * a.width;
-        const T* dh = a.dh != nullptr ? static_cast<const T*>(a.dh) + row * a.width : nullptr;
+        const T* dh = static_cast<const T*>(a.dh) + (DH ? row * a.width : 0);
         const T* h = static_cast<const T*>(a.h) + row * a.width;
         T* dx = static_cast<T*>(a.dx) + row * a.width;
         const float rstd = a.rstd[row];
@@ -264,16 +283,19 @@ __global__ __launch_bounds__(kThreads) void k_norm_backward(NormBackwardArgs a) 
             FloatVec<V> o;
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = fmaf(rstd, dn[j] - n[j] * dot, g[j]);
-            store_values<T, V>(dx, col, a.width, o);
+            store_unit<T, V>(dx, col, a.width, o);
         };
         if constexpr (NV > 0) {
             FloatVec<V> d[NV], n[NV], g[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int64_t col = static_cast<int64_t>(i * L + lane) * V;
-                d[i] = load_values<T, V>(dy, col, a.width);
-                n[i] = load_values<T, V>(h, col, a.width);
-                g[i] = dh != nullptr ? load_values<T, V>(dh, col, a.width) : FloatVec<V>(0.0f);
+                d[i] = load_unit<T, V>(dy, col, a.width);
+                n[i] = load_unit<T, V>(h, col, a.width);
+                if constexpr (DH)
+                    g[i] = load_unit<T, V>(dh, col, a.width);
+                else
+                    g[i] = FloatVec<V>(0.0f);
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -289,15 +311,16 @@ __global__ __launch_bounds__(kThreads) void k_norm_backward(NormBackwardArgs a) 
         } else {
             for (int64_t i = 0; i < units; ++i) {
                 const int64_t col = (i * L + lane) * V;
-                dots(load_values<T, V>(dy, col, a.width) * load_values<T, V>(w, col, a.width),
-                     load_values<T, V>(h, col, a.width) * rstd);
+                dots(load_unit<T, V>(dy, col, a.width) * load_unit<T, V>(w, col, a.width),
+                     load_unit<T, V>(h, col, a.width) * rstd);
             }
             dot = group_sum<L>(dot, lds) * share;
             for (int64_t i = 0; i < units; ++i) {
                 const int64_t col = (i * L + lane) * V;
-                finish(col, load_values<T, V>(dy, col, a.width) * load_values<T, V>(w, col, a.width),
-                       load_values<T, V>(h, col, a.width) * rstd,
-                       dh != nullptr ? load_values<T, V>(dh, col, a.width) : FloatVec<V>(0.0f));
+                FloatVec<V> g = FloatVec<V>(0.0f);
+                if constexpr (DH) g = load_unit<T, V>(dh, col, a.width);
+                finish(col, load_unit<T, V>(dy, col, a.width) * load_unit<T, V>(w, col, a.width),
+                       load_unit<T, V>(h, col, a.width) * rstd, g);
             }
         }
     }
@@ -305,7 +328,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_backward(NormBackwardArgs a) 
         if constexpr (L == kThreads) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                store_values<float, V>(a.partial + blockIdx.x * a.width, static_cast<int64_t>(i * L + lane) * V, a.width,
+                store_unit<float, V>(a.partial + blockIdx.x * a.width, static_cast<int64_t>(i * L + lane) * V, a.width,
                                        sum_w[i]);
         } else {
             __shared__ float part[kThreads * NV * V];
@@ -364,18 +387,27 @@ __global__ __launch_bounds__(kFoldCols * kFoldRows) void k_norm_fold(const float
 constexpr int64_t kMaxBlocks = 1024;
 constexpr int64_t kLongRows = 64;  // rows of a workgroup of k_norm_weight_partial, at least
 
-// Whether rows are read in 16-byte units: every row of every array starts on a
-// dword (else a lane takes one value at a time).
+// Values of a lane's unit: 16 bytes where they divide the row and every row of every
+// array starts on a dword, else a dword, else one value.
 template <typename T>
-bool whole_units(int64_t width, std::initializer_list<const void*> arrays) {
-    if (sizeof(T) * width % 4 != 0) return false;
-    for (const void* p : arrays)
-        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return false;
-    return true;
+int unit_values(int64_t width, std::initializer_list<const void*> arrays) {
+    bool dwords = sizeof(T) * width % 4 == 0;
+    for (const void* p : arrays) dwords = dwords && reinterpret_cast<uintptr_t>(p) % 4 == 0;
+    if (!dwords) return 1;
+    return width % kLaneValues<T> == 0 ? kLaneValues<T> : 4 / static_cast<int>(sizeof(T));
+}
+template <typename T, typename F>
+void with_unit(int values, F&& f) {
+    if (values == kLaneValues<T>)
+        f(std::integral_constant<int, kLaneValues<T>>{});
+    else if (sizeof(T) < 4 && values == 2)
+        f(std::integral_constant<int, sizeof(T) < 4 ? 2 : 1>{});
+    else
+        f(std::integral_constant<int, 1>{});
 }
 
 // Lanes of a row and units of a lane for `units` units: the fewest lanes that
-// hold a row in one unit each, up to a wave (then two and four units, and the
+// hold a row in one unit each, up to a wave (then two to four units, and the
 // workgroup's lanes from 257 units on, four of each at most).  nv = 0: walked.
 struct NormShape {
     int lanes;
@@ -387,6 +419,7 @@ NormShape norm_shape(int64_t units) {
     if (units <= 32) return {32, 1};
     if (units <= 64) return {64, 1};
     if (units <= 128) return {64, 2};
+    if (units <= 192) return {64, 3};
     if (units <= 256) return {64, 4};
     if (units <= 512) return {kThreads, 2};
     if (units <= 1024) return {kThreads, 4};
@@ -406,6 +439,7 @@ void with_shape(NormShape s, F&& f) {
     RELM_SHAPE(32, 1)
     RELM_SHAPE(64, 1)
     RELM_SHAPE(64, 2)
+    RELM_SHAPE(64, 3)
     RELM_SHAPE(64, 4)
     RELM_SHAPE(kThreads, 2)
     RELM_SHAPE(kThreads, 4)
@@ -420,10 +454,9 @@ hipError_t norm_forward(const NormArgs& a, bool fp8, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + groups - 1) / groups, 256 * 32)));
     with_shape(s, [&](auto l, auto n) {
         constexpr int L = decltype(l)::value, NV = decltype(n)::value;
-        if (fp8)
-            hipLaunchKernelGGL((k_norm<T, V, NV, L, true>), grid, dim3(kThreads), 0, st, a);
-        else
-            hipLaunchKernelGGL((k_norm<T, V, NV, L, false>), grid, dim3(kThreads), 0, st, a);
+        const auto kernel = a.r != nullptr ? (fp8 ? k_norm<T, V, NV, L, true, true> : k_norm<T, V, NV, L, false, true>)
+                                           : (fp8 ? k_norm<T, V, NV, L, true, false> : k_norm<T, V, NV, L, false, false>);
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, a);
     });
     return hipGetLastError();
 }
@@ -443,7 +476,8 @@ hipError_t norm_backward(NormBackwardArgs a, void* dw, hipStream_t st) {
     with_shape(s, [&](auto l, auto n) {
         constexpr int L = decltype(l)::value, NV = decltype(n)::value;
         const int64_t grid = NV > 0 ? blocks : std::min<int64_t>(a.rows, 256 * 8);
-        hipLaunchKernelGGL((k_norm_backward<T, V, NV, L>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
+        const auto kernel = a.dh != nullptr ? k_norm_backward<T, V, NV, L, true> : k_norm_backward<T, V, NV, L, false>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
     });
     if (s.nv == 0) {
         const int64_t per_block = (a.rows + blocks - 1) / blocks;
@@ -465,9 +499,8 @@ hipError_t launch_add_rms_norm(int dtype, const void* x, const void* r, const vo
     const NormArgs a{x, r, w, y, h, scale, rstd, rows, width, eps};
     with_value_type(dtype, [&](auto t) {
         using T = decltype(t);
-        e = whole_units<T>(width, {x, r, w, scale != nullptr ? nullptr : y, h})
-                ? norm_forward<T, kLaneValues<T>>(a, scale != nullptr, st)
-                : norm_forward<T, 1>(a, scale != nullptr, st);
+        with_unit<T>(unit_values<T>(width, {x, r, w, scale != nullptr ? nullptr : y, h}),
+                     [&](auto v) { e = norm_forward<T, decltype(v)::value>(a, scale != nullptr, st); });
     });
     return e;
 }
@@ -475,9 +508,9 @@ hipError_t launch_add_rms_norm(int dtype, const void* x, const void* r, const vo
 size_t add_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t width) {
     if (rows <= 0 || width <= 0) return 0;
     int64_t blocks = 0;
-    with_value_type(dtype, [&](auto t) {  // of either unit: the arrays' addresses choose later
-        constexpr int V = kLaneValues<decltype(t)>;
-        blocks = std::max(backward_blocks(rows, (width + V - 1) / V), backward_blocks(rows, width));
+    with_value_type(dtype, [&](auto t) {  // of any unit: the arrays' addresses choose later
+        for (const int v : {kLaneValues<decltype(t)>, 2, 1})
+            blocks = std::max(blocks, backward_blocks(rows, (width + v - 1) / v));
     });
     return static_cast<size_t>(blocks * width) * sizeof(float);
 }
@@ -496,8 +529,8 @@ hipError_t launch_add_rms_norm_backward(int dtype, const void* dy, const void* d
             e = hipGetLastError();
             return;
         }
-        e = whole_units<T>(width, {dy, dh, h, w, dx}) ? norm_backward<T, kLaneValues<T>>(a, dw, st)
-                                                      : norm_backward<T, 1>(a, dw, st);
+        with_unit<T>(unit_values<T>(width, {dy, dh, h, w, dx}),
+                     [&](auto v) { e = norm_backward<T, decltype(v)::value>(a, dw, st); });
     });
     return e;
 }

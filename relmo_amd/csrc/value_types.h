@@ -50,22 +50,6 @@ __device__ __forceinline__ FloatVec<N> load_values(const T* __restrict__ row, in
     return x;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void store_values(T* __restrict__ row, int64_t col, int64_t width, FloatVec<N> x) {
-    if constexpr (N == 1) {
-        if (col < width) row[col] = round_to<T>(x[0]);
-    } else if (col + N <= width) {
-        ValueVec<T, N> v;
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = round_to<T>(x[i]);
-        *reinterpret_cast<ValueVec<T, N>*>(row + col) = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (col + i < width) row[col + i] = round_to<T>(x[i]);
-    }
-}
-
 // Calls f with a value of the type that a dtype code stands for; false where it
 // stands for none of them.
 template <typename F>
