@@ -45,35 +45,50 @@ Rows<T> rows_of(const relm_mp_head_rows& r) {
     return {static_cast<const T*>(r.data), r.row_stride, r.head_stride};
 }
 
-// Whether every row of every head starts on a dword.
-bool on_dwords(const relm_mp_head_rows& r, size_t value) {
-    return reinterpret_cast<uintptr_t>(r.data) % 4 == 0 && r.row_stride * value % 4 == 0 && r.head_stride * value % 4 == 0;
-}
+// Units of 16 bytes of a row of `dim` values, from column `col` on, zero past its end: one
+// access each, wherever rows start.  A unit that lies past the row is its first; one that
+// ends past it (kCut: 8 does not divide dim) is read ending with the row and moved down
+// after (settle_unit: 3 to 6% of a kernel's time, so rows of whole units have kernels without
+// it).  Rows of fewer than 8 values (kShort) go value by value.  Nothing branches: loads on
+// both sides of a branch would wait for one another.
+enum Fit { kShort, kCut, kWhole };
 
-// N values of T of a row of `dim` at p, from column `col` on, zero past its end.  WHOLE: 8
-// divides dim and every row of every operand starts on a dword, so 16-byte accesses serve;
-// else value by value.  Neither way branches: loads on both sides of a branch would wait
-// for one another.
+template <typename T>
+constexpr int kUnit = 16 / static_cast<int>(sizeof(T));
 template <typename T, int N>
 using Values = T __attribute__((ext_vector_type(N)));
+template <typename T>
+using Unit = Values<T, kUnit<T>>;
 
-template <typename T, int N, bool WHOLE>
-__device__ __forceinline__ Values<T, N> take(const T* p, int col, int dim) {
-    Values<T, N> v;
-    const bool live = col < dim;
-    if constexpr (WHOLE) {
-        const T* at = p + (live ? col : 0);
-        constexpr int M = N * sizeof(T) <= 16 ? N : 16 / sizeof(T);
-#pragma unroll
-        for (int c = 0; c < N / M; ++c) {
-            const ValueVec<T, M> part = *reinterpret_cast<const ValueVec<T, M>*>(at + c * M);
-#pragma unroll
-            for (int j = 0; j < M; ++j) v[c * M + j] = part[j];
-        }
-        if (!live) v = Values<T, N>(static_cast<T>(0.0f));
+template <typename T, int FIT>
+__device__ __forceinline__ Unit<T> load_unit(const T* p, int col, int dim) {
+    constexpr int N = kUnit<T>;
+    if constexpr (FIT != kShort) {
+        return *reinterpret_cast<const ValueVec<T, N>*>(p + (col < dim ? min(col, dim - N) : 0));
     } else {
+        Unit<T> v;
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = p[min(col + j, dim - 1)];
+        return v;
+    }
+}
+
+template <typename T, int FIT>
+__device__ __forceinline__ Unit<T> settle_unit(Unit<T> v, int col, int dim) {
+    constexpr int N = kUnit<T>;
+    if constexpr (FIT != kShort) {
+        if constexpr (FIT == kCut) {
+            const int down = (col < dim ? max(col + N - dim, 0) : 0) * static_cast<int>(8 * sizeof(T));  // bits
+            struct Words {
+                uint64_t lo, hi;
+            } w = __builtin_bit_cast(Words, v);
+            const uint64_t carried = down == 0 ? 0 : w.hi << ((64 - down) & 63);
+            w.lo = down >= 64 ? w.hi >> (down & 63) : (w.lo >> (down & 63)) | carried;
+            w.hi = down >= 64 ? 0 : w.hi >> (down & 63);
+            v = __builtin_bit_cast(Unit<T>, w);
+        }
+        if (col >= dim) v = Unit<T>(static_cast<T>(0.0f));
+    } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
             if (col + j >= dim) v[j] = static_cast<T>(0.0f);
@@ -82,8 +97,8 @@ __device__ __forceinline__ Values<T, N> take(const T* p, int col, int dim) {
 }
 
 template <typename T>
-__device__ __forceinline__ void put4(T* p, int col, int dim, bool whole, f32x4 x) {
-    if (whole && col + 4 <= dim) {
+__device__ __forceinline__ void put4(T* p, int col, int dim, f32x4 x) {
+    if (col + 4 <= dim) {
         ValueVec<T, 4> v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = round_to<T>(x[j]);
@@ -113,7 +128,6 @@ struct Args {
     float* parts;        // sums of the parts, rows of part_stride floats
     float* part_stats;   // forward: their maxima and totals
     int part_stride;
-    bool out_whole;  // rows of head_dim values side by side start on dwords
 };
 
 // A workgroup's item and key head.  Neighbouring heads of an item share the lines of
@@ -147,31 +161,30 @@ constexpr int kLdsStride = DP + 16 / static_cast<int>(sizeof(T));
 
 template <typename T, int DP, int BN>
 struct TileLoad {
-    static constexpr int kV = 16 / static_cast<int>(sizeof(T));
-    static constexpr int kUnits = DP / kV;               // of a row
+    static constexpr int kUnits = DP / kUnit<T>;         // of a row
     static constexpr int kStep = kThreads / kUnits;      // rows of a round
     static constexpr int kRounds = BN / kStep;
     static_assert(kThreads % kUnits == 0 && BN % kStep == 0, "whole rounds");
-    Values<T, kV> v[kRounds];
+    Unit<T> v[kRounds];
 
     static __device__ __forceinline__ int first_row() { return static_cast<int>(threadIdx.x) / kUnits; }
-    static __device__ __forceinline__ int column() { return (static_cast<int>(threadIdx.x) % kUnits) * kV; }
+    static __device__ __forceinline__ int column() { return (static_cast<int>(threadIdx.x) % kUnits) * kUnit<T>; }
 
     // place(row): where a row of the tile lies (some row that exists for one that does not)
-    template <bool WHOLE, typename F>
+    template <int FIT, typename F>
     __device__ __forceinline__ void fetch(F&& place, int dim) {
 #pragma unroll
-        for (int i = 0; i < kRounds; ++i) v[i] = take<T, kV, WHOLE>(place(first_row() + i * kStep), column(), dim);
+        for (int i = 0; i < kRounds; ++i) v[i] = load_unit<T, FIT>(place(first_row() + i * kStep), column(), dim);
     }
     // Into LDS; unless `all` rows enter, those that keep(row) leaves out as zeros.
-    template <typename F>
-    __device__ __forceinline__ void store(T* tile, bool all, F&& keep) const {
+    template <int FIT, typename F>
+    __device__ __forceinline__ void store(T* tile, int dim, bool all, F&& keep) const {
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
             const int row = first_row() + i * kStep;
-            Values<T, kV> x = v[i];
-            if (!all && !keep(row)) x = Values<T, kV>(static_cast<T>(0.0f));
-            *reinterpret_cast<Values<T, kV>*>(tile + row * kLdsStride<T, DP> + column()) = x;
+            Unit<T> x = settle_unit<T, FIT>(v[i], column(), dim);
+            if (!all && !keep(row)) x = Unit<T>(static_cast<T>(0.0f));
+            *reinterpret_cast<Unit<T>*>(tile + row * kLdsStride<T, DP> + column()) = x;
         }
     }
 };
@@ -203,11 +216,23 @@ struct KeyBits {
 template <typename T, int DP>
 struct RowFrags {
     Frag<T> f[DP / 32];
-    template <bool WHOLE>
+    template <int FIT>
     __device__ __forceinline__ void fetch(const T* p, int dim) {
         const int g = lane_id() / 16;
+        constexpr int N = kUnit<T>;
+        Unit<T> u[DP / 32][8 / N];
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) f[c] = take<T, 8, WHOLE>(p, c * 32 + g * 8, dim);
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int h = 0; h < 8 / N; ++h) u[c][h] = load_unit<T, FIT>(p, c * 32 + g * 8 + h * N, dim);
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int h = 0; h < 8 / N; ++h) {
+                const Unit<T> x = settle_unit<T, FIT>(u[c][h], c * 32 + g * 8 + h * N, dim);
+#pragma unroll
+                for (int j = 0; j < N; ++j) f[c][h * N + j] = x[j];
+            }
     }
 };
 
@@ -264,7 +289,7 @@ struct RowShape {
 
 // Forward.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with the running maximum m:
 // when a key tile raises it, what has been added up is scaled by exp(m_old - m_new).
-template <typename T, int DP, int RT, int WM, bool WHOLE>
+template <typename T, int DP, int RT, int WM, int FIT>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T> a) {
     using S = RowShape<RT, WM>;
     constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
@@ -288,7 +313,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
         real[r] = row < w.it.rows;
         at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
         // a row past the item reads its first: a column of the scores, used by no other
-        qf[r].template fetch<WHOLE>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
+        qf[r].template fetch<FIT>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
     }
     f32x4 o[RT][ND];
     float m[RT], total[RT];
@@ -307,16 +332,16 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
         const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
         const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
         const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
-        kl.template fetch<WHOLE>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
-        vl.template fetch<WHOLE>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
+        kl.template fetch<FIT>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
+        vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         __syncthreads();
-        kl.store(kt, bits.all(), [&](int row) { return bits.has(row); });
-        vl.store(vt, bits.all(), [&](int row) { return bits.has(row); });
+        kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         if (threadIdx.x < BN) starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
         __syncthreads();
         if (k0 + BN < w.it.keys) fetch(k0 + BN);
@@ -378,7 +403,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
     const auto finish = [&](int row, Place p, int col, f32x4 sum, float top, float sum_p) {
         if (w.it.part < 0) {
             const float inv = sum_p == 0.0f ? 0.0f : 1.0f / sum_p;
-            put4<T>(a.out + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * inv);
+            put4<T>(a.out + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * inv);
             if (col == 0 && a.lse != nullptr)
                 a.lse[p.row * a.heads + p.head] = sum_p == 0.0f ? -kInf : (top + log2f(sum_p)) * kLn2;
         } else {
@@ -503,9 +528,9 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
     const Place p = place_of(a, j.q_first, head, j.row0 + row);
     T* to = (DQ ? a.dq : a.out) + (p.row * a.heads + p.head) * a.dim;
     if constexpr (DQ) {
-        put4<T>(to, col, a.dim, a.out_whole, sum * a.scale);
+        put4<T>(to, col, a.dim, sum * a.scale);
     } else {
-        put4<T>(to, col, a.dim, a.out_whole, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+        put4<T>(to, col, a.dim, sum * (total == 0.0f ? 0.0f : 1.0f / total));
         if (col == 0 && a.lse != nullptr)
             a.lse[p.row * a.heads + p.head] = total == 0.0f ? -kInf : (top + log2f(total)) * kLn2;
     }
@@ -561,7 +586,7 @@ __device__ __forceinline__ float lse2_of(float lse) { return lse == -kInf ? kInf
 
 // dq of a row item: like the forward, with the probabilities recomputed from lse.  The
 // item over a row's first keys also leaves its delta for the key kernel.
-template <typename T, int DP, int RT, int WM, bool WHOLE>
+template <typename T, int DP, int RT, int WM, int FIT>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Args<T> a) {
     using S = RowShape<RT, WM>;
     constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
@@ -586,10 +611,10 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         const int row = (row_wave * RT + r) * 16 + l % 16;
         real[r] = row < w.it.rows;
         at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
-        qf[r].template fetch<WHOLE>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
-        gf[r].template fetch<WHOLE>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
+        qf[r].template fetch<FIT>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
+        gf[r].template fetch<FIT>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
         RowFrags<T, DP> of;
-        of.template fetch<WHOLE>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
+        of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
         float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c)
@@ -610,16 +635,16 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
         const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
         const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
-        kl.template fetch<WHOLE>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
-        vl.template fetch<WHOLE>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
+        kl.template fetch<FIT>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
+        vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         __syncthreads();
-        kl.store(kt, bits.all(), [&](int row) { return bits.has(row); });
-        vl.store(vt, bits.all(), [&](int row) { return bits.has(row); });
+        kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         if (threadIdx.x < BN) starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
         __syncthreads();
         if (k0 + BN < w.it.keys) fetch(k0 + BN);
@@ -653,7 +678,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         for (int n = 0; n < ND; ++n) dq[r][n] *= 1.0f / unit[r];
     const auto finish = [&](int row, Place p, int col, f32x4 sum) {
         if (w.it.part < 0) {
-            put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * a.scale);
+            put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * a.scale);
         } else {
             const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
             if (col < a.part_stride) *reinterpret_cast<f32x4*>(a.parts + slot * a.part_stride + col) = sum;
@@ -695,7 +720,7 @@ constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
 // dk and dv of a key item: a wave keeps KT tiles of 16 keys and walks the graph's rows
 // (rows down, keys across, so that a lane's probabilities are the operand of the products
 // over rows).
-template <typename T, int DP, int KT, bool WHOLE>
+template <typename T, int DP, int KT, int FIT>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Args<T> a) {
     constexpr int BR = 64, ST = kLdsStride<T, DP>, ND = DP / 16;
     __shared__ __align__(16) T qt[BR * ST];
@@ -721,8 +746,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         real[t] = key < w.it.keys;
         const int64_t at = static_cast<int64_t>(w.it.key_first) + min(key, w.it.keys - 1);
         const bool kept = real[t] && (a.key_mask == nullptr || a.key_mask[at] != 0);
-        kf[t].template fetch<WHOLE>(a.k.data + at * a.k.row_stride + head * a.k.head_stride, a.dim);
-        vf[t].template fetch<WHOLE>(a.v.data + at * a.v.row_stride + head * a.v.head_stride, a.dim);
+        kf[t].template fetch<FIT>(a.k.data + at * a.k.row_stride + head * a.k.head_stride, a.dim);
+        vf[t].template fetch<FIT>(a.v.data + at * a.v.row_stride + head * a.v.head_stride, a.dim);
         if (!kept) {
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) kf[t].f[c] = vf[t].f[c] = Frag<T>(static_cast<T>(0.0f));
@@ -738,11 +763,11 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
     const auto fetch = [&](int r0) {
         const int left = w.it.rows - r0;
         const auto place = [&](int row) { return place_of(a, w.it.q_first, head, w.it.row0 + r0 + min(row, left - 1)); };
-        ql.template fetch<WHOLE>([&](int row) {
+        ql.template fetch<FIT>([&](int row) {
             const Place p = place(row);
             return a.q.data + p.row * a.q.row_stride + p.head * a.q.head_stride;
         }, a.dim);
-        gl.template fetch<WHOLE>([&](int row) {
+        gl.template fetch<FIT>([&](int row) {
             const Place p = place(row);
             return a.grad.data + p.row * a.grad.row_stride + p.head * a.grad.head_stride;
         }, a.dim);
@@ -756,8 +781,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
     for (int r0 = 0; r0 < w.it.rows; r0 += BR) {
         __syncthreads();
         const int left = w.it.rows - r0;
-        ql.store(qt, left >= BR, [&](int row) { return row < left; });
-        gl.store(gt, left >= BR, [&](int row) { return row < left; });
+        ql.template store<FIT>(qt, a.dim, left >= BR, [&](int row) { return row < left; });
+        gl.template store<FIT>(gt, a.dim, left >= BR, [&](int row) { return row < left; });
         if (threadIdx.x < BR) {
             row_lse2[threadIdx.x] = lse_in;
             row_delta[threadIdx.x] = delta_in;
@@ -827,8 +852,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
             const int col = n * 16 + g * 4;
             dk[t][n] *= 1.0f / unit[t];
             if (w.it.part < 0) {
-                put4<T>(a.dk + at * a.dim, col, a.dim, a.out_whole, dk[t][n] * a.scale);
-                put4<T>(a.dv + at * a.dim, col, a.dim, a.out_whole, dv[t][n] * (1.0f / kProbabilityUnit<T>));
+                put4<T>(a.dk + at * a.dim, col, a.dim, dk[t][n] * a.scale);
+                put4<T>(a.dv + at * a.dim, col, a.dim, dv[t][n] * (1.0f / kProbabilityUnit<T>));
             } else {
                 float* to = a.parts + ((static_cast<int64_t>(w.it.part) * a.kv_heads + head) * a.key_tile + key) *
                                           (2 * a.part_stride) + col;
@@ -858,9 +883,9 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv_join(Args<T> a) {
     for (int p = 0; p < j.parts; ++p) sum += *reinterpret_cast<const f32x4*>(part + p * step);
     const int64_t at = ((static_cast<int64_t>(j.key_first) + key) * a.kv_heads + head) * a.dim;
     if (which == 0)
-        put4<T>(a.dk + at, col, a.dim, a.out_whole, sum * a.scale);
+        put4<T>(a.dk + at, col, a.dim, sum * a.scale);
     else
-        put4<T>(a.dv + at, col, a.dim, a.out_whole, sum);
+        put4<T>(a.dv + at, col, a.dim, sum);
 }
 
 // The whole backward of a batch whose graphs have at most 32 rows: a workgroup has all of a
@@ -883,7 +908,7 @@ struct FewRows {
     __align__(16) float delta[32];
 };
 
-template <typename T, int DP, int RT, bool WHOLE>
+template <typename T, int DP, int RT, int FIT>
 __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& w, FewRows<T, DP>& m) {
     using M = FewRows<T, DP>;
     constexpr int BN = M::kKeys, ST = M::kStride, ND = DP / 16;
@@ -897,8 +922,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         const int64_t first = static_cast<int64_t>(w.it.key_first) + k0;
         const T* kp = a.k.data + first * a.k.row_stride + w.head * a.k.head_stride;
         const T* vp = a.v.data + first * a.v.row_stride + w.head * a.v.head_stride;
-        kl.template fetch<WHOLE>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
-        vl.template fetch<WHOLE>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
+        kl.template fetch<FIT>([&](int row) { return kp + min(row, left - 1) * a.k.row_stride; }, a.dim);
+        vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
@@ -913,10 +938,10 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         const int row = r * 16 + l % 16;
         real[r] = row < w.it.rows;
         at[r] = place_of(a, w.it.q_first, w.head, w.it.row0 + (real[r] ? row : 0));
-        qf[r].template fetch<WHOLE>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
-        gf[r].template fetch<WHOLE>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
+        qf[r].template fetch<FIT>(a.q.data + at[r].row * a.q.row_stride + at[r].head * a.q.head_stride, a.dim);
+        gf[r].template fetch<FIT>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
         RowFrags<T, DP> of;
-        of.template fetch<WHOLE>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
+        of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
         float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c)
@@ -949,8 +974,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         __syncthreads();
-        kl.store(m.k, bits.all(), [&](int row) { return bits.has(row); });
-        vl.store(m.v, bits.all(), [&](int row) { return bits.has(row); });
+        kl.template store<FIT>(m.k, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        vl.template store<FIT>(m.v, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         if (threadIdx.x < BN) m.starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
         __syncthreads();
         if (k0 + BN < w.it.keys) fetch(k0 + BN);
@@ -1024,8 +1049,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 const int key = k0 + key0 + 16 * t + l % 16;
                 if (key < w.it.keys) {
                     const int64_t to = ((static_cast<int64_t>(w.it.key_first) + key) * a.kv_heads + w.head) * a.dim;
-                    put4<T>(a.dk + to, n * 16 + g * 4, a.dim, a.out_whole, dk * (a.scale / unit2[t]));
-                    put4<T>(a.dv + to, n * 16 + g * 4, a.dim, a.out_whole, dv * (1.0f / kProbabilityUnit<T>));
+                    put4<T>(a.dk + to, n * 16 + g * 4, a.dim, dk * (a.scale / unit2[t]));
+                    put4<T>(a.dv + to, n * 16 + g * 4, a.dim, dv * (1.0f / kProbabilityUnit<T>));
                 }
             }
         }
@@ -1049,7 +1074,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         for (int v = 1; v < kWaves; ++v) sum += *reinterpret_cast<const f32x4*>(sums + (v * R + row) * DP + col);
         if (w.it.part < 0) {
             const Place p = place_of(a, w.it.q_first, w.head, w.it.row0 + row);
-            put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, a.out_whole, sum * a.scale);
+            put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * a.scale);
         } else if (col < a.part_stride) {
             const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
             *reinterpret_cast<f32x4*>(a.parts + slot * a.part_stride + col) = sum;
@@ -1062,7 +1087,7 @@ template <typename T, int DP>
 constexpr int kFewRowsWaves = sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 ? 2 : 1) : (DP == 32 ? 2 : 1);
 
 // Items of graphs without queries have no rows: their keys get zeros.
-template <typename T, int DP, bool WHOLE>
+template <typename T, int DP, int FIT>
 __global__ __launch_bounds__(kThreads, (kFewRowsWaves<T, DP>)) void k_attention_few_rows_backward(Args<T> a) {
     __shared__ FewRows<T, DP> m;
     const Work w = work_of(a.items, a.num_items, a.kv_heads);
@@ -1070,18 +1095,18 @@ __global__ __launch_bounds__(kThreads, (kFewRowsWaves<T, DP>)) void k_attention_
         for (int u = static_cast<int>(threadIdx.x); u < w.it.keys * (DP / 4); u += kThreads) {
             const int col = (u % (DP / 4)) * 4;
             const int64_t to = ((static_cast<int64_t>(w.it.key_first) + u / (DP / 4)) * a.kv_heads + w.head) * a.dim;
-            put4<T>(a.dk + to, col, a.dim, a.out_whole, f32x4(0.0f));
-            put4<T>(a.dv + to, col, a.dim, a.out_whole, f32x4(0.0f));
+            put4<T>(a.dk + to, col, a.dim, f32x4(0.0f));
+            put4<T>(a.dv + to, col, a.dim, f32x4(0.0f));
         }
         return;
     }
     if constexpr (FewRows<T, DP>::kRows == 32) {
         if (w.it.rows > 16) {
-            few_rows_backward<T, DP, 2, WHOLE>(a, w, m);
+            few_rows_backward<T, DP, 2, FIT>(a, w, m);
             return;
         }
     }
-    few_rows_backward<T, DP, 1, WHOLE>(a, w, m);
+    few_rows_backward<T, DP, 1, FIT>(a, w, m);
 }
 
 // ---- launches -----------------------------------------------------------------------
@@ -1113,25 +1138,19 @@ Args<T> args_of(const relm_mp_attention_plan& p, const AttnOperands& o) {
     a.parts = o.parts;
     a.part_stride = static_cast<int>(attention_part_stride(o.head_dim));
     a.part_stats = o.parts + attention_part_rows(p) * a.part_stride;
-    a.out_whole = sizeof(T) * o.head_dim % 4 == 0;
-    for (const void* x : {o.out, o.dq, o.dk, o.dv}) a.out_whole = a.out_whole && reinterpret_cast<uintptr_t>(x) % 4 == 0;
     return a;
 }
 
-// The WHOLE of the kernels.
-bool whole_rows(const AttnOperands& o, size_t value) {
-    return o.head_dim % 8 == 0 && reinterpret_cast<uintptr_t>(o.out) % 4 == 0 && on_dwords(o.q, value) &&
-           on_dwords(o.k, value) && on_dwords(o.v, value) && on_dwords(o.grad, value);
-}
-
-// f with the padded head size (32, 64 or 128), WHOLE, and the rows' shape of the plan.
+// f with the padded head size (32, 64 or 128), FIT, and the rows' shape of the plan.
 template <typename F>
-void with_dim(int64_t dim, bool whole, F&& f) {
+void with_dim(int64_t dim, F&& f) {
     const auto with = [&](auto dp) {
-        if (whole)
-            f(dp, std::true_type{});
-        else
-            f(dp, std::false_type{});
+        if (dim % 8 == 0)
+            f(dp, std::integral_constant<int, kWhole>{});
+        else if (decltype(dp)::value > 32 || dim > 8)
+            f(dp, std::integral_constant<int, kCut>{});
+        else if constexpr (decltype(dp)::value == 32)
+            f(dp, std::integral_constant<int, kShort>{});
     };
     if (dim <= 32)
         with(std::integral_constant<int, 32>{});
@@ -1173,9 +1192,9 @@ template <typename T>
 hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
     const Args<T> a = args_of<T>(p, o);
     if (p.num_items == 0) return hipSuccess;
-    with_dim(o.head_dim, whole_rows(o, sizeof(T)), [&](auto dp, auto whole) {
+    with_dim(o.head_dim, [&](auto dp, auto whole) {
         constexpr int DP = decltype(dp)::value;
-        constexpr bool W = decltype(whole)::value;
+        constexpr int W = decltype(whole)::value;
         with_rows<T, DP>(p.row_tile, [&](auto rt, auto wm) {
             hipLaunchKernelGGL((k_attention<T, DP, decltype(rt)::value, decltype(wm)::value, W>),
                                dim3(static_cast<unsigned>(p.num_items) * p.kv_heads), dim3(kThreads), 0, st, a);
@@ -1188,9 +1207,9 @@ hipError_t forward(const relm_mp_attention_plan& p, const AttnOperands& o, hipSt
 template <typename T>
 hipError_t backward(const relm_mp_attention_plan& p, const AttnOperands& o, hipStream_t st) {
     Args<T> a = args_of<T>(p, o);
-    with_dim(o.head_dim, whole_rows(o, sizeof(T)), [&](auto dp, auto whole) {
+    with_dim(o.head_dim, [&](auto dp, auto whole) {
         constexpr int DP = decltype(dp)::value;
-        constexpr bool W = decltype(whole)::value;
+        constexpr int W = decltype(whole)::value;
         if (p.row_tile <= FewRows<T, DP>::kRows) {
             a.num_items = p.num_items + p.num_idle_items;
             if (a.num_items > 0)

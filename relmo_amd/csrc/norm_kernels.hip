@@ -13,7 +13,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <initializer_list>
 
 #include "device_utils.h"
 #include "internal.h"
@@ -387,14 +386,12 @@ __global__ __launch_bounds__(kFoldCols * kFoldRows) void k_norm_fold(const float
 constexpr int64_t kMaxBlocks = 1024;
 constexpr int64_t kLongRows = 64;  // rows of a workgroup of k_norm_weight_partial, at least
 
-// Values of a lane's unit: 16 bytes where they divide the row and every row of every
-// array starts on a dword, else a dword, else one value.
+// Values of a lane's unit: 16 bytes where they divide the row, else a dword, else one
+// value.
 template <typename T>
-int unit_values(int64_t width, std::initializer_list<const void*> arrays) {
-    bool dwords = sizeof(T) * width % 4 == 0;
-    for (const void* p : arrays) dwords = dwords && reinterpret_cast<uintptr_t>(p) % 4 == 0;
-    if (!dwords) return 1;
-    return width % kLaneValues<T> == 0 ? kLaneValues<T> : 4 / static_cast<int>(sizeof(T));
+int unit_values(int64_t width) {
+    constexpr int kDword = 4 / static_cast<int>(sizeof(T));
+    return width % kLaneValues<T> == 0 ? kLaneValues<T> : width % kDword == 0 ? kDword : 1;
 }
 template <typename T, typename F>
 void with_unit(int values, F&& f) {
@@ -499,7 +496,7 @@ hipError_t launch_add_rms_norm(int dtype, const void* x, const void* r, const vo
     const NormArgs a{x, r, w, y, h, scale, rstd, rows, width, eps};
     with_value_type(dtype, [&](auto t) {
         using T = decltype(t);
-        with_unit<T>(unit_values<T>(width, {x, r, w, scale != nullptr ? nullptr : y, h}),
+        with_unit<T>(unit_values<T>(width),
                      [&](auto v) { e = norm_forward<T, decltype(v)::value>(a, scale != nullptr, st); });
     });
     return e;
@@ -508,9 +505,8 @@ hipError_t launch_add_rms_norm(int dtype, const void* x, const void* r, const vo
 size_t add_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t width) {
     if (rows <= 0 || width <= 0) return 0;
     int64_t blocks = 0;
-    with_value_type(dtype, [&](auto t) {  // of any unit: the arrays' addresses choose later
-        for (const int v : {kLaneValues<decltype(t)>, 2, 1})
-            blocks = std::max(blocks, backward_blocks(rows, (width + v - 1) / v));
+    with_value_type(dtype, [&](auto t) {
+        blocks = backward_blocks(rows, width / unit_values<decltype(t)>(width));
     });
     return static_cast<size_t>(blocks * width) * sizeof(float);
 }
@@ -529,7 +525,7 @@ hipError_t launch_add_rms_norm_backward(int dtype, const void* dy, const void* d
             e = hipGetLastError();
             return;
         }
-        with_unit<T>(unit_values<T>(width, {dy, dh, h, w, dx}),
+        with_unit<T>(unit_values<T>(width),
                      [&](auto v) { e = norm_backward<T, decltype(v)::value>(a, dw, st); });
     });
     return e;

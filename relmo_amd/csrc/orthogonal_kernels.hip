@@ -293,25 +293,16 @@ __global__ __launch_bounds__(kThreads) void k_ortho_norm(OrthoBatch batch, void*
     const int64_t rows = d.tall ? d.n : d.m;
     const int cols = d.tall ? d.m : d.n;
     const int wave = static_cast<int>(threadIdx.x) / kWave;
-    // rows on dwords are read in 16-byte units, the last one's values past the row as zeros
-    constexpr int V = kLaneValues<T>;
-    const bool whole = reinterpret_cast<uintptr_t>(d.in) % 4 == 0 && d.in_stride * sizeof(T) % 4 == 0;
+    constexpr int V = kLaneValues<T>;  // the last unit's values past the row are zeros
     double sum = 0.0;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + wave; r < rows;
          r += kNormParts * (kThreads / kWave)) {
         const T* in = static_cast<const T*>(d.in) + r * d.in_stride;
-        if (whole) {
 #pragma unroll 4
-            for (int c = lane_id() * V; c < cols; c += kWave * V) {
-                const FloatVec<V> x = load_values<T, V>(in, c, cols);
+        for (int c = lane_id() * V; c < cols; c += kWave * V) {
+            const FloatVec<V> x = load_values<T, V>(in, c, cols);
 #pragma unroll
-                for (int j = 0; j < V; ++j) sum = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum);
-            }
-        } else {
-            for (int c = lane_id(); c < cols; c += kWave) {
-                const double x = static_cast<double>(static_cast<float>(in[c]));
-                sum = fma(x, x, sum);
-            }
+            for (int j = 0; j < V; ++j) sum = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum);
         }
     }
     sum = wave_sum(sum);

@@ -15,10 +15,10 @@ namespace relm_mp {
 using bf16 = __bf16;
 using f16 = _Float16;
 
-// N values of T at the alignment of a row's start: global memory takes accesses
-// of up to 16 bytes at any dword.
+// N values of T wherever they start: the target's global memory takes accesses of up to
+// 16 bytes at any address, and the compiler makes one of each.
 template <typename T, int N>
-using ValueVec = T __attribute__((ext_vector_type(N), aligned(sizeof(T) * N < 4 ? sizeof(T) * N : 4)));
+using ValueVec = T __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 template <int N>
 using FloatVec = float __attribute__((ext_vector_type(N)));
 
