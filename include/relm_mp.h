@@ -531,7 +531,7 @@ int relm_mp_film_mish_backward_sums(const float* s, const float* dy, int64_t row
 int relm_mp_add_rms_norm(int dtype, const void* x, const void* r, const void* w, int64_t rows, int64_t width,
                          float eps, void* y, void* h, float* rstd, relm_mp_stream_t stream);
 /* The same with y in 8 bits for serving: q [rows, width] e4m3 bytes, scale [rows] floats
- * = max|y| / 448 of the row (1 for a row of zeros): y ~ q * scale. */
+ * = max|y| / 448 of the row (1 where that is 0): y ~ q * scale. */
 int relm_mp_add_rms_norm_fp8(int dtype, const void* x, const void* r, const void* w, int64_t rows, int64_t width,
                              float eps, void* q, float* scale, void* h, relm_mp_stream_t stream);
 /* Backward: dx [rows, width] (the gradient of x and of r alike) and dw [width] from dy

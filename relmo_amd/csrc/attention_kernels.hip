@@ -208,6 +208,7 @@ struct KeyBits {
         for (int w = 0; w < BN / 64; ++w) bits[w] = __ballot(byte[w] != 0);
     }
     __device__ __forceinline__ bool all() const { return (bits[0] & bits[BN / 64 - 1]) == ~0ull; }
+    __device__ __forceinline__ bool none() const { return (bits[0] | bits[BN / 64 - 1]) == 0; }
     __device__ __forceinline__ uint64_t word(int k) const { return BN == 128 && (k & 64) ? bits[BN / 64 - 1] : bits[0]; }
     __device__ __forceinline__ bool has(int k) const { return (word(k) >> (k % 64)) & 1; }
 };
@@ -339,6 +340,10 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
+        if (bits.none()) {  // nothing of this tile is kept (the same for all waves)
+            if (k0 + BN < w.it.keys) fetch(k0 + BN);
+            continue;
+        }
         __syncthreads();
         kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
@@ -642,6 +647,10 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
+        if (bits.none()) {  // nothing of this tile is kept (the same for all waves)
+            if (k0 + BN < w.it.keys) fetch(k0 + BN);
+            continue;
+        }
         __syncthreads();
         kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
@@ -851,6 +860,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         for (int n = 0; n < ND; ++n) {
             const int col = n * 16 + g * 4;
             dk[t][n] *= 1.0f / unit[t];
+            if (start[t][0] != 0.0f) dk[t][n] = dv[t][n] = f32x4(0.0f);  // whatever an infinite query made of it
             if (w.it.part < 0) {
                 put4<T>(a.dk + at * a.dim, col, a.dim, dk[t][n] * a.scale);
                 put4<T>(a.dv + at * a.dim, col, a.dim, dv[t][n] * (1.0f / kProbabilityUnit<T>));
@@ -1044,8 +1054,10 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
             const Frag<T> qt = rows_frag_t<T, RT>(m.q, ST, n * 16);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const f32x4 dv = mma<T>(gt, pf[t], f32x4(0.0f));
-                const f32x4 dk = mma<T>(qt, dsf[t], f32x4(0.0f));
+                f32x4 dv = mma<T>(gt, pf[t], f32x4(0.0f));
+                f32x4 dk = mma<T>(qt, dsf[t], f32x4(0.0f));
+                // a key that is not kept gets 0, whatever an infinite query made of it
+                if (m.starts[key0 + 16 * t + l % 16] != 0.0f) dk = dv = f32x4(0.0f);
                 const int key = k0 + key0 + 16 * t + l % 16;
                 if (key < w.it.keys) {
                     const int64_t to = ((static_cast<int64_t>(w.it.key_first) + key) * a.kv_heads + w.head) * a.dim;

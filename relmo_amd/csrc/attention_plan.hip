@@ -180,8 +180,10 @@ int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, i
     p.num_key_parts = L.num_key_parts;
     p.num_key_joins = static_cast<int32_t>(L.key_joins.size());
     p.num_idle_items = static_cast<int32_t>(L.idle.size());
-    if (static_cast<int64_t>(std::max(L.items.size() + L.idle.size(), 2 * L.key_items.size())) * kv_heads > 0x7fffffff ||
-        static_cast<int64_t>(std::max(L.joins.size(), L.key_joins.size())) * 128 > 0x7fffffff || kv_heads > 65535)
+    // a launch has fewer than 2^32 threads
+    constexpr int64_t kMostBlocks = (int64_t{1} << 24) - 1;
+    if (static_cast<int64_t>(std::max(L.items.size() + L.idle.size(), 2 * L.key_items.size())) * kv_heads > kMostBlocks ||
+        static_cast<int64_t>(std::max(L.joins.size(), L.key_joins.size())) * 128 * kv_heads > kMostBlocks)
         return bad("too many items for one launch");
     if (table != nullptr) {
         if (table_bytes < static_cast<size_t>(p.table_bytes))

@@ -209,7 +209,8 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs a) {
                 for (int64_t i = 0; i < units; ++i) magnitude(result(i));
             }
             most = group_max<L>(most, lds);
-            const float scale = most == 0.0f ? 1.0f : most / kFp8Max;
+            float scale = most / kFp8Max;
+            if (scale == 0.0f) scale = 1.0f;  // zeros, or too small to have a scale
             if (lane == 0) a.scale[row] = scale;
             // a scale below the smallest normal float may round up to 9% off: the
             // quotient is held to the type's range

@@ -235,8 +235,8 @@ def add_rms_norm_fp8(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """:func:`add_rms_norm` with ``y`` in 8 bits, for serving: ``(q, scale, h)``.
 
-    ``q`` is float8_e4m3fn and ``scale`` float32 [...], one per row: ``max|y| / 448`` (1 for
-    a row of zeros), so ``y ~ q * scale`` and no value saturates.  A row with a NaN or
+    ``q`` is float8_e4m3fn and ``scale`` float32 [...], one per row: ``max|y| / 448`` (1 where
+    that is 0), so ``y ~ q * scale`` and no value saturates.  A row with a NaN or
     infinite ``y`` has that as its scale.  No gradient."""
 
     require_torch("add_rms_norm_fp8")

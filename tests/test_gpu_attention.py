@@ -140,6 +140,10 @@ RAGGED = [
     ([70], [9_000], 1, 1, 32),
     ([5_003, 2], [40, 1], 1, 1, 24),                    # few keys: parts over the rows
     ([600], [70], 8, 1, 128),
+    ([20, 3], [50, 130], 2, 1, 7),                      # rows shorter than a unit, and cut ones
+    ([5, 33], [90, 64], 2, 2, 9),
+    ([33, 90], [200, 70], 2, 1, 65),
+    ([12], [300], 1, 1, 127),
     ([2] * 700, [3, 11] * 350, 2, 2, 8),
 ]
 
@@ -214,6 +218,26 @@ def test_infinite_scores_spoil_their_row_only() -> None:
     out = mp.cross_attention(q, k, v, plan)
     rows = [0, 2, 3, 4]
     assert torch.equal(out[rows], clean[rows]) and bool(out[1].isnan().all())
+
+
+@pytest.mark.parametrize("queries", [[2, 9], [60, 33], [200, 130]])
+def test_infinite_queries_and_left_out_keys(queries) -> None:
+    """An infinite query spoils neither the gradients of left-out keys nor the zeros of a graph without a key."""
+    from relmo_amd import mp
+
+    keys = [150, 90]
+    q, k, v, grad, mask = _make(queries, keys, 1, 1, 32, torch.float32, seed=14, mask="first graph")
+    plan = mp.attention_plan(_offsets(queries), _offsets(keys), 1)
+    clean = _run(q, k, v, grad, plan, mask)
+    q = q.clone()
+    q[0, 0, 3] = float("inf")  # in the graph without a key
+    out, dq, dk, dv = _run(q, k, v, grad, plan, mask)
+    assert torch.equal(out, clean[0]) and torch.equal(dk, clean[2]) and torch.equal(dv, clean[3])
+    assert torch.equal(dq[queries[0]:], clean[1][queries[0]:]) and float(dq[1:queries[0]].abs().sum()) == 0
+    q[-1, 0, 3] = float("inf")
+    out, dq, dk, dv = _run(q, k, v, grad, plan, mask)
+    assert torch.equal(out[:-1], clean[0][:-1])
+    assert float(dk[~mask].abs().sum()) == 0 and float(dv[~mask].abs().sum()) == 0
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -165,6 +165,22 @@ def test_fp8_output(rows: int, width: int, dtype) -> None:
     assert bool(((at == 448) | (most == 0)).all())
 
 
+def test_fp8_rows_too_small_for_a_scale() -> None:
+    from relmo_amd import mp
+
+    # y = x / sqrt(eps) * w: about 1e-44, whose 448th is no float; and subnormal scales
+    x = torch.full((2, 16), 1e-30, device=DEV)
+    w = torch.ones(16, device=DEV) * 1e-17
+    x[1] *= 1e3
+    q, scale, _ = mp.add_rms_norm_fp8(x, None, w, eps=1e-6)
+    y = mp.rms_norm(x, w, eps=1e-6)
+    assert float(scale[0]) == 1.0 and float(q[0].float().abs().sum()) == 0
+    assert bool(q.float().isfinite().all())
+    assert abs(float(scale[1]) * 448 - float(y[1].double().max())) <= 0.5 * 2.0 ** -149 * 448  # 16 units of 2^-149
+    # a subnormal scale of a few units is off by up to half of one
+    assert float(((q[1].double() * scale[1].double()) - y[1].double()).abs().max()) <= 0.5 * 2.0 ** -149 * 448 + 2.0 ** -4 * 1e-41
+
+
 def test_fp8_rows_with_infinite_and_nan_values_stay_apart() -> None:
     from relmo_amd import mp
 
