@@ -337,13 +337,11 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
         vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
+    bool any = false;  // whether some key of the item is kept (the same for all waves)
     if (w.it.keys > 0) fetch(0);
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
-        if (bits.none()) {  // nothing of this tile is kept (the same for all waves)
-            if (k0 + BN < w.it.keys) fetch(k0 + BN);
-            continue;
-        }
+        any = any || !bits.none();
         __syncthreads();
         kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
@@ -403,7 +401,15 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
         }
     }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) total[r] = lanes_sum(total[r]);
+    for (int r = 0; r < RT; ++r) {
+        total[r] = lanes_sum(total[r]);
+        if (!any) {  // nothing to read: zeros, whatever an infinite query made of it
+            m[r] = -kInf;
+            total[r] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) o[r][n] = f32x4(0.0f);
+        }
+    }
 
     const auto finish = [&](int row, Place p, int col, f32x4 sum, float top, float sum_p) {
         if (w.it.part < 0) {
@@ -553,6 +559,22 @@ __device__ __forceinline__ void backward_scores(f32x4 (&s)[2], f32x4 (&dp)[2], f
         }
 }
 
+// Whether a graph keeps exactly one key (graphs of at most 128 are looked at; the same for
+// all waves).  Its queries' probability is 1 whatever the scores, so ds is 0 - not what is
+// left when two roundings of <grad, v> are subtracted.
+__device__ __forceinline__ bool one_key(const uint8_t* mask, const AttnItem& it) {
+    if (it.graph_keys > 128 || (mask == nullptr && it.graph_keys != 1)) return false;
+    if (mask == nullptr) return true;
+    int kept = 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const int k = w * 64 + lane_id();
+        const bool is = mask[it.graph_key_first + static_cast<int64_t>(min(k, it.graph_keys - 1))] != 0;
+        kept += __popcll(__ballot(k < it.graph_keys && is));
+    }
+    return kept == 1;
+}
+
 // Half values lose bits below 2^-14, where ds of keys with small probabilities lies.  A lane
 // holds ds of one query (key) and the sum over keys (queries) that it enters: both are kept
 // in units of a power of two, which falls as the largest ds seen so far rises (like the
@@ -644,13 +666,12 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
-    if (w.it.keys > 0) fetch(0);
-    for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
+    const int keys = w.it.keys == 0 || one_key(a.key_mask, w.it) ? 0 : w.it.keys;  // to walk: none leaves dq = 0
+    bool any = false;  // whether some key of the item is kept (the same for all waves)
+    if (keys > 0) fetch(0);
+    for (int k0 = 0; k0 < keys; k0 += BN) {
         bits.settle();
-        if (bits.none()) {  // nothing of this tile is kept (the same for all waves)
-            if (k0 + BN < w.it.keys) fetch(k0 + BN);
-            continue;
-        }
+        any = any || !bits.none();
         __syncthreads();
         kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
@@ -684,7 +705,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int n = 0; n < ND; ++n) dq[r][n] *= 1.0f / unit[r];
+        for (int n = 0; n < ND; ++n) dq[r][n] = any ? dq[r][n] * (1.0f / unit[r]) : f32x4(0.0f);
     const auto finish = [&](int row, Place p, int col, f32x4 sum) {
         if (w.it.part < 0) {
             put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * a.scale);
@@ -767,6 +788,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         unit[t] = kStartUnit<T>;
     }
 
+    const bool alone = one_key(a.key_mask, w.it);
     TileLoad<T, DP, BR> ql, gl;
     float lse_in = 0.0f, delta_in = 0.0f;
     const auto fetch = [&](int r0) {
@@ -836,6 +858,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
                     }
                 }
                 pf[t] = frag_of<T>(s[t][0] * kProbabilityUnit<T>, s[t][1] * kProbabilityUnit<T>);
+                if (alone) dp[t][0] = dp[t][1] = f32x4(0.0f);
                 into_unit<T>(dp[t], unit[t], dk[t]);
                 dsf[t] = frag_of<T>(dp[t][0], dp[t][1]);
             }
@@ -937,6 +960,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
+    const bool alone = w.it.keys > 0 && one_key(a.key_mask, w.it);
 
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
@@ -981,8 +1005,10 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         }
     }
 
+    bool any = false;  // whether some key of the item is kept (the same for all waves)
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
+        any = any || !bits.none();
         __syncthreads();
         kl.template store<FIT>(m.k, a.dim, bits.all(), [&](int row) { return bits.has(row); });
         vl.template store<FIT>(m.v, a.dim, bits.all(), [&](int row) { return bits.has(row); });
@@ -1002,6 +1028,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             backward_scores(s[r], dp[r], sl2, lse2[r], delta[r]);
+            if (alone) dp[r][0] = dp[r][1] = f32x4(0.0f);
             into_unit<T>(dp[r], unit[r], dq[r]);
             ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
         }
@@ -1044,6 +1071,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 }
             }
             pf[t] = frag_of<T>(pr[0] * kProbabilityUnit<T>, pr[1] * kProbabilityUnit<T>);
+            if (alone) dr[0] = dr[1] = f32x4(0.0f);
             unit2[t] = kStartUnit<T>;
             into_unit<T>(dr, unit2[t], none);
             dsf[t] = frag_of<T>(dr[0], dr[1]);
@@ -1077,7 +1105,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int n = 0; n < ND; ++n)
-            *reinterpret_cast<f32x4*>(sums + (wave * R + r * 16 + l % 16) * DP + n * 16 + g * 4) = dq[r][n] * (1.0f / unit[r]);
+            *reinterpret_cast<f32x4*>(sums + (wave * R + r * 16 + l % 16) * DP + n * 16 + g * 4) =
+                any ? dq[r][n] * (1.0f / unit[r]) : f32x4(0.0f);
     __syncthreads();
     for (int u = static_cast<int>(threadIdx.x); u < w.it.rows * (DP / 4); u += kThreads) {
         const int row = u / (DP / 4), col = (u % (DP / 4)) * 4;

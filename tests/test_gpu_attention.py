@@ -220,6 +220,25 @@ def test_infinite_scores_spoil_their_row_only() -> None:
     assert torch.equal(out[rows], clean[rows]) and bool(out[1].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [[2, 9, 4], [60, 33, 1], [200, 130, 9]])
+def test_one_key_leaves_no_gradient_of_the_scores(queries, dtype) -> None:
+    """A softmax over one key is 1: dq and dk are 0, not a rounding's rest, with one key and with one kept key."""
+    from relmo_amd import mp
+
+    for keys, mask in (([1, 1, 1], None), ([1, 0, 100], "one")):
+        q, k, v, grad, _ = _make(queries, keys, 2, 1, 33, dtype, seed=15)
+        key_mask = None
+        if mask:
+            key_mask = torch.zeros(sum(keys), dtype=torch.bool, device=DEV)
+            key_mask[0] = key_mask[-7] = True
+        plan = mp.attention_plan(_offsets(queries), _offsets(keys), 2, 1)
+        out, dq, dk, dv = _run(q, k, v, grad, plan, key_mask)
+        assert float(dq.abs().sum()) == 0 and float(dk.abs().sum()) == 0
+        val, tol = _definition(q, k, v, grad, key_mask, queries, keys, 33 ** -0.5)
+        _check((out, dq, dk, dv), val, tol, 2.0 ** -24 if dtype == torch.float16 else 1e-15)
+
+
 @pytest.mark.parametrize("queries", [[2, 9], [60, 33], [200, 130]])
 def test_infinite_queries_and_left_out_keys(queries) -> None:
     """An infinite query spoils neither the gradients of left-out keys nor the zeros of a graph without a key."""
@@ -233,7 +252,7 @@ def test_infinite_queries_and_left_out_keys(queries) -> None:
     q[0, 0, 3] = float("inf")  # in the graph without a key
     out, dq, dk, dv = _run(q, k, v, grad, plan, mask)
     assert torch.equal(out, clean[0]) and torch.equal(dk, clean[2]) and torch.equal(dv, clean[3])
-    assert torch.equal(dq[queries[0]:], clean[1][queries[0]:]) and float(dq[1:queries[0]].abs().sum()) == 0
+    assert torch.equal(dq[queries[0]:], clean[1][queries[0]:]) and float(dq[:queries[0]].abs().sum()) == 0
     q[-1, 0, 3] = float("inf")
     out, dq, dk, dv = _run(q, k, v, grad, plan, mask)
     assert torch.equal(out[:-1], clean[0][:-1])
