@@ -573,9 +573,10 @@ typedef struct relm_mp_attention_plan {
 } relm_mp_attention_plan;
 
 /* Host only.  q_offsets and k_offsets: graphs + 1 host values from 0 to q_rows / k_rows,
- * ascending.  table NULL: fills *plan but for its pointer (table_bytes among it); else
- * also writes the table into `table` (host memory of table_bytes), which the caller
- * copies to the device and stores in plan->table. */
+ * ascending.  Fills *plan but for its pointer (plan->table_bytes among it); with `table`
+ * not NULL also writes the table there (host memory of table_bytes; RELM_MP_ERR_WORKSPACE
+ * if that is less than plan->table_bytes), which the caller copies to the device and
+ * stores in plan->table. */
 int relm_mp_attention_plan_build(const int64_t* q_offsets, const int64_t* k_offsets, int64_t graphs,
                                  int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads,
                                  void* table, size_t table_bytes, relm_mp_attention_plan* plan);

