@@ -291,11 +291,11 @@ struct RowShape {
 // Forward.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with the running maximum m:
 // when a key tile raises it, what has been added up is scaled by exp(m_old - m_new).
 // Long rows of work are bound by the exponentials and conversions beside the matrix
-// instructions (equal shares at 128 values, 32 rows to a wave): 4 x 2048 queries x 4096 keys,
+// instructions: 4 x 2048 queries x 4096 keys,
 // 16 heads of 128 over 4 key heads, bfloat16, 335 us (820 TFLOP/s).  Few rows are bound by
 // the reads of keys and values: one query over 262,147 keys, 2 key heads of 64 in half
 // precision, in 512 parts 31 us (4.3 TB/s); 2048 graphs of 64 to 512 keys, up to 32 queries,
-// 4 heads of 32 in bfloat16 92 us (3.6 TB/s).
+// 4 heads of 32 in bfloat16 92 us (3.5 TB/s).
 template <typename T, int DP, int RT, int WM, int FIT>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T> a) {
     using S = RowShape<RT, WM>;
@@ -936,9 +936,10 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv_join(Args<T> a) {
 // all have, and keys and values are read once.  A wave takes 32 keys of a tile.  dq sums over
 // keys and wants them down (as in the forward), dk and dv over rows and want those down: the
 // scores are computed both ways, from the same fragments with the operands exchanged, and
-// their exponentials twice.  Bound by latency at three waves to a SIMD, then by the reads and
-// writes (keys, values and their gradients once each): 2048 graphs of 64 to 512 keys, up to 32
-// queries, 4 heads of 32 in bfloat16 190 us (3.2 TB/s) against 318 for the two kernels of longer rows.
+// their exponentials twice.  Bound by latency, then by the reads and writes
+// (keys, values and their gradients once each): 2048 graphs of 64 to 512 keys, up to 32
+// queries, 4 heads of 32 in bfloat16 192 us (291 before the items were dealt by length, then
+// 318 for the two kernels of longer rows).
 template <typename T, int DP>
 struct FewRows {
     static constexpr int kKeys = 128, kStride = kLdsStride<T, DP>;

@@ -364,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_weight_partial(NormBackwardAr
 }
 
 // dw[col] = the blocks' partial sums added up: kFoldRows partial chains per column, then
-// those in order.  Latency bound: 1024 rows of partial sums in 16 rounds, 7 us at 128 columns.
+// those in order.  Latency bound: 7 us after 589,825 rows of 128 floats.
 constexpr int kFoldCols = 16;
 constexpr int kFoldRows = 64;
 

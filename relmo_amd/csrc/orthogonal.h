@@ -24,9 +24,9 @@ struct OrthoMatrix {
 constexpr int kOrthoBatch = 28;
 constexpr int kNormParts = 256;  // partial sums of squares of a matrix: a wave adds them
 // Tiles of 128 x 128 from which on they are taken instead of 64 x 64 ones: of the symmetric
-// products, of the update.  2048 x 2048 (136 lower tiles) takes 855 us with both large, 1018
-// with small lower ones; 1500 x 2600 (78 and 252 tiles) 688 us with small lower and large
-// update tiles, 798 with all small.
+// products, of the update.  Symmetric: 2048 x 2048 (136 tiles) takes 855 us with large ones,
+// 1018 with small.  Update: 2048 x 2048 (256 tiles) 836 us with large ones, 941 with small,
+// 1500 x 2600 (252) 661 and 732.  The thresholds between measured counts are not tuned.
 constexpr int64_t kLargeTiles[2] = {100, 128};
 
 struct OrthoRule {

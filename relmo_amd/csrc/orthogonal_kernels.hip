@@ -11,10 +11,12 @@
 // 22 bits, at scales (powers of two, exact) that keep the halves within their normal
 // range.  A product of two such matrices is three matrix-instruction products, hi hi + hi
 // lo + lo hi, added in float: about float's own accuracy at a third of the 16-bit rate,
-// five times the float instructions' rate.  The Frobenius norm is added in double.
+// five times the float instructions' rate (2048 x 2048: error 1.9e-6, in float products
+// 2.9e-6).  One half would leave 1.3e-3 to 1.6e-3 by its rounding, a pair 3e-7 (96 x 96 to
+// 512 x 512, simulated in double).  The Frobenius norm is added in double.
 //
-// A and B are symmetric: of A X^T-like products only the lower tiles are computed and
-// written twice, and both operands of every product are read along their rows.
+// A and B are symmetric: only their lower tiles are computed, and written twice, and both
+// operands of every product are read along their rows (of X there is a transposed copy).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -84,8 +86,7 @@ struct OrthoBatch {
 // Latency bound (a product of 96 x 96 is 36 matrix instructions to a wave): few barriers
 // (4 a step), operands from LDS in blocks of 32 x 32, a step's A kept in the registers
 // of the wave that computed it.  14 matrices of 32 x 32 to 96 x 96 take 45 us: 7 a step for
-// the largest, 10 for the launch and the two readings.  16 waves with a tile of 16 x 16 each
-// ran out of registers and took 56.
+// the largest, the rest outside the steps.  16 waves ran out of registers and spilled.
 template <typename T>
 __global__ __launch_bounds__(kSmallThreads) void k_ortho_small(OrthoBatch batch, OrthoRule rule) {
     extern __shared__ __align__(16) f16 pool[];
@@ -334,6 +335,7 @@ __device__ __forceinline__ Planes planes_a(void* ws, const OrthoMatrix& d) { ret
 __device__ __forceinline__ Planes planes_b(void* ws, const OrthoMatrix& d) { return planes(ws, d.b, d.m, d.mp); }
 
 // X and its transpose as pairs, 32 x 32 entries to a workgroup; the padding of every plane.
+// Bound by memory and the launch: 2048 x 2048 floats 14.7 us.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_ortho_split(OrthoBatch batch, OrthoRule rule, void* ws) {
     __shared__ float tile[32][33];
@@ -398,9 +400,8 @@ enum Product { kGram, kSquare, kUpdate };
 // fragments come from LDS, the one after it goes from registers to LDS and the third is on
 // its way from memory: one barrier a stage.  Bound by the matrix instructions: a wave of the
 // 128-tile runs 48 of them (768 cycles) a stage beside 16 LDS reads and 8 writes of 1 KB.
-// 2048 x 2048: the 136 lower tiles 50 us (a tile's 64 stages at 1,600 cycles: half of them
-// the matrix instructions', the rest waits at the barrier and moves of accumulators), the
-// update's 256 tiles 65 us; as 528 tiles of 64 x 64 the lower ones take 68.
+// 2048 x 2048: the 136 lower tiles 50 us (matrix instructions are busy for 48% of the
+// waves' cycles), the update's 256 tiles 67 us; as 528 tiles of 64 x 64 the lower ones take 68.
 template <typename T, int PRODUCT, int BT>
 __global__ __launch_bounds__(kThreads, 2) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
     constexpr int MT = BT / 32;
