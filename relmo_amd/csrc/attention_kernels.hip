@@ -273,6 +273,12 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// Half values end at 2^-14 (below, they lose bits, and below 2^-25 all of them): the
+// probabilities of a query with tens of thousands of keys would, and those of all keys beside
+// one that lies 10 above them.  They are at most 1, so products read them in units of 2^-15.
+template <typename T>
+constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
+
 // Two waves to a SIMD with 16-bit values: one's matrix instructions run beside the other's
 // exponentials.  Float rows need the registers of both.
 template <typename T>
@@ -388,7 +394,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float p = exp2_of(fmaf(s[c][r][t][i], sl2, -base));
-                        s[c][r][t][i] = p;
+                        s[c][r][t][i] = p * kProbabilityUnit<T>;
                         total[r] += p;
                     }
         }
@@ -409,6 +415,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         total[r] = lanes_sum(total[r]);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) o[r][n] *= 1.0f / kProbabilityUnit<T>;
         if (!any) {  // nothing to read: zeros, whatever an infinite query made of it
             m[r] = -kInf;
             total[r] = 0.0f;
@@ -749,12 +757,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         }
     }
 }
-
-// Half values end at 2^-14 (below, they lose bits): the probabilities of a query with
-// tens of thousands of keys would.  They are at most 1, so dv adds them up in units of
-// 2^-15.
-template <typename T>
-constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
 
 // dk and dv of a key item: a wave keeps KT tiles of 16 keys and walks the graph's rows
 // (rows down, keys across, so that a lane's probabilities are the operand of the products
