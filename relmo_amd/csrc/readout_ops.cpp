@@ -249,8 +249,9 @@ c10::intrusive_ptr<AttentionPlan> plan_of(int64_t number, const char* op) {
     return plan;
 }
 
-std::tuple<c10::intrusive_ptr<AttentionPlan>, int64_t> attention_plan(const Tensor& q_offsets, const Tensor& k_offsets,
-                                                                      int64_t heads, int64_t kv_heads) {
+// The plan, its number, and the offsets it was made from ([2, graphs + 1], in host memory).
+std::tuple<c10::intrusive_ptr<AttentionPlan>, int64_t, Tensor> attention_plan(const Tensor& q_offsets, const Tensor& k_offsets,
+                                                                              int64_t heads, int64_t kv_heads) {
     for (const Tensor* t : {&q_offsets, &k_offsets})
         TORCH_CHECK(t->dim() == 1 && t->scalar_type() == at::kLong && t->is_cuda() && t->numel() >= 1 &&
                         t->device() == q_offsets.device() && t->numel() == q_offsets.numel(),
@@ -284,7 +285,7 @@ std::tuple<c10::intrusive_ptr<AttentionPlan>, int64_t> attention_plan(const Tens
     const std::lock_guard<std::mutex> hold(list.lock);
     ref->number = list.next++;
     list.plans.emplace(ref->number, c10::weak_intrusive_ptr<AttentionPlan>(ref));
-    return {ref, ref->number};
+    return {ref, ref->number, host};
 }
 
 namespace {
@@ -454,7 +455,7 @@ TORCH_LIBRARY_FRAGMENT(relm_mp, m) {
     m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");
     m.def("add_rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
     m.class_<relm_amd::readout::AttentionPlan>("AttentionPlan");
-    m.def("attention_plan(Tensor q_offsets, Tensor k_offsets, int heads, int kv_heads) -> (__torch__.torch.classes.relm_mp.AttentionPlan, int)");
+    m.def("attention_plan(Tensor q_offsets, Tensor k_offsets, int heads, int kv_heads) -> (__torch__.torch.classes.relm_mp.AttentionPlan, int, Tensor)");
     m.def("cross_attention(Tensor q, Tensor k, Tensor v, int plan, Tensor? key_mask, float scale) -> Tensor");
     m.def("orthogonalise(Tensor[] updates, int steps, float[] coefficients, float eps) -> Tensor[]");
 }

@@ -78,7 +78,9 @@ def add_rms_norm_fp8(x, residual, weight, eps: float):
 
 
 class AttentionPlan:
-    """The lengths of a batch's graphs and, on the GPU, how their attention is laid over the device."""
+    """The lengths of a batch's graphs and, on the GPU, how their attention is laid over the device.
+
+    ``q_offsets`` and ``k_offsets`` are the plan's own, in host memory."""
 
     def __init__(self, q_offsets, k_offsets, heads: int, kv_heads: int, ref=None, number: int | None = None):
         self.q_offsets, self.k_offsets = q_offsets, k_offsets
@@ -97,7 +99,9 @@ def attention_plan(q_offsets, k_offsets, heads: int, kv_heads: int | None) -> At
             raise ValueError(f"attention_plan expects {name} to be int64 [graphs + 1].")
     op = library_op("attention_plan", tensor=q_offsets, gpu_only=True)
     if op is not None:
-        return AttentionPlan(q_offsets, k_offsets, heads, kv_heads, *op(q_offsets, k_offsets, heads, kv_heads))
+        ref, number, own = op(q_offsets, k_offsets, heads, kv_heads)
+        return AttentionPlan(own[0], own[1], heads, kv_heads, ref, number)
+    q_offsets, k_offsets = (t.detach().to("cpu", copy=True) for t in (q_offsets, k_offsets))
     for name, t in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
         if int(t[0]) != 0 or bool((t[1:] < t[:-1]).any()):
             raise RuntimeError(f"relm_mp attention plan: {name} must ascend from 0.")

@@ -69,6 +69,20 @@ def test_attention_formulation_and_gradient(mask) -> None:
         lambda *a: mp.cross_attention(*a, plan, key_mask=kept if mask else None, scale=0.7), (q, k, v))
 
 
+def test_plan_keeps_its_own_lengths() -> None:
+    """Later writes to the offsets neither move a plan's graphs nor undo the check that was made of them."""
+
+    qo, ko = torch.tensor([0, 2, 5]), torch.tensor([0, 3, 9])
+    q, k, v = (_randn(n, 2, 4, seed=n) for n in (5, 9, 9))
+    plan = mp.attention_plan(qo, ko, 2)
+    want = mp.cross_attention(q, k, v, plan)
+    ko[1], qo[1] = 5, 1
+    assert torch.equal(mp.cross_attention(q, k, v, plan), want)
+    ko[1] = 100
+    assert torch.equal(mp.cross_attention(q, k, v, plan), want)
+    assert plan.k_offsets.tolist() == [0, 3, 9] and plan.q_offsets.tolist() == [0, 2, 5]
+
+
 def test_orthogonalise_formulation() -> None:
     tall = _randn(9, 4, seed=5)
     got = mp.orthogonalise(tall, steps=8, coefficients=(1.5, -0.5, 0.0))
