@@ -567,7 +567,7 @@ typedef struct relm_mp_attention_plan {
     int32_t num_key_items; /* key items: keys of a graph against a range of its rows     */
     int32_t num_key_parts;
     int32_t num_key_joins;
-    int32_t num_idle_items; /* graphs with keys and no queries                           */
+    int32_t num_idle_items; /* ranges of keys of graphs without queries                  */
     int32_t reserved;
     const void* table;
 } relm_mp_attention_plan;

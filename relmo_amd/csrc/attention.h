@@ -36,8 +36,8 @@ struct AttnJoin {
 };
 static_assert(sizeof(AttnItem) == 32 && sizeof(AttnJoin) == 32, "table records");
 
-// The tables of a plan, one after the other; behind the row items those of graphs that have
-// keys and no queries.
+// The tables of a plan, one after the other; behind the row items the ranges of keys of
+// graphs that have no queries.
 inline const AttnItem* plan_items(const relm_mp_attention_plan& p) { return static_cast<const AttnItem*>(p.table); }
 inline const AttnJoin* plan_joins(const relm_mp_attention_plan& p) {
     return reinterpret_cast<const AttnJoin*>(plan_items(p) + p.num_items + p.num_idle_items);

@@ -19,6 +19,7 @@ constexpr int64_t kLargeWorkgroups = 512;
 constexpr int64_t kPartUnit = 128;     // parts end on whole tiles of keys and rows
 constexpr int64_t kLeastKeys = 512;    // of a part: shorter ones cost more to join than to walk
 constexpr int64_t kLeastRows = 256;
+constexpr int64_t kIdleKeys = 1024;    // of an item of a graph without queries, whose keys get zeros: at most 1 MB of them
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -114,9 +115,10 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
                                    s.parts > 1 ? L.num_parts++ : -1, static_cast<int32_t>(ko[b]),
                                    static_cast<int32_t>(keys[b])});
         }
-        if (rows[b] == 0 && keys[b] > 0)
-            L.idle.push_back({static_cast<int32_t>(qo[b]), 0, 0, static_cast<int32_t>(ko[b]), static_cast<int32_t>(keys[b]), -1,
-                              static_cast<int32_t>(ko[b]), static_cast<int32_t>(keys[b])});
+        for (int64_t k = 0; rows[b] == 0 && k < keys[b]; k += kIdleKeys)
+            L.idle.push_back({static_cast<int32_t>(qo[b]), 0, 0, static_cast<int32_t>(ko[b] + k),
+                              static_cast<int32_t>(std::min(kIdleKeys, keys[b] - k)), -1, static_cast<int32_t>(ko[b]),
+                              static_cast<int32_t>(keys[b])});
         const Split t = split(rows[b], row_share);
         for (int64_t k = 0; k < keys[b]; k += L.key_tile) {
             const int32_t n = static_cast<int32_t>(std::min<int64_t>(L.key_tile, keys[b] - k));

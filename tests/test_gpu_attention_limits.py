@@ -50,3 +50,23 @@ def test_values_far_below_the_dominant_key(queries, dim, keys, dtype) -> None:
             tol = want * (2 * UNIT[dtype] + (16 + gap) * U + _walk(keys)) + (2.0 ** -24 if dtype == torch.float16 else 0)
             over = (out.double() - want).abs() - tol
             assert bool((over <= 0).all()), (gap, at, float((out.double() / want - 1).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,dim", [([0, 3], 64), ([9, 0], 33), ([0, 60], 128), ([0, 0], 5)])
+def test_keys_of_graphs_without_queries_get_zeros(queries, dim, dtype) -> None:
+    from relmo_amd import mp
+
+    keys = [70_001, 5_000]
+    g = _gen(dim)
+    q, grad = (torch.randn(sum(queries), 2, dim, device=DEV, generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(sum(keys), 1, dim, device=DEV, generator=g).to(dtype) for _ in range(2))
+    plan = mp.attention_plan(_offsets(queries), _offsets(keys), 2, 1)
+    for _ in range(3):  # memory that the results will take
+        torch.full_like(k, float("nan"))
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    _dq, dk, dv = torch.autograd.grad(mp.cross_attention(q, k, v, plan), (q, k, v), grad)
+    edge = keys[0]
+    for b, rows in enumerate((slice(0, edge), slice(edge, None))):
+        for t in (dk, dv):
+            assert bool(t[rows].isfinite().all()) and (queries[b] > 0) == bool(t[rows].abs().sum() > 0)

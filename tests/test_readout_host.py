@@ -217,6 +217,28 @@ def test_plan_covers_every_pair_once(capi, queries, keys, heads, kv_heads) -> No
         assert len(parts) == j[6] and {(r[3], r[4]) for r in parts} == {(j[3], j[4])}
 
 
+@pytest.mark.parametrize("queries,keys", [([0], [1 << 27]), ([3, 0, 0, 2], [50, 1_000_001, 4, 0]), ([0, 0], [1024, 1025])])
+def test_keys_without_queries_are_cut_into_short_ranges(capi, queries, keys) -> None:
+    """A graph's keys that no query reads are listed once each, in order, in ranges short enough that a workgroup's
+    share of them (keys times quarters of 128 values) counts in 32 bits and that many workgroups share a long graph."""
+
+    plan, (_items, idle, *_rest) = _build(capi, queries, keys, 1, 1)
+    ko = _offsets(keys)
+    at = {ko[b]: ko[b + 1] for b, n in enumerate(queries) if n == 0 and keys[b]}
+    ends = dict(at)
+    for _q, _r, rows, first, n, part, graph_first, graph_keys in idle:
+        assert rows == 0 and part < 0 and 1 <= n <= 4096 and n * 32 < 1 << 31
+        assert graph_first in ends and graph_first + graph_keys == ends[graph_first]
+        at_now = [k for k in at if k == first]
+        assert at_now, first  # starts where the range before it ended
+        end = at.pop(first)
+        if first + n < end:
+            at[first + n] = end
+        else:
+            assert first + n == end
+    assert not at
+
+
 def test_plan_refusals(capi) -> None:
     plan = capi.AttentionPlan()
 
