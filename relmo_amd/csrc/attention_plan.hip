@@ -92,15 +92,30 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
     L.key_tile = 5 * padded(keys, 128) <= 6 * padded(keys, 64) ? 128 : 64;
 
     // A share is what a workgroup gets when all the work is dealt to them.
-    int64_t row_work = 0, key_work = 0;
+    using Work = unsigned __int128;  // rows, keys and heads of 2^31, 2^31 and 2^12
+    Work row_work = 0, key_work = 0;
     for (int64_t b = 0; b < graphs; ++b) {
-        row_work += ceil_div(rows[b], L.row_tile) * keys[b] * kv_heads;
-        key_work += ceil_div(keys[b], L.key_tile) * rows[b] * kv_heads;
+        row_work += static_cast<Work>(ceil_div(rows[b], L.row_tile)) * keys[b] * kv_heads;
+        key_work += static_cast<Work>(ceil_div(keys[b], L.key_tile)) * rows[b] * kv_heads;
     }
-    const int64_t key_share = std::max(kLeastKeys, ceil_div(row_work, L.row_tile >= 64 ? kLargeWorkgroups : kWorkgroups));
-    const int64_t row_share = std::max(kLeastRows, ceil_div(key_work, L.key_tile == 128 ? kLargeWorkgroups : kWorkgroups));
+    const auto share = [](Work work, int64_t workgroups, int64_t least) {
+        const Work s = (work + workgroups - 1) / workgroups;
+        return s > RELM_MP_MAX_ROWS ? int64_t{RELM_MP_MAX_ROWS} : std::max(least, static_cast<int64_t>(s));
+    };
+    const int64_t key_share = share(row_work, L.row_tile >= 64 ? kLargeWorkgroups : kWorkgroups, kLeastKeys);
+    const int64_t row_share = share(key_work, L.key_tile == 128 ? kLargeWorkgroups : kWorkgroups, kLeastRows);
 
-    constexpr size_t kMost = size_t{1} << 24;  // table records: 512 MB
+    // table records: 512 MB of them at most, counted before any is made
+    constexpr int64_t kMost = int64_t{1} << 24;
+    int64_t records = 0;
+    for (int64_t b = 0; b < graphs; ++b) {
+        const int64_t row_parts = split(keys[b], key_share).parts, key_parts = split(rows[b], row_share).parts;
+        records += ceil_div(rows[b], L.row_tile) * (row_parts + (row_parts > 1 ? 1 : 0));
+        records += ceil_div(keys[b], L.key_tile) * (key_parts + (key_parts > 1 ? 1 : 0));
+        if (rows[b] == 0) records += ceil_div(keys[b], kIdleKeys);
+        if (records > kMost)
+            return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: too many queries and keys for one plan");
+    }
     for (int64_t b = 0; b < graphs; ++b) {
         const Split s = split(keys[b], key_share);
         for (int64_t r = 0; r < rows[b]; r += L.row_tile) {
@@ -131,8 +146,6 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
                                        static_cast<int32_t>(ko[b] + k), n, t.parts > 1 ? L.num_key_parts++ : -1,
                                        static_cast<int32_t>(ko[b]), static_cast<int32_t>(keys[b])});
         }
-        if (L.items.size() + L.idle.size() + L.key_items.size() + L.joins.size() + L.key_joins.size() > kMost)
-            return set_error(RELM_MP_ERR_INVALID_ARGUMENT, "relm_mp attention plan: too many queries and keys for one plan");
     }
     deal(L.items, [](const AttnItem& i) { return i.keys; });
     // graphs of few rows have their backward in one kernel over the row items, but for float

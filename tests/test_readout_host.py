@@ -259,6 +259,36 @@ def test_plan_refusals(capi) -> None:
                                                    ctypes.byref(plan)) == capi.ERR_WORKSPACE
 
 
+def test_plans_past_the_table_are_refused_before_they_are_laid_out() -> None:
+    """The longest lengths, whose pairs do not count in 64 bits: refused by their counts, in little memory."""
+
+    import subprocess
+    import sys
+
+    code = """
+import ctypes, resource
+from relmo_amd import capi
+lib = capi.lib()
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (256 << 20), resource.getrlimit(resource.RLIMIT_AS)[1]))
+most = (1 << 31) - 2
+plan = capi.AttentionPlan()
+for nq, nk, heads, kv_heads in ((most, most, 4096, 4096), (most, most, 1, 1), (most, 1, 1, 1), (0, most, 1, 1), (most // 4096, most, 4096, 1)):
+    o = [(ctypes.c_int64 * 2)(0, n) for n in (nq, nk)]
+    rc = lib.relm_mp_attention_plan_build(o[0], o[1], 1, nq, nk, heads, kv_heads, None, 0, ctypes.byref(plan))
+    print(rc, capi.last_error())
+"""
+    from pathlib import Path
+
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100,
+                         cwd=Path(__file__).resolve().parent.parent)
+    assert run.returncode == 0, run.stderr[-2000:]
+    lines = run.stdout.strip().splitlines()
+    assert len(lines) == 5
+    for line in lines:
+        assert line.startswith("1 ") and "too many queries and keys" in line, lines
+
+
 @pytest.mark.parametrize("struct", ["relm_mp_attention_plan", "relm_mp_head_rows", "relm_mp_update"])
 def test_readout_struct_layouts_match_header(tmp_path, capi, struct) -> None:
     import subprocess
