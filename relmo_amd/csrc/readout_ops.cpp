@@ -41,6 +41,13 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
+// The ops have no forward-mode formula.  A tangent does not need requires_grad (nor grad mode),
+// so every call looks for one: the result would leave it out.
+void refuse_tangents(std::initializer_list<const Tensor*> tensors, const char* op) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivative is implemented.");
+}
+
 // Gradients that are themselves not differentiated: with create_graph, differentiating
 // them raises.
 variable_list once(variable_list grads, const char* op) {
@@ -150,6 +157,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         if (!grads[0].defined()) return {grads[1], grads[1], Tensor(), Tensor()};
+        refuse_tangents({&grads[0], &grads[1]}, "add_rms_norm backward");
         const auto [dx, dw] = norm_backward(grads[0], grads[1], saved[0], saved[1], saved[2]);
         return once({dx, dx, dw, Tensor()}, "add_rms_norm");
     }
@@ -163,6 +171,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
+        refuse_tangents({&grads[0]}, "rms_norm backward");
         const auto [dx, dw] = norm_backward(grads[0], Tensor(), saved[0], saved[1], saved[2]);
         return once({dx, dw, Tensor()}, "rms_norm");
     }
@@ -171,6 +180,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 }  // namespace
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+    refuse_tangents({&x, &residual, &weight}, "add_rms_norm");
     if (wants_grad({&x, &residual, &weight})) {
         const variable_list o = AddRmsNorm::apply(x, residual, weight, eps);
         return {o[0], o[1]};
@@ -180,6 +190,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual,
 }
 
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
+    refuse_tangents({&x, &weight}, "rms_norm");
     if (wants_grad({&x, &weight})) return RmsNorm::apply(x, weight, eps);
     return norm_forward(x, std::nullopt, weight, eps, false).y;
 }
@@ -187,6 +198,8 @@ Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
 // (q, scale, h); without a residual h is empty (it would be x).
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& residual,
                                                     const Tensor& weight, double eps) {
+    refuse_tangents({&x, &weight}, "add_rms_norm_fp8");
+    if (residual.has_value()) refuse_tangents({&*residual}, "add_rms_norm_fp8");
     const NormArgs a = norm_args(x, residual, weight, "add_rms_norm_fp8");
     c10::OptionalDeviceGuard guard(x.device());
     Tensor q = at::empty(x.sizes(), a.x.options().dtype(at::kFloat8_e4m3fn));
@@ -392,6 +405,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto s = ctx->get_saved_variables();
+        refuse_tangents({&grads[0]}, "cross_attention backward");
         const auto plan = ctx->saved_data["plan"].toCustomClass<AttentionPlan>();
         const auto [dq, dk, dv] = attention_backward(grads[0], s[0], s[1], s[2], *plan, s[3],
                                                      ctx->saved_data["scale"].toDouble(), s[4], s[5]);
@@ -403,6 +417,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 
 Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t plan, const std::optional<Tensor>& key_mask,
                        double scale) {
+    refuse_tangents({&q, &k, &v}, "cross_attention");
     const auto p = plan_of(plan, "cross_attention");
     if (wants_grad({&q, &k, &v})) return CrossAttention::apply(q, k, v, key_mask, p, scale);
     return std::get<0>(attention_forward(q, k, v, *p, key_mask.value_or(Tensor()), scale, false));
@@ -423,6 +438,7 @@ std::vector<Tensor> orthogonalise(at::TensorList updates, int64_t steps, at::Arr
     results.reserve(updates.size());
     mats.reserve(updates.size());
     for (const Tensor& u : updates) {
+        refuse_tangents({&u}, op);
         check_like(u, updates[0], op, "every update");
         TORCH_CHECK_VALUE(u.dim() >= 2, op, ": updates must be matrices or stacks of them.");
         const int64_t rows = u.size(-2), cols = u.size(-1);

@@ -3,7 +3,7 @@
 ``add_rms_norm`` (a residual stream's norm, also with an 8-bit output),
 ``cross_attention`` (per-graph queries to the graphs' objects) and ``orthogonalise``
 (the weight updates of what they train), without counterparts in relmo.  GPU tensors of float32, bfloat16 or float16 run the library's ops, which check
-their arguments and make their own autograd nodes; CPU tensors (and the policy's fallback)
+their arguments and make their own autograd nodes (reverse mode once; forward mode raises); CPU tensors (and the policy's fallback)
 run the ATen formulations below, which autograd differentiates.
 """
 
