@@ -597,8 +597,16 @@ int relm_mp_cross_attention(int dtype, const relm_mp_attention_plan* plan, const
                             const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim,
                             const uint8_t* key_mask, float scale, void* out, float* lse,
                             void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
+/* The same for training: in place of lse, stats [q_rows, heads, 2] receives each row's
+ * largest score <q, k_j> and 1 / sum_j exp(scale * (<q, k_j> - largest)) (both 0 for a row
+ * without a kept key), from which the backward has the forward's own probabilities. */
+int relm_mp_cross_attention_keep(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* q,
+                                 const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim,
+                                 const uint8_t* key_mask, float scale, void* out, float* stats,
+                                 void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
 
-/* Backward from grad (of out), the forward's inputs, out and lse:
+/* Backward from grad (of out), the forward's inputs, out and stats (_kept) or lse (which
+ * rounds the row's maximum and total into one float: probabilities err by |lse| 2^-23):
  *   delta = <grad, out>, ds_j = p_j (<grad, v_j> - delta), dq = scale sum_j ds_j k_j,
  *   dk_j = scale sum ds_j q, dv_j = sum p_j grad (over the queries and heads that read j).
  * dq [q_rows, heads, head_dim], dk and dv [k_rows, kv_heads, head_dim] contiguous, fully
@@ -610,6 +618,12 @@ int relm_mp_cross_attention_backward(int dtype, const relm_mp_attention_plan* pl
                                      int64_t head_dim, const uint8_t* key_mask, float scale,
                                      const void* out, const float* lse, void* dq, void* dk, void* dv,
                                      void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
+int relm_mp_cross_attention_backward_kept(int dtype, const relm_mp_attention_plan* plan,
+                                          const relm_mp_head_rows* grad, const relm_mp_head_rows* q,
+                                          const relm_mp_head_rows* k, const relm_mp_head_rows* v,
+                                          int64_t head_dim, const uint8_t* key_mask, float scale,
+                                          const void* out, const float* stats, void* dq, void* dk, void* dv,
+                                          void* workspace, size_t workspace_bytes, relm_mp_stream_t stream);
 
 /* ---- orthogonalised update ----------------------------------------------------
  * Per matrix: X = in / (|in|_F + eps), then `steps` times A = X X^T, X <- a X + (b A + c

@@ -80,8 +80,10 @@ EXPORTED_SYMBOLS = (
     "relm_mp_attention_plan_build",
     "relm_mp_cross_attention_workspace_size",
     "relm_mp_cross_attention",
+    "relm_mp_cross_attention_keep",
     "relm_mp_cross_attention_backward_workspace_size",
     "relm_mp_cross_attention_backward",
+    "relm_mp_cross_attention_backward_kept",
     "relm_mp_orthogonalise_workspace_size",
     "relm_mp_orthogonalise",
 )
@@ -258,8 +260,12 @@ _SIGNATURES = {
     "relm_mp_cross_attention_workspace_size": (_sz, [_AP, _i64]),
     "relm_mp_cross_attention": (
         _int, [_int, _AP, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "relm_mp_cross_attention_keep": (
+        _int, [_int, _AP, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _sz, _vp]),
     "relm_mp_cross_attention_backward_workspace_size": (_sz, [_AP, _i64]),
     "relm_mp_cross_attention_backward": (
+        _int, [_int, _AP, _HR, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "relm_mp_cross_attention_backward_kept": (
         _int, [_int, _AP, _HR, _HR, _HR, _HR, _i64, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "relm_mp_orthogonalise_workspace_size": (_sz, [ctypes.POINTER(Update), ctypes.c_int32]),
     "relm_mp_orthogonalise": (

@@ -63,13 +63,21 @@ inline size_t attention_key_part_floats(const relm_mp_attention_plan& p, int64_t
     return static_cast<size_t>(p.num_key_parts) * p.kv_heads * p.key_tile * 2 * attention_part_stride(head_dim);
 }
 
+// What the forward keeps of a row for the backward: its largest score (not scaled) and one over
+// the total of exp(scale * (s - top)).
+struct RowStats {
+    float top, inv_total;
+};
+static_assert(sizeof(RowStats) == 8, "two floats to a row");
+
 struct AttnOperands {
     relm_mp_head_rows q, k, v, grad;
     int64_t head_dim;
     const uint8_t* key_mask;
     float scale;
     void* out;       // forward's output; the backward reads it
-    float* lse;
+    float* lse;      // forward
+    RowStats* stats;
     float* delta;    // backward: [q_rows, heads]
     void *dq, *dk, *dv;
     float* parts;

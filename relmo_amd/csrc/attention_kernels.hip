@@ -15,6 +15,8 @@
 // outputs' own; with float values nothing is rounded).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "attention.h"
 #include "device_utils.h"
 #include "internal.h"
@@ -122,13 +124,23 @@ struct Args {
     const AttnItem* items;
     const AttnJoin* joins;
     T* out;
-    float* lse;
+    float* lse;     // forward, may be NULL
+    RowStats* stats;  // forward (may be NULL): written; backward: read
     float* delta;
     T *dq, *dk, *dv;
     float* parts;        // sums of the parts, rows of part_stride floats
     float* part_stats;   // forward: their maxima and totals
     int part_stride;
 };
+
+// What the forward leaves of row `at` (query and head): its statistics and their logarithm.  A
+// row that had no finite score gets probabilities of 0.
+template <typename T>
+__device__ __forceinline__ void put_stats(const Args<T>& a, int64_t at, float top, float total) {
+    const bool none = total == 0.0f;
+    if (a.lse != nullptr) a.lse[at] = none ? -kInf : fmaf(top, a.scale, log2f(total) * kLn2);
+    if (a.stats != nullptr) a.stats[at] = {none ? 0.0f : top, none ? 0.0f : 1.0f / total};
+}
 
 // A workgroup's item and key head.  Neighbouring heads of an item share the lines of
 // its rows, and neighbouring items a graph's keys: they run on one XCD.
@@ -370,23 +382,22 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            // the maximum of scale * log2(e) * s; the factor is positive
-            float top = -kInf;
+            float top = -kInf;  // the scale is positive: also the scaled scores' maximum
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, s[c][r][t][i]);
-            const float most = fmaxf(m[r], lanes_max(top) * sl2);
+            const float most = fmaxf(m[r], lanes_max(top));
             if (__any(most > m[r])) {
-                const float shrink = exp2_of(m[r] - (most == -kInf ? 0.0f : most));
+                const float shrink = exp2_of(m[r] * sl2 - (most == -kInf ? 0.0f : most * sl2));
                 total[r] *= shrink;
 #pragma unroll
                 for (int n = 0; n < ND; ++n) o[r][n] *= shrink;
                 m[r] = most;
             }
-            const float base = m[r] == -kInf ? 0.0f : m[r];
+            const float base = m[r] == -kInf ? 0.0f : m[r] * sl2;
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
@@ -429,8 +440,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
         if (w.it.part < 0) {
             const float inv = sum_p == 0.0f ? 0.0f : 1.0f / sum_p;
             put4<T>(a.out + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * inv);
-            if (col == 0 && a.lse != nullptr)
-                a.lse[p.row * a.heads + p.head] = sum_p == 0.0f ? -kInf : (top + log2f(sum_p)) * kLn2;
+            if (col == 0) put_stats(a, p.row * a.heads + p.head, top, sum_p);
         } else {
             const int64_t slot = (static_cast<int64_t>(w.it.part) * a.kv_heads + w.head) * a.row_tile + row;
             if (col < a.part_stride) *reinterpret_cast<f32x4*>(a.parts + slot * a.part_stride + col) = sum;
@@ -474,11 +484,11 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
             float top = -kInf, sum_p = 0.0f;
 #pragma unroll
             for (int v = 0; v < S::kSharers; ++v) top = fmaxf(top, tops[v * R + slot]);
-            const float base = top == -kInf ? 0.0f : top;
+            const float base = top == -kInf ? 0.0f : top * sl2;
             f32x4 sum = f32x4(0.0f);
 #pragma unroll
             for (int v = 0; v < S::kSharers; ++v) {
-                const float share = exp2_of(tops[v * R + slot] - base);
+                const float share = exp2_of(tops[v * R + slot] * sl2 - base);
                 sum_p = fmaf(totals[v * R + slot], share, sum_p);
                 sum += *reinterpret_cast<const f32x4*>(sums + (v * R + slot) * DP + col) * share;
             }
@@ -487,7 +497,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
     }
 }
 
-// Joins the parts of a row: out = sum_p 2^(m_p - m) sum_p / sum_p 2^(m_p - m) total_p, or
+// Joins the parts of a row: out = sum_p e^(m_p - m) sum_p / sum_p e^(m_p - m) total_p, or
 // dq = sum of the parts (DQ).  Thread groups of DP / 4 threads hold a row's sums.  MANY: a
 // workgroup per row and key head, its groups taking every kJoinGroups-th part; else a row
 // to each group.  Latency bound: 512 parts are 32 rounds of loads of a group, four at a time
@@ -522,7 +532,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
             for (int p = 0; p < j.parts; ++p) top = fmaxf(top, a.part_stats[2 * (slot0 + p * step)]);
         }
     }
-    const float base = top == -kInf ? 0.0f : top;
+    const float sl2 = a.scale * kLog2e, base = top == -kInf ? 0.0f : top * sl2;
     f32x4 sum = f32x4(0.0f);
     float total = 0.0f;
     if (mine) {
@@ -533,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
             if constexpr (DQ) {
                 sum += x;
             } else {
-                const float share = exp2_of(a.part_stats[2 * slot] - base);
+                const float share = exp2_of(a.part_stats[2 * slot] * sl2 - base);
                 total = fmaf(a.part_stats[2 * slot + 1], share, total);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = fmaf(x[i], share, sum[i]);
@@ -557,21 +567,19 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
         put4<T>(to, col, a.dim, sum * a.scale);
     } else {
         put4<T>(to, col, a.dim, sum * (total == 0.0f ? 0.0f : 1.0f / total));
-        if (col == 0 && a.lse != nullptr)
-            a.lse[p.row * a.heads + p.head] = total == 0.0f ? -kInf : (top + log2f(total)) * kLn2;
+        if (col == 0) put_stats(a, p.row * a.heads + p.head, top, total);
     }
 }
 
-// Scores to probabilities and their gradients in place: s becomes p, dp becomes ds.
-__device__ __forceinline__ void backward_scores(f32x4 (&s)[2], f32x4 (&dp)[2], float sl2, float lse2, float delta) {
+// The probabilities of the backward are the forward's: 2^(sl2 s - base) / total with the row's
+// maximum and total as they were (the logarithm of the total would enter the exponent
+// rounded at its own size).  dp of a query's keys becomes ds times the query's total, by which
+// dq is divided at the end.
+__device__ __forceinline__ void backward_scores(const f32x4 (&s)[2], f32x4 (&dp)[2], float sl2, float base, float delta) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float p = exp2_of(fmaf(s[t][i], sl2, -lse2));
-            s[t][i] = p;
-            dp[t][i] = p * (dp[t][i] - delta);
-        }
+        for (int i = 0; i < 4; ++i) dp[t][i] = exp2_of(fmaf(s[t][i], sl2, -base)) * (dp[t][i] - delta);
 }
 
 // Whether a graph keeps exactly one key (graphs of at most 128 are looked at; the same for
@@ -622,11 +630,7 @@ __device__ __forceinline__ void into_unit(f32x4 (&ds)[2], float& unit, f32x4 (&s
     }
 }
 
-// A row's log2 total for the backward; +inf (all probabilities 0) for a row that had no
-// finite score.
-__device__ __forceinline__ float lse2_of(float lse) { return lse == -kInf ? kInf : lse * kLog2e; }
-
-// dq of a row item: like the forward, with the probabilities recomputed from lse.  A row's
+// dq of a row item: like the forward, with the probabilities recomputed from its statistics.  A row's
 // delta is left for the key kernel (parts of one row leave the same).  Three products to the
 // forward's two, bound alike: 8 graphs of 500 to 1500 queries x 900 to 2100 keys, 8 heads
 // of 64 in bfloat16, 70 us (490 TFLOP/s).
@@ -648,7 +652,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
     bool real[RT];
-    float lse2[RT], delta[RT], unit[RT];
+    float base[RT], share[RT], delta[RT], unit[RT];
     f32x4 dq[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -665,7 +669,9 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
         delta[r] = lanes_sum(sum);
-        lse2[r] = lse2_of(a.lse[at[r].row * a.heads + at[r].head]);
+        const RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
+        base[r] = stats.top * sl2;
+        share[r] = stats.inv_total;
         unit[r] = kStartUnit<T>;
         if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
 #pragma unroll
@@ -706,7 +712,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
             Frag<T> ds[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                backward_scores(s[r], dp[r], sl2, lse2[r], delta[r]);
+                backward_scores(s[r], dp[r], sl2, base[r], delta[r]);
                 into_unit<T>(dp[r], unit[r], dq[r]);
                 ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
             }
@@ -722,7 +728,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int n = 0; n < ND; ++n) dq[r][n] = any ? dq[r][n] * (1.0f / unit[r]) : f32x4(0.0f);
+        for (int n = 0; n < ND; ++n) dq[r][n] = any ? dq[r][n] * (share[r] / unit[r]) : f32x4(0.0f);
     const auto finish = [&](int row, Place p, int col, f32x4 sum) {
         if (w.it.part < 0) {
             put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * a.scale);
@@ -767,7 +773,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
     constexpr int BR = 64, ST = kLdsStride<T, DP>, ND = DP / 16;
     __shared__ __align__(16) T qt[BR * ST];
     __shared__ __align__(16) T gt[BR * ST];
-    __shared__ __align__(16) float row_lse2[BR];
+    __shared__ __align__(16) float row_base[BR];
+    __shared__ __align__(16) float row_share[BR];
     __shared__ __align__(16) float row_delta[BR];
     // an item's keys are taken by key_tile / (64 KT) workgroups
     const int slices = a.key_tile / (64 * KT);
@@ -802,7 +809,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
 
     const bool alone = one_key(a.key_mask, w.it);
     TileLoad<T, DP, BR> ql, gl;
-    float lse_in = 0.0f, delta_in = 0.0f;
+    float base_in = 0.0f, share_in = 0.0f, delta_in = 0.0f;
     const auto fetch = [&](int r0) {
         const int left = w.it.rows - r0;
         const auto place = [&](int row) { return place_of(a, w.it.q_first, head, w.it.row0 + r0 + min(row, left - 1)); };
@@ -816,9 +823,14 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         }, a.dim);
         const int row = static_cast<int>(threadIdx.x) % BR;
         const Place p = place(row);
-        lse_in = lse2_of(a.lse[p.row * a.heads + p.head]);
+        const RowStats stats = a.stats[p.row * a.heads + p.head];
+        base_in = stats.top * sl2;
+        share_in = stats.inv_total;
         delta_in = a.delta[p.row * a.heads + p.head];
-        if (row >= left) lse_in = kInf;  // probability 0
+        if (row >= left) {  // probability 0
+            base_in = kInf;
+            share_in = 0.0f;
+        }
     };
     if (w.it.rows > 0) fetch(0);
     for (int r0 = 0; r0 < w.it.rows; r0 += BR) {
@@ -827,7 +839,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         ql.template store<FIT>(qt, a.dim, left >= BR, [&](int row) { return row < left; });
         gl.template store<FIT>(gt, a.dim, left >= BR, [&](int row) { return row < left; });
         if (threadIdx.x < BR) {
-            row_lse2[threadIdx.x] = lse_in;
+            row_base[threadIdx.x] = base_in;
+            row_share[threadIdx.x] = share_in;
             row_delta[threadIdx.x] = delta_in;
         }
         __syncthreads();
@@ -860,11 +873,12 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
             for (int t = 0; t < KT; ++t) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const f32x4 lse2 = *reinterpret_cast<const f32x4*>(row_lse2 + c * 32 + h * 16 + g * 4);
+                    const f32x4 base = *reinterpret_cast<const f32x4*>(row_base + c * 32 + h * 16 + g * 4);
+                    const f32x4 share = *reinterpret_cast<const f32x4*>(row_share + c * 32 + h * 16 + g * 4);
                     const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + c * 32 + h * 16 + g * 4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = exp2_of(fmaf(s[t][h][i], sl2, -lse2[i]));
+                        const float p = exp2_of(fmaf(s[t][h][i], sl2, -base[i])) * share[i];
                         s[t][h][i] = p;
                         dp[t][h][i] = p * (dp[t][h][i] - delta[i]);
                     }
@@ -952,7 +966,8 @@ struct FewRows {
     __align__(16) T q[kRows * kStride];
     __align__(16) T g[kRows * kStride];
     __align__(16) float starts[kKeys];
-    __align__(16) float lse2[32];
+    __align__(16) float base[32];
+    __align__(16) float share[32];
     __align__(16) float delta[32];
 };
 
@@ -980,7 +995,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
     bool real[RT];
-    float lse2[RT], delta[RT], unit[RT];
+    float base[RT], delta[RT], unit[RT];
     f32x4 dq[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -997,9 +1012,11 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
         delta[r] = lanes_sum(sum);
-        lse2[r] = lse2_of(a.lse[at[r].row * a.heads + at[r].head]);
+        RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
+        base[r] = stats.top * sl2;
         if (!real[r]) {  // a sum over rows must not see it
-            lse2[r] = kInf;
+            base[r] = kInf;
+            stats.inv_total = 0.0f;
             delta[r] = 0.0f;
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) qf[r].f[c] = gf[r].f[c] = Frag<T>(static_cast<T>(0.0f));
@@ -1014,7 +1031,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 lds_put<T>(m.g + row * ST + c * 32 + g * 8, gf[r].f[c]);
             }
             if (g == 0) {
-                m.lse2[row] = lse2[r];
+                m.base[row] = base[r];
+                m.share[row] = stats.inv_total;
                 m.delta[row] = delta[r];
             }
         }
@@ -1042,7 +1060,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         Frag<T> ds[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            backward_scores(s[r], dp[r], sl2, lse2[r], delta[r]);
+            backward_scores(s[r], dp[r], sl2, base[r], delta[r]);
             if (alone) dp[r][0] = dp[r][1] = f32x4(0.0f);
             into_unit<T>(dp[r], unit[r], dq[r]);
             ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
@@ -1077,11 +1095,12 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
             f32x4 pr[2] = {f32x4(0.0f), f32x4(0.0f)}, dr[2] = {f32x4(0.0f), f32x4(0.0f)}, none[1] = {f32x4(0.0f)};
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const f32x4 row_lse2 = *reinterpret_cast<const f32x4*>(m.lse2 + r * 16 + g * 4);
+                const f32x4 row_base = *reinterpret_cast<const f32x4*>(m.base + r * 16 + g * 4);
+                const f32x4 row_share = *reinterpret_cast<const f32x4*>(m.share + r * 16 + g * 4);
                 const f32x4 row_delta = *reinterpret_cast<const f32x4*>(m.delta + r * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    pr[r][i] = exp2_of(fmaf(s2[r][i], sl2, -row_lse2[i]));
+                    pr[r][i] = exp2_of(fmaf(s2[r][i], sl2, -row_base[i])) * row_share[i];
                     dr[r][i] = pr[r][i] * (dp2[r][i] - row_delta[i]);
                 }
             }
@@ -1121,7 +1140,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
 #pragma unroll
         for (int n = 0; n < ND; ++n)
             *reinterpret_cast<f32x4*>(sums + (wave * R + r * 16 + l % 16) * DP + n * 16 + g * 4) =
-                any ? dq[r][n] * (1.0f / unit[r]) : f32x4(0.0f);
+                any ? dq[r][n] * (m.share[r * 16 + l % 16] / unit[r]) : f32x4(0.0f);
     __syncthreads();
     for (int u = static_cast<int>(threadIdx.x); u < w.it.rows * (DP / 4); u += kThreads) {
         const int row = u / (DP / 4), col = (u % (DP / 4)) * 4;
@@ -1165,6 +1184,16 @@ __global__ __launch_bounds__(kThreads, (kFewRowsWaves<T, DP>)) void k_attention_
     few_rows_backward<T, DP, 1, FIT>(a, w, m);
 }
 
+// The statistics of rows of which only the logarithm of the total was kept: those of a single
+// score of that size.
+__global__ __launch_bounds__(kThreads) void k_attention_stats(const float* lse, int64_t rows, float scale, RowStats* stats) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; at < rows; at += step) {
+        const float x = lse[at];
+        stats[at] = {x == -kInf ? 0.0f : x / scale, x == -kInf ? 0.0f : 1.0f};
+    }
+}
+
 // ---- launches -----------------------------------------------------------------------
 
 template <typename T>
@@ -1187,6 +1216,7 @@ Args<T> args_of(const relm_mp_attention_plan& p, const AttnOperands& o) {
     a.joins = plan_joins(p);
     a.out = static_cast<T*>(o.out);
     a.lse = o.lse;
+    a.stats = o.stats;
     a.delta = o.delta;
     a.dq = static_cast<T*>(o.dq);
     a.dk = static_cast<T*>(o.dk);
@@ -1308,6 +1338,14 @@ hipError_t launch_cross_attention(int dtype, const relm_mp_attention_plan& p, co
     hipError_t e = hipErrorInvalidValue;
     with_value_type(dtype, [&](auto t) { e = forward<decltype(t)>(p, o, st); });
     return e;
+}
+
+hipError_t launch_attention_stats(const relm_mp_attention_plan& p, const float* lse, float scale, RowStats* stats, hipStream_t st) {
+    const int64_t rows = p.q_rows * p.heads;
+    const int64_t blocks = std::min<int64_t>((rows + kThreads - 1) / kThreads, 256 * 32);
+    if (rows > 0)
+        hipLaunchKernelGGL(k_attention_stats, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, lse, rows, scale, stats);
+    return hipGetLastError();
 }
 
 hipError_t launch_cross_attention_backward(int dtype, const relm_mp_attention_plan& p, const AttnOperands& o,

@@ -59,10 +59,13 @@ int norm(int dtype, const void* x, const void* r, const void* w, int64_t rows, i
     return RELM_MP_OK;
 }
 
-// The backward's delta first, then the parts of dq or of dk and dv (one after the other
-// in the same memory).
+// The backward's delta first, then the rows' statistics where only their lse is given, then the
+// parts of dq or of dk and dv (one after the other in the same memory).
 size_t delta_bytes(const relm_mp_attention_plan& p) {
     return align_up(static_cast<size_t>(p.q_rows) * p.heads * sizeof(float), 256);
+}
+size_t stats_bytes(const relm_mp_attention_plan& p) {
+    return align_up(static_cast<size_t>(p.q_rows) * p.heads * sizeof(RowStats), 256);
 }
 
 bool null_rows(const relm_mp_head_rows* r) { return r == nullptr || r->data == nullptr; }
@@ -73,6 +76,74 @@ int check_attention(int dtype, const relm_mp_attention_plan* plan, int64_t head_
     if (head_dim < 1 || head_dim > RELM_MP_MAX_HEAD_DIM) return bad("cross_attention: head_dim must be in [1, 128]");
     if (!(scale > 0.0f) || std::isinf(scale)) return bad("cross_attention: scale must be finite and positive");
     if (plan->table == nullptr && plan->table_bytes > 0) return bad("cross_attention: the plan has no table");
+    return RELM_MP_OK;
+}
+
+int attention_forward(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* q, const relm_mp_head_rows* k,
+                      const relm_mp_head_rows* v, int64_t head_dim, const uint8_t* key_mask, float scale, void* out, float* lse,
+                      RowStats* stats, void* workspace, size_t workspace_bytes, relm_mp_stream_t stream) {
+    RELM_TRY(check_attention(dtype, plan, head_dim, scale));
+    if (plan->q_rows == 0) return RELM_MP_OK;
+    if (null_rows(q) || out == nullptr || (plan->k_rows > 0 && (null_rows(k) || null_rows(v))))
+        return bad("cross_attention: NULL array");
+    RELM_TRY(check_workspace(workspace, workspace_bytes, relm_mp_cross_attention_workspace_size(plan, head_dim),
+                             "cross_attention"));
+    AttnOperands o{};
+    o.q = *q;
+    if (plan->k_rows > 0) {
+        o.k = *k;
+        o.v = *v;
+    }
+    o.head_dim = head_dim;
+    o.key_mask = key_mask;
+    o.scale = scale;
+    o.out = out;
+    o.lse = lse;
+    o.stats = stats;
+    o.parts = static_cast<float*>(workspace);
+    RELM_HIP(launch_cross_attention(dtype, *plan, o, static_cast<hipStream_t>(stream)), "relm_mp cross_attention kernel");
+    return RELM_MP_OK;
+}
+
+// From the rows' statistics, or from their lse (then stats is NULL).
+int attention_backward(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* grad, const relm_mp_head_rows* q,
+                       const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim, const uint8_t* key_mask,
+                       float scale, const void* out, const float* lse, const RowStats* stats, void* dq, void* dk, void* dv,
+                       void* workspace, size_t workspace_bytes, relm_mp_stream_t stream) {
+    RELM_TRY(check_attention(dtype, plan, head_dim, scale));
+    if (plan->q_rows == 0 && plan->k_rows == 0) return RELM_MP_OK;
+    if ((plan->q_rows > 0 &&
+         (null_rows(grad) || null_rows(q) || out == nullptr || (lse == nullptr && stats == nullptr) || dq == nullptr)) ||
+        (plan->k_rows > 0 && (null_rows(k) || null_rows(v) || dk == nullptr || dv == nullptr)))
+        return bad("cross_attention_backward: NULL array");
+    RELM_TRY(check_workspace(workspace, workspace_bytes, relm_mp_cross_attention_backward_workspace_size(plan, head_dim),
+                             "cross_attention_backward"));
+    char* const at = static_cast<char*>(workspace);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    AttnOperands o{};
+    if (plan->q_rows > 0) {
+        o.q = *q;
+        o.grad = *grad;
+    }
+    if (plan->k_rows > 0) {
+        o.k = *k;
+        o.v = *v;
+    }
+    o.head_dim = head_dim;
+    o.key_mask = key_mask;
+    o.scale = scale;
+    o.out = const_cast<void*>(out);  // read only
+    o.delta = reinterpret_cast<float*>(at);
+    o.stats = const_cast<RowStats*>(stats);
+    if (stats == nullptr) {
+        o.stats = reinterpret_cast<RowStats*>(at + delta_bytes(*plan));
+        RELM_HIP(launch_attention_stats(*plan, lse, scale, o.stats, st), "relm_mp cross_attention statistics kernel");
+    }
+    o.dq = dq;
+    o.dk = dk;
+    o.dv = dv;
+    o.parts = reinterpret_cast<float*>(at + delta_bytes(*plan) + stats_bytes(*plan));
+    RELM_HIP(launch_cross_attention_backward(dtype, *plan, o, st), "relm_mp cross_attention backward kernels");
     return RELM_MP_OK;
 }
 
@@ -164,31 +235,22 @@ int relm_mp_cross_attention(int dtype, const relm_mp_attention_plan* plan, const
                             const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim, const uint8_t* key_mask,
                             float scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
                             relm_mp_stream_t stream) {
-    RELM_TRY(check_attention(dtype, plan, head_dim, scale));
-    if (plan->q_rows == 0) return RELM_MP_OK;
-    if (null_rows(q) || out == nullptr || (plan->k_rows > 0 && (null_rows(k) || null_rows(v))))
-        return bad("cross_attention: NULL array");
-    RELM_TRY(check_workspace(workspace, workspace_bytes, relm_mp_cross_attention_workspace_size(plan, head_dim),
-                             "cross_attention"));
-    AttnOperands o{};
-    o.q = *q;
-    if (plan->k_rows > 0) {
-        o.k = *k;
-        o.v = *v;
-    }
-    o.head_dim = head_dim;
-    o.key_mask = key_mask;
-    o.scale = scale;
-    o.out = out;
-    o.lse = lse;
-    o.parts = static_cast<float*>(workspace);
-    RELM_HIP(launch_cross_attention(dtype, *plan, o, static_cast<hipStream_t>(stream)), "relm_mp cross_attention kernel");
-    return RELM_MP_OK;
+    return attention_forward(dtype, plan, q, k, v, head_dim, key_mask, scale, out, lse, nullptr, workspace, workspace_bytes,
+                             stream);
+}
+
+int relm_mp_cross_attention_keep(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* q,
+                                 const relm_mp_head_rows* k, const relm_mp_head_rows* v, int64_t head_dim,
+                                 const uint8_t* key_mask, float scale, void* out, float* stats, void* workspace,
+                                 size_t workspace_bytes, relm_mp_stream_t stream) {
+    if (plan != nullptr && plan->q_rows > 0 && stats == nullptr) return bad("cross_attention_keep: NULL array");
+    return attention_forward(dtype, plan, q, k, v, head_dim, key_mask, scale, out, nullptr, reinterpret_cast<RowStats*>(stats),
+                             workspace, workspace_bytes, stream);
 }
 
 size_t relm_mp_cross_attention_backward_workspace_size(const relm_mp_attention_plan* plan, int64_t head_dim) {
     if (plan == nullptr) return 0;
-    return delta_bytes(*plan) +
+    return delta_bytes(*plan) + stats_bytes(*plan) +
            std::max(attention_part_floats(*plan, head_dim), attention_key_part_floats(*plan, head_dim)) * sizeof(float);
 }
 
@@ -197,35 +259,17 @@ int relm_mp_cross_attention_backward(int dtype, const relm_mp_attention_plan* pl
                                      int64_t head_dim, const uint8_t* key_mask, float scale, const void* out, const float* lse,
                                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                                      relm_mp_stream_t stream) {
-    RELM_TRY(check_attention(dtype, plan, head_dim, scale));
-    if (plan->q_rows == 0 && plan->k_rows == 0) return RELM_MP_OK;
-    if ((plan->q_rows > 0 && (null_rows(grad) || null_rows(q) || out == nullptr || lse == nullptr || dq == nullptr)) ||
-        (plan->k_rows > 0 && (null_rows(k) || null_rows(v) || dk == nullptr || dv == nullptr)))
-        return bad("cross_attention_backward: NULL array");
-    RELM_TRY(check_workspace(workspace, workspace_bytes, relm_mp_cross_attention_backward_workspace_size(plan, head_dim),
-                             "cross_attention_backward"));
-    AttnOperands o{};
-    if (plan->q_rows > 0) {
-        o.q = *q;
-        o.grad = *grad;
-    }
-    if (plan->k_rows > 0) {
-        o.k = *k;
-        o.v = *v;
-    }
-    o.head_dim = head_dim;
-    o.key_mask = key_mask;
-    o.scale = scale;
-    o.out = const_cast<void*>(out);  // read only
-    o.lse = const_cast<float*>(lse);
-    o.delta = static_cast<float*>(workspace);
-    o.dq = dq;
-    o.dk = dk;
-    o.dv = dv;
-    o.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(*plan));
-    RELM_HIP(launch_cross_attention_backward(dtype, *plan, o, static_cast<hipStream_t>(stream)),
-             "relm_mp cross_attention backward kernels");
-    return RELM_MP_OK;
+    return attention_backward(dtype, plan, grad, q, k, v, head_dim, key_mask, scale, out, lse, nullptr, dq, dk, dv, workspace,
+                              workspace_bytes, stream);
+}
+
+int relm_mp_cross_attention_backward_kept(int dtype, const relm_mp_attention_plan* plan, const relm_mp_head_rows* grad,
+                                          const relm_mp_head_rows* q, const relm_mp_head_rows* k, const relm_mp_head_rows* v,
+                                          int64_t head_dim, const uint8_t* key_mask, float scale, const void* out,
+                                          const float* stats, void* dq, void* dk, void* dv, void* workspace,
+                                          size_t workspace_bytes, relm_mp_stream_t stream) {
+    return attention_backward(dtype, plan, grad, q, k, v, head_dim, key_mask, scale, out, nullptr,
+                              reinterpret_cast<const RowStats*>(stats), dq, dk, dv, workspace, workspace_bytes, stream);
 }
 
 size_t relm_mp_orthogonalise_workspace_size(const relm_mp_update* updates, int32_t count) {

@@ -231,6 +231,9 @@ struct AttnOperands;
 int build_attention_plan(const int64_t* q_offsets, const int64_t* k_offsets, int64_t graphs, int64_t q_rows, int64_t k_rows,
                          int32_t heads, int32_t kv_heads, void* table, size_t table_bytes, relm_mp_attention_plan* plan);
 hipError_t launch_cross_attention(int dtype, const relm_mp_attention_plan& plan, const AttnOperands& o, hipStream_t st);
+struct RowStats;  // of rows whose lse is given
+hipError_t launch_attention_stats(const relm_mp_attention_plan& plan, const float* lse, float scale, RowStats* stats,
+                                  hipStream_t st);
 hipError_t launch_cross_attention_backward(int dtype, const relm_mp_attention_plan& plan, const AttnOperands& o,
                                            hipStream_t st);
 

@@ -351,27 +351,31 @@ AttnArgs attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const
     return a;
 }
 
-// (out, lse); lse only if kept.
+// (out, stats); stats only if kept.
 std::tuple<Tensor, Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionPlan& plan,
                                              const Tensor& key_mask, double scale, bool keep) {
     const AttnArgs a = attention_args(q, k, v, plan, key_mask, scale);
     c10::OptionalDeviceGuard guard(q.device());
     const auto stream = c10::hip::getCurrentHIPStream(q.get_device());
     plan.used_on(stream);
-    Tensor out = at::empty(q.sizes(), q.options()), lse;
-    if (keep) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    Tensor out = at::empty(q.sizes(), q.options()), stats;
+    if (keep) stats = at::empty({q.size(0), q.size(1), 2}, q.options().dtype(at::kFloat));
     const size_t need = relm_mp_cross_attention_workspace_size(&plan.plan, a.dim);
     const Tensor ws = need > 0 ? bytes(need, q) : Tensor();
     const relm_mp_head_rows qr = head_rows(a.q), kr = head_rows(a.k), vr = head_rows(a.v);
-    raise_if(relm_mp_cross_attention(a.dtype, &plan.plan, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale, out.data_ptr(),
-                                     keep ? lse.data_ptr<float>() : nullptr, need > 0 ? ws.data_ptr() : nullptr, need,
-                                     stream.stream()));
-    return {out, lse};
+    void* const wp = need > 0 ? ws.data_ptr() : nullptr;
+    if (keep)
+        raise_if(relm_mp_cross_attention_keep(a.dtype, &plan.plan, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale, out.data_ptr(),
+                                              stats.data_ptr<float>(), wp, need, stream.stream()));
+    else
+        raise_if(relm_mp_cross_attention(a.dtype, &plan.plan, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale, out.data_ptr(),
+                                         nullptr, wp, need, stream.stream()));
+    return {out, stats};
 }
 
 std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v,
                                                       const AttentionPlan& plan, const Tensor& key_mask, double scale,
-                                                      const Tensor& out, const Tensor& lse) {
+                                                      const Tensor& out, const Tensor& stats) {
     const AttnArgs a = attention_args(q, k, v, plan, key_mask, scale);
     check_same(grad, q, "cross_attention", "its gradient");
     c10::OptionalDeviceGuard guard(q.device());
@@ -384,21 +388,21 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& grad, const 
     const size_t need = relm_mp_cross_attention_backward_workspace_size(&plan.plan, a.dim);
     const Tensor ws = bytes(need, q);
     const relm_mp_head_rows gr = head_rows(g), qr = head_rows(a.q), kr = head_rows(a.k), vr = head_rows(a.v);
-    raise_if(relm_mp_cross_attention_backward(a.dtype, &plan.plan, &gr, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale,
-                                              out.const_data_ptr(), lse.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
-                                              dv.data_ptr(), ws.data_ptr(), need, stream.stream()));
+    raise_if(relm_mp_cross_attention_backward_kept(a.dtype, &plan.plan, &gr, &qr, &kr, &vr, a.dim, a.mask_ptr(), a.scale,
+                                                   out.const_data_ptr(), stats.const_data_ptr<float>(), dq.data_ptr(),
+                                                   dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need, stream.stream()));
     return {dq, dk, dv};
 }
 
-// Keeps the inputs, the output and each row's logarithm of its total; the backward
-// computes the probabilities again.
+// Keeps the inputs, the output and each row's maximum and total; the backward computes the
+// probabilities again.
 struct CrossAttention : torch::autograd::Function<CrossAttention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                           const std::optional<Tensor>& key_mask, const c10::intrusive_ptr<AttentionPlan>& plan,
                           double scale) {
         const Tensor mask = key_mask.value_or(Tensor());
-        const auto [out, lse] = attention_forward(q, k, v, *plan, mask, scale, true);
-        ctx->save_for_backward({q, k, v, mask, out, lse});
+        const auto [out, stats] = attention_forward(q, k, v, *plan, mask, scale, true);
+        ctx->save_for_backward({q, k, v, mask, out, stats});
         ctx->saved_data["plan"] = plan;
         ctx->saved_data["scale"] = scale;
         return out;

@@ -9,7 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from .test_gpu_attention import DEV, DTYPES, U, UNIT, _gen, _offsets, _walk
+from .test_gpu_attention import DEV, DTYPES, U, UNIT, _check, _definition, _gen, _make, _offsets, _run, _walk
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,87 @@ def test_keys_of_graphs_without_queries_get_zeros(queries, dim, dtype) -> None:
     for b, rows in enumerate((slice(0, edge), slice(edge, None))):
         for t in (dk, dv):
             assert bool(t[rows].isfinite().all()) and (queries[b] > 0) == bool(t[rows].abs().sum() > 0)
+
+
+def _ladder(queries, keys, dim, dtype, size, scale=1.0, step=1):
+    """q, k, v, grad whose scores are size * scale less 0 .. 5 steps, exactly."""
+
+    g = _gen(keys)
+    root = 2.0 ** round(0.5 * torch.tensor(float(size)).log2().item())
+    level = torch.randint(0, 6, (keys,), device=DEV, generator=g)
+    level[keys // 3] = 0
+    q = torch.zeros(queries, 1, dim, device=DEV, dtype=torch.float64)
+    k = torch.zeros(keys, 1, dim, device=DEV, dtype=torch.float64)
+    q[:, 0, 0] = root
+    k[:, 0, 0] = size / root - level.double() * step / root
+    v, grad = torch.randn(keys, 1, dim, device=DEV, generator=g), torch.randn(queries, 1, dim, device=DEV, generator=g)
+    return q.to(dtype), k.to(dtype), v.to(dtype), grad.to(dtype), -level.double() * step * scale
+
+
+@pytest.mark.parametrize("queries,dim", ROWS)
+@pytest.mark.parametrize("size", [2.0 ** 4, 2.0 ** 8, 2.0 ** 12, 2.0 ** 16])
+def test_probabilities_of_large_scores_add_up_to_one(queries, dim, size) -> None:
+    """Scores of a row a few units apart around a large one: the backward's probabilities are the forward's."""
+    from relmo_amd import mp
+
+    keys = 700
+    q, k, v, grad, s = _ladder(queries, keys, dim, torch.float32, size)
+    plan = mp.attention_plan(_offsets([queries]), _offsets([keys]), 1)
+    out, dq, dk, dv = _run(q, k, v, grad, plan, None, scale=1.0)
+    p = torch.softmax(s, 0)
+    ep = (16 + 5) * U
+    V, G = v[:, 0].double(), grad[:, 0].double()
+    want = (p[:, None] * V).sum(0)
+    assert float(((out[:, 0].double() - want).abs() - (ep + _walk(keys)) * (p[:, None] * V.abs()).sum(0)).max()) <= 0
+    want = p[:, None] * G.sum(0)
+    assert float(((dv[:, 0].double() - want).abs() - (ep + _walk(queries) + U) * p[:, None] * G.abs().sum(0)).max()) <= 0
+    # ds adds up to nothing over a row's keys, up to its terms' errors
+    ds = dk[:, 0, 0].double() / float(q[0, 0, 0])
+    dp_err = 3 * _walk(dim) * (G.abs().sum(0) * V.abs().amax(0)).sum() + _walk(keys) * (G.abs().sum(0) * V.abs().amax(0)).sum()
+    assert abs(float(ds.sum())) <= float(dp_err + 2 * ep * ds.abs().sum() + _walk(keys) * ds.abs().sum())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,keys,dim", [([3, 0, 9], [70, 5, 0], 32), ([60, 33], [70, 300], 64), ([1], [6_000], 40)])
+def test_c_entries_from_the_logarithm_of_the_total(queries, keys, dim, dtype) -> None:
+    """``relm_mp_cross_attention`` with its lse and the backward from it, without the torch binding."""
+    import ctypes
+
+    from relmo_amd import capi
+
+    lib, code = capi.lib(), {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}[dtype]
+    q, k, v, grad, mask = _make(queries, keys, 2, 1, dim, dtype, seed=dim, mask="random")
+    offsets = [_offsets(n).cpu() for n in (queries, keys)]
+    plan = capi.AttentionPlan()
+    args = (offsets[0].data_ptr(), offsets[1].data_ptr(), len(queries), sum(queries), sum(keys), 2, 1)
+    capi.check(lib.relm_mp_attention_plan_build(*args, None, 0, ctypes.byref(plan)))
+    table = torch.empty(plan.table_bytes, dtype=torch.uint8)
+    capi.check(lib.relm_mp_attention_plan_build(*args, table.data_ptr(), plan.table_bytes, ctypes.byref(plan)))
+    table = table.to(DEV)
+    plan.table = table.data_ptr()
+    rows = [ctypes.byref(capi.HeadRows(t.data_ptr(), t.stride(0), t.stride(1))) for t in (q, k, v, grad)]
+    scale, stream = dim ** -0.5, capi._stream(q)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    ws = torch.empty(max(lib.relm_mp_cross_attention_workspace_size(plan, dim),
+                         lib.relm_mp_cross_attention_backward_workspace_size(plan, dim)), dtype=torch.uint8, device=DEV)
+    capi.check(lib.relm_mp_cross_attention(code, plan, *rows[:3], dim, mask.data_ptr(), scale, out.data_ptr(), lse.data_ptr(),
+                                           ws.data_ptr(), ws.numel(), stream))
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    capi.check(lib.relm_mp_cross_attention_backward(code, plan, rows[3], *rows[:3], dim, mask.data_ptr(), scale, out.data_ptr(),
+                                                    lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
+                                                    ws.numel(), stream))
+    val, tol = _definition(q, k, v, grad, mask, queries, keys, scale)
+    _check((out, dq, dk, dv), val, tol, 2.0 ** -24 if dtype == torch.float16 else 1e-30)
+    q0 = k0 = 0
+    for nq, nk in zip(queries, keys):
+        kept = k[k0:k0 + nk, 0][mask[k0:k0 + nk]].double()
+        s = torch.einsum("nhd,kd->nhk", q[q0:q0 + nq].double(), kept) * scale
+        want = torch.logsumexp(s, 2) if kept.size(0) else torch.full(s.shape[:2], -torch.inf, device=DEV, dtype=torch.float64)
+        got = lse[q0:q0 + nq].double()
+        err = _walk(dim) * scale * q[q0:q0 + nq].double().norm(dim=2) * (kept.norm(dim=1).max() if kept.size(0) else 0)
+        assert torch.equal(got.isinf(), want.isinf())
+        fine = ~want.isinf()
+        assert bool(((got - want).abs()[fine] <= (err + 16 * U * (1 + want.abs()))[fine]).all())
+        q0, k0 = q0 + nq, k0 + nk
+    null = lib.relm_mp_cross_attention_keep(code, plan, *rows[:3], dim, None, scale, out.data_ptr(), None, ws.data_ptr(), ws.numel(), stream)
+    assert null == capi.ERR_INVALID_ARGUMENT and "NULL" in capi.last_error()
