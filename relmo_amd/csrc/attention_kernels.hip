@@ -291,6 +291,34 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <typename T>
 constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
 
+// The exponent of a score s under its row's maximum m, sl2 (s - m).  As fma(s, sl2, -(sl2 m)) it is
+// one instruction, and off by the rounding of sl2 m: nothing of a row's own distribution is
+// lost, but the largest probability is not 1, and from 2^30 on that rounding passes the
+// exponent's range (below the largest float everything was infinite, or 0).  Rows past
+// kFarScore take the difference first, which is exact near the maximum: `off` is then m and
+// `base` 0.  Float rows always do (2^-24 is their own accuracy, and matrix instructions bound
+// them); 16-bit ones have 2^-17 up to there, a thirtieth of a half's unit.
+constexpr float kFarScore = 256.0f;
+
+template <typename T>
+struct Under {
+    float base, off;
+    __device__ __forceinline__ Under() = default;
+    __device__ __forceinline__ Under(float top, float sl2) {
+        const float m = top == -kInf ? 0.0f : top;
+        const bool far = sizeof(T) == 4 || fabsf(m * sl2) >= kFarScore;
+        base = far ? 0.0f : m * sl2;
+        off = far ? m : 0.0f;
+    }
+    __device__ __forceinline__ bool far() const { return sizeof(T) == 4 || off != 0.0f; }
+};
+// Takes off from scores where some row of the wave is far.
+template <int N>
+__device__ __forceinline__ void lower(f32x4 (&s)[N], float off) {
+#pragma unroll
+    for (int t = 0; t < N; ++t) s[t] -= off;
+}
+
 // Two waves to a SIMD with 16-bit values: one's matrix instructions run beside the other's
 // exponentials.  Float rows need the registers of both.
 template <typename T>
@@ -342,10 +370,13 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
     }
     f32x4 o[RT][ND];
     float m[RT], total[RT];
+    Under<T> under[RT];
+    bool far = false;  // whether some row of the wave is
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         m[r] = -kInf;
         total[r] = 0.0f;
+        under[r] = Under<T>(m[r], sl2);
 #pragma unroll
         for (int n = 0; n < ND; ++n) o[r][n] = f32x4(0.0f);
     }
@@ -391,20 +422,25 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, s[c][r][t][i]);
             const float most = fmaxf(m[r], lanes_max(top));
             if (__any(most > m[r])) {
-                const float shrink = exp2_of(m[r] * sl2 - (most == -kInf ? 0.0f : most * sl2));
+                const float shrink = exp2_of((m[r] - (most == -kInf ? 0.0f : most)) * sl2);
                 total[r] *= shrink;
 #pragma unroll
                 for (int n = 0; n < ND; ++n) o[r][n] *= shrink;
                 m[r] = most;
+                under[r] = Under<T>(most, sl2);
+                far = far || __any(under[r].far());
             }
-            const float base = m[r] == -kInf ? 0.0f : m[r] * sl2;
+            if (far) {
+#pragma unroll
+                for (int c = 0; c < S::kChunks; ++c) lower(s[c][r], under[r].off);
+            }
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = exp2_of(fmaf(s[c][r][t][i], sl2, -base));
+                        const float p = exp2_of(fmaf(s[c][r][t][i], sl2, -under[r].base));
                         s[c][r][t][i] = p * kProbabilityUnit<T>;
                         total[r] += p;
                     }
@@ -484,11 +520,11 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
             float top = -kInf, sum_p = 0.0f;
 #pragma unroll
             for (int v = 0; v < S::kSharers; ++v) top = fmaxf(top, tops[v * R + slot]);
-            const float base = top == -kInf ? 0.0f : top * sl2;
+            const float most = top == -kInf ? 0.0f : top;
             f32x4 sum = f32x4(0.0f);
 #pragma unroll
             for (int v = 0; v < S::kSharers; ++v) {
-                const float share = exp2_of(tops[v * R + slot] * sl2 - base);
+                const float share = exp2_of((tops[v * R + slot] - most) * sl2);
                 sum_p = fmaf(totals[v * R + slot], share, sum_p);
                 sum += *reinterpret_cast<const f32x4*>(sums + (v * R + slot) * DP + col) * share;
             }
@@ -532,7 +568,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
             for (int p = 0; p < j.parts; ++p) top = fmaxf(top, a.part_stats[2 * (slot0 + p * step)]);
         }
     }
-    const float sl2 = a.scale * kLog2e, base = top == -kInf ? 0.0f : top * sl2;
+    const float sl2 = a.scale * kLog2e, most = top == -kInf ? 0.0f : top;
     f32x4 sum = f32x4(0.0f);
     float total = 0.0f;
     if (mine) {
@@ -543,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
             if constexpr (DQ) {
                 sum += x;
             } else {
-                const float share = exp2_of(a.part_stats[2 * slot] * sl2 - base);
+                const float share = exp2_of((a.part_stats[2 * slot] - most) * sl2);
                 total = fmaf(a.part_stats[2 * slot + 1], share, total);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = fmaf(x[i], share, sum[i]);
@@ -571,7 +607,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
     }
 }
 
-// The probabilities of the backward are the forward's: 2^(sl2 s - base) / total with the row's
+// The probabilities of the backward are the forward's: 2^(sl2 (s - top)) / total with the row's
 // maximum and total as they were (the logarithm of the total would enter the exponent
 // rounded at its own size).  dp of a query's keys becomes ds times the query's total, by which
 // dq is divided at the end.
@@ -652,7 +688,9 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
     bool real[RT];
-    float base[RT], share[RT], delta[RT], unit[RT];
+    Under<T> under[RT];
+    float share[RT], delta[RT], unit[RT];
+    bool far = false;
     f32x4 dq[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -670,7 +708,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
             for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
         delta[r] = lanes_sum(sum);
         const RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
-        base[r] = stats.top * sl2;
+        under[r] = Under<T>(stats.top, sl2);
+        far = far || __any(under[r].far());
         share[r] = stats.inv_total;
         unit[r] = kStartUnit<T>;
         if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
@@ -712,7 +751,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
             Frag<T> ds[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                backward_scores(s[r], dp[r], sl2, base[r], delta[r]);
+                if (far) lower(s[r], under[r].off);
+                backward_scores(s[r], dp[r], sl2, under[r].base, delta[r]);
                 into_unit<T>(dp[r], unit[r], dq[r]);
                 ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
             }
@@ -774,6 +814,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
     __shared__ __align__(16) T qt[BR * ST];
     __shared__ __align__(16) T gt[BR * ST];
     __shared__ __align__(16) float row_base[BR];
+    __shared__ __align__(16) float row_off[BR];
     __shared__ __align__(16) float row_share[BR];
     __shared__ __align__(16) float row_delta[BR];
     // an item's keys are taken by key_tile / (64 KT) workgroups
@@ -809,7 +850,9 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
 
     const bool alone = one_key(a.key_mask, w.it);
     TileLoad<T, DP, BR> ql, gl;
-    float base_in = 0.0f, share_in = 0.0f, delta_in = 0.0f;
+    Under<T> under_in;
+    float share_in = 0.0f, delta_in = 0.0f;
+    static_assert(BR == kWave, "a wave's lanes hold the statistics of a tile's rows");
     const auto fetch = [&](int r0) {
         const int left = w.it.rows - r0;
         const auto place = [&](int row) { return place_of(a, w.it.q_first, head, w.it.row0 + r0 + min(row, left - 1)); };
@@ -824,11 +867,12 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         const int row = static_cast<int>(threadIdx.x) % BR;
         const Place p = place(row);
         const RowStats stats = a.stats[p.row * a.heads + p.head];
-        base_in = stats.top * sl2;
+        under_in = Under<T>(stats.top, sl2);
         share_in = stats.inv_total;
         delta_in = a.delta[p.row * a.heads + p.head];
         if (row >= left) {  // probability 0
-            base_in = kInf;
+            under_in.base = kInf;
+            under_in.off = 0.0f;
             share_in = 0.0f;
         }
     };
@@ -839,10 +883,12 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         ql.template store<FIT>(qt, a.dim, left >= BR, [&](int row) { return row < left; });
         gl.template store<FIT>(gt, a.dim, left >= BR, [&](int row) { return row < left; });
         if (threadIdx.x < BR) {
-            row_base[threadIdx.x] = base_in;
+            row_base[threadIdx.x] = under_in.base;
+            row_off[threadIdx.x] = under_in.off;
             row_share[threadIdx.x] = share_in;
             row_delta[threadIdx.x] = delta_in;
         }
+        const bool far = __any(under_in.far());  // a wave's lanes hold all rows of the tile
         __syncthreads();
         if (left > BR) fetch(r0 + BR);
 #pragma unroll
@@ -866,6 +912,14 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
                         s[t][h] = mma<T>(qr, kf[t].f[i], s[t][h]);
                         dp[t][h] = mma<T>(gr, vf[t].f[i], dp[t][h]);
                     }
+                }
+            }
+            if (far) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 off = *reinterpret_cast<const f32x4*>(row_off + c * 32 + h * 16 + g * 4);
+#pragma unroll
+                    for (int t = 0; t < KT; ++t) s[t][h] -= off;
                 }
             }
             Frag<T> pf[KT], dsf[KT];
@@ -967,6 +1021,7 @@ struct FewRows {
     __align__(16) T g[kRows * kStride];
     __align__(16) float starts[kKeys];
     __align__(16) float base[32];
+    __align__(16) float off[32];
     __align__(16) float share[32];
     __align__(16) float delta[32];
 };
@@ -995,7 +1050,8 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
     bool real[RT];
-    float base[RT], delta[RT], unit[RT];
+    float unit[RT];
+    bool far = false;
     f32x4 dq[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -1011,16 +1067,18 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
-        delta[r] = lanes_sum(sum);
+        float delta = lanes_sum(sum);
         RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
-        base[r] = stats.top * sl2;
+        Under<T> under(stats.top, sl2);
         if (!real[r]) {  // a sum over rows must not see it
-            base[r] = kInf;
+            under.base = kInf;
+            under.off = 0.0f;
             stats.inv_total = 0.0f;
-            delta[r] = 0.0f;
+            delta = 0.0f;
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) qf[r].f[c] = gf[r].f[c] = Frag<T>(static_cast<T>(0.0f));
         }
+        far = far || __any(under.far());
         unit[r] = kStartUnit<T>;
 #pragma unroll
         for (int n = 0; n < ND; ++n) dq[r][n] = f32x4(0.0f);
@@ -1031,9 +1089,10 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 lds_put<T>(m.g + row * ST + c * 32 + g * 8, gf[r].f[c]);
             }
             if (g == 0) {
-                m.base[row] = base[r];
+                m.base[row] = under.base;
+                m.off[row] = under.off;
                 m.share[row] = stats.inv_total;
-                m.delta[row] = delta[r];
+                m.delta[row] = delta;
             }
         }
     }
@@ -1060,7 +1119,9 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         Frag<T> ds[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            backward_scores(s[r], dp[r], sl2, base[r], delta[r]);
+            const int row = r * 16 + l % 16;  // its statistics from LDS: in registers they spilled others
+            if (far) lower(s[r], m.off[row]);
+            backward_scores(s[r], dp[r], sl2, m.base[row], m.delta[row]);
             if (alone) dp[r][0] = dp[r][1] = f32x4(0.0f);
             into_unit<T>(dp[r], unit[r], dq[r]);
             ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
@@ -1098,6 +1159,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 const f32x4 row_base = *reinterpret_cast<const f32x4*>(m.base + r * 16 + g * 4);
                 const f32x4 row_share = *reinterpret_cast<const f32x4*>(m.share + r * 16 + g * 4);
                 const f32x4 row_delta = *reinterpret_cast<const f32x4*>(m.delta + r * 16 + g * 4);
+                if (far) s2[r] -= *reinterpret_cast<const f32x4*>(m.off + r * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     pr[r][i] = exp2_of(fmaf(s2[r][i], sl2, -row_base[i])) * row_share[i];

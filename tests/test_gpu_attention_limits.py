@@ -1,4 +1,5 @@
-"""GPU tests of ``mp.cross_attention`` where its numbers run out: probabilities that a 16-bit type cannot hold.
+"""GPU tests of ``mp.cross_attention`` where its numbers run out: probabilities that a 16-bit type cannot hold,
+scores of any size.
 
 Scores are made exact here (one value of a query, a power of two, meets one value of a key), so a probability errs by
 its own roundings only: at most 16 units of 2^-24 and one for each unit of the score's distance from the row's maximum,
@@ -154,3 +155,34 @@ def test_c_entries_from_the_logarithm_of_the_total(queries, keys, dim, dtype) ->
         q0, k0 = q0 + nq, k0 + nk
     null = lib.relm_mp_cross_attention_keep(code, plan, *rows[:3], dim, None, scale, out.data_ptr(), None, ws.data_ptr(), ws.numel(), stream)
     assert null == capi.ERR_INVALID_ARGUMENT and "NULL" in capi.last_error()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,dim", ROWS)
+@pytest.mark.parametrize("keys", [100, 6_000])
+def test_scores_past_the_floats_units(queries, dim, keys, dtype) -> None:
+    """Scores whose neighbours in float lie hundreds apart: the largest takes all, two equal ones take half each."""
+    from relmo_amd import mp
+
+    g = _gen(3)
+    plan = mp.attention_plan(_offsets([queries]), _offsets([keys]), 1)
+    for scale in (1.0, 1.3):
+        for ties in (1, 2):
+            q = torch.zeros(queries, 1, dim, device=DEV)
+            k = torch.zeros(keys, 1, dim, device=DEV)
+            q[:, 0, 2] = 2.0 ** 14
+            k[:, 0, 2] = -(2.0 ** 13)
+            top = [7, keys - 9][:ties]
+            k[top, 0, 2] = 57344.0  # 7 * 2^13
+            v, grad = torch.randn(keys, 1, dim, device=DEV, generator=g), torch.randn(queries, 1, dim, device=DEV, generator=g)
+            v, grad = v.to(dtype), grad.to(dtype)
+            out, _dq, dk, dv = _run(q.to(dtype), k.to(dtype), v, grad, plan, None, scale=scale * 2.0 ** 12)
+            u = max(UNIT[dtype], U)
+            want = v[top].double().mean(0)
+            assert bool(((out.double() - want).abs() <= 2 * u * want.abs() + 16 * U).all())
+            G = grad.double().sum(0)
+            tol = (2 * u + _walk(queries)) * grad.double().abs().sum(0) / ties
+            assert bool(((dv[top].double() - G / ties).abs() <= tol).all())
+            rest = torch.ones(keys, dtype=torch.bool, device=DEV)
+            rest[top] = False
+            assert float(dv[rest].abs().sum()) == 0 and float(dk[rest].abs().sum()) == 0
