@@ -19,8 +19,7 @@ struct AttnItem {
     int32_t key_first;  // first key of the item in the batch
     int32_t keys;
     int32_t part;       // -1: the item's rows (keys) are whole; else where its sums go
-    int32_t graph_key_first;
-    int32_t graph_keys;
+    int32_t pad[2];
 };
 
 // Rows (keys) whose parts [part0, part0 + parts) are joined.

@@ -618,20 +618,19 @@ __device__ __forceinline__ void backward_scores(const f32x4 (&s)[2], f32x4 (&dp)
         for (int i = 0; i < 4; ++i) dp[t][i] = exp2_of(fmaf(s[t][i], sl2, -base)) * (dp[t][i] - delta);
 }
 
-// Whether a graph keeps exactly one key (graphs of at most 128 are looked at; the same for
-// all waves).  Its queries' probability is 1 whatever the scores, so ds is 0 - not what is
-// left when two roundings of <grad, v> are subtracted.
-__device__ __forceinline__ bool one_key(const uint8_t* mask, const AttnItem& it) {
-    if (it.graph_keys > 128 || (mask == nullptr && it.graph_keys != 1)) return false;
-    if (mask == nullptr) return true;
-    int kept = 0;
+// <grad, out> of a wave's 16 rows, each in the four lanes that share its row: the diagonal of a
+// matrix product of the rows, whose sums run in the same order as those of <grad, v>.  A row
+// whose softmax is one key then has <grad, v> - delta = 0, not what is left when two
+// roundings are subtracted; and what is no number stays none.
+template <typename T, int DP>
+__device__ __forceinline__ float row_delta_of(const RowFrags<T, DP>& out, const RowFrags<T, DP>& grad) {
+    f32x4 d = f32x4(0.0f);
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const int k = w * 64 + lane_id();
-        const bool is = mask[it.graph_key_first + static_cast<int64_t>(min(k, it.graph_keys - 1))] != 0;
-        kept += __popcll(__ballot(k < it.graph_keys && is));
-    }
-    return kept == 1;
+    for (int c = 0; c < DP / 32; ++c) d = mma<T>(out.f[c], grad.f[c], d);
+    // entry i of lane l is <out of row 4 (l / 16) + i, grad of row l % 16>
+    const int l = lane_id(), i = l % 4, row = l % 16;
+    const float mine = i == 0 ? d[0] : i == 1 ? d[1] : i == 2 ? d[2] : d[3];
+    return __shfl(mine, (row / 4) * 16 + row);
 }
 
 // Half values lose bits below 2^-14, where ds of keys with small probabilities lies.  A lane
@@ -701,12 +700,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         gf[r].template fetch<FIT>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
         RowFrags<T, DP> of;
         of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
-        float sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
-        delta[r] = lanes_sum(sum);
+        delta[r] = row_delta_of<T, DP>(of, gf[r]);
         const RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
         under[r] = Under<T>(stats.top, sl2);
         far = far || __any(under[r].far());
@@ -728,10 +722,9 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
-    const int keys = w.it.keys == 0 || one_key(a.key_mask, w.it) ? 0 : w.it.keys;  // to walk: none leaves dq = 0
     bool any = false;  // whether some key of the item is kept (the same for all waves)
-    if (keys > 0) fetch(0);
-    for (int k0 = 0; k0 < keys; k0 += BN) {
+    if (w.it.keys > 0) fetch(0);
+    for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         any = any || !bits.none();
         __syncthreads();
@@ -848,7 +841,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         unit[t] = kStartUnit<T>;
     }
 
-    const bool alone = one_key(a.key_mask, w.it);
     TileLoad<T, DP, BR> ql, gl;
     Under<T> under_in;
     float share_in = 0.0f, delta_in = 0.0f;
@@ -938,7 +930,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
                     }
                 }
                 pf[t] = frag_of<T>(s[t][0] * kProbabilityUnit<T>, s[t][1] * kProbabilityUnit<T>);
-                if (alone) dp[t][0] = dp[t][1] = f32x4(0.0f);
                 into_unit<T>(dp[t], unit[t], dk[t]);
                 dsf[t] = frag_of<T>(dp[t][0], dp[t][1]);
             }
@@ -1045,7 +1036,6 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         bits.fetch(a.key_mask, first, left);
     };
     if (w.it.keys > 0) fetch(0);
-    const bool alone = w.it.keys > 0 && one_key(a.key_mask, w.it);
 
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
@@ -1062,12 +1052,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         gf[r].template fetch<FIT>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
         RowFrags<T, DP> of;
         of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
-        float sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(static_cast<float>(gf[r].f[c][j]), static_cast<float>(of.f[c][j]), sum);
-        float delta = lanes_sum(sum);
+        float delta = row_delta_of<T, DP>(of, gf[r]);
         RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
         Under<T> under(stats.top, sl2);
         if (!real[r]) {  // a sum over rows must not see it
@@ -1122,7 +1107,6 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
             const int row = r * 16 + l % 16;  // its statistics from LDS: in registers they spilled others
             if (far) lower(s[r], m.off[row]);
             backward_scores(s[r], dp[r], sl2, m.base[row], m.delta[row]);
-            if (alone) dp[r][0] = dp[r][1] = f32x4(0.0f);
             into_unit<T>(dp[r], unit[r], dq[r]);
             ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
         }
@@ -1167,7 +1151,6 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 }
             }
             pf[t] = frag_of<T>(pr[0] * kProbabilityUnit<T>, pr[1] * kProbabilityUnit<T>);
-            if (alone) dr[0] = dr[1] = f32x4(0.0f);
             unit2[t] = kStartUnit<T>;
             into_unit<T>(dr, unit2[t], none);
             dsf[t] = frag_of<T>(dr[0], dr[1]);

@@ -127,13 +127,11 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
                 L.items.push_back({static_cast<int32_t>(qo[b]), static_cast<int32_t>(r), n,
                                    static_cast<int32_t>(ko[b] + p * s.size),
                                    static_cast<int32_t>(std::min(s.size, keys[b] - p * s.size)),
-                                   s.parts > 1 ? L.num_parts++ : -1, static_cast<int32_t>(ko[b]),
-                                   static_cast<int32_t>(keys[b])});
+                                   s.parts > 1 ? L.num_parts++ : -1, {}});
         }
         for (int64_t k = 0; rows[b] == 0 && k < keys[b]; k += kIdleKeys)
             L.idle.push_back({static_cast<int32_t>(qo[b]), 0, 0, static_cast<int32_t>(ko[b] + k),
-                              static_cast<int32_t>(std::min(kIdleKeys, keys[b] - k)), -1, static_cast<int32_t>(ko[b]),
-                              static_cast<int32_t>(keys[b])});
+                              static_cast<int32_t>(std::min(kIdleKeys, keys[b] - k)), -1, {}});
         const Split t = split(rows[b], row_share);
         for (int64_t k = 0; k < keys[b]; k += L.key_tile) {
             const int32_t n = static_cast<int32_t>(std::min<int64_t>(L.key_tile, keys[b] - k));
@@ -143,8 +141,7 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
             for (int64_t p = 0; p < t.parts; ++p)
                 L.key_items.push_back({static_cast<int32_t>(qo[b]), static_cast<int32_t>(p * t.size),
                                        static_cast<int32_t>(std::min(t.size, rows[b] - p * t.size)),
-                                       static_cast<int32_t>(ko[b] + k), n, t.parts > 1 ? L.num_key_parts++ : -1,
-                                       static_cast<int32_t>(ko[b]), static_cast<int32_t>(keys[b])});
+                                       static_cast<int32_t>(ko[b] + k), n, t.parts > 1 ? L.num_key_parts++ : -1, {}});
         }
     }
     deal(L.items, [](const AttnItem& i) { return i.keys; });

@@ -1,5 +1,5 @@
 """GPU tests of ``mp.cross_attention`` where its numbers run out: probabilities that a 16-bit type cannot hold,
-scores of any size.
+scores of any size, softmaxes of one key, gradients that are no numbers.
 
 Scores are made exact here (one value of a query, a power of two, meets one value of a key), so a probability errs by
 its own roundings only: at most 16 units of 2^-24 and one for each unit of the score's distance from the row's maximum,
@@ -186,3 +186,65 @@ def test_scores_past_the_floats_units(queries, dim, keys, dtype) -> None:
             rest = torch.ones(keys, dtype=torch.bool, device=DEV)
             rest[top] = False
             assert float(dv[rest].abs().sum()) == 0 and float(dk[rest].abs().sum()) == 0
+
+
+ONE_KEY = [([2, 1], 7), ([20, 3], 33), ([60, 33], 64), ([200, 130], 128)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,dim", ONE_KEY)
+@pytest.mark.parametrize("keys", [1, 100, 129, 200, 5_000, 20_011])
+def test_one_kept_key_among_any_number(queries, dim, keys, dtype) -> None:
+    """A softmax over one kept key is 1 and its gradient nothing, however many keys are left out around it."""
+    from relmo_amd import mp
+
+    lengths = [keys, 3]
+    q, k, v, grad, _ = _make(queries, lengths, 2, 1, dim, dtype, seed=dim + keys)
+    mask = torch.zeros(sum(lengths), dtype=torch.bool, device=DEV)
+    mask[keys // 2] = mask[keys + 1] = True
+    plan = mp.attention_plan(_offsets(queries), _offsets(lengths), 2, 1)
+    out, dq, dk, dv = _run(q, k, v, grad, plan, mask)
+    assert torch.equal(out[:queries[0]], v[keys // 2].expand(queries[0], 2, dim))
+    assert float(dq.abs().sum()) == 0 and float(dk.abs().sum()) == 0
+    val, tol = _definition(q, k, v, grad, mask, queries, lengths, dim ** -0.5)
+    _check((out, dq, dk, dv), val, tol, 2.0 ** -24 if dtype == torch.float16 else 1e-30)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,dim", ONE_KEY)
+@pytest.mark.parametrize("keys", [1, 100, 5_000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_gradients_that_are_no_numbers_show_through_one_kept_key(queries, dim, keys, dtype, bad) -> None:
+    from relmo_amd import mp
+
+    lengths = [keys, 3]
+    q, k, v, grad, _ = _make(queries, lengths, 2, 1, dim, dtype, seed=dim + keys)
+    mask = torch.zeros(sum(lengths), dtype=torch.bool, device=DEV)
+    mask[keys // 2] = mask[keys + 1] = True
+    grad[1, 1, dim // 2] = bad
+    plan = mp.attention_plan(_offsets(queries), _offsets(lengths), 2, 1)
+    _out, dq, dk, dv = _run(q, k, v, grad, plan, mask)
+    assert bool(dq[1, 1].isnan().all()) and bool(dk[keys // 2].isnan().all())
+    assert not bool(dv[keys // 2, 0, dim // 2].isfinite())
+    dq[1, 1] = 0
+    assert float(dq.abs().sum()) == 0 and float(dk[~mask].abs().sum()) == 0 and float(dv[~mask].abs().sum()) == 0
+    assert float(dk[keys + 1].abs().sum()) == 0 and bool(dv[keys + 1].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,dim", ROWS)
+@pytest.mark.parametrize("size", [2.0 ** 5, 2.0 ** 11, 2.0 ** 20, 2.0 ** 34])
+def test_a_dominant_key_leaves_no_gradient_of_the_scores(queries, dim, size, dtype) -> None:
+    """All but one key lie far below: their probabilities are 0 in float, as if they were left out."""
+    from relmo_amd import mp
+
+    keys = 300
+    g = _gen(7)
+    plan = mp.attention_plan(_offsets([queries]), _offsets([keys]), 1)
+    q, k = torch.zeros(queries, 1, dim, device=DEV), torch.zeros(keys, 1, dim, device=DEV)
+    q[:, 0, 0], k[:, 0, 0], k[211, 0, 0] = 8.0, -64.0, size / 8 if size < 2.0 ** 16 else 2.0 ** 13
+    v, grad = torch.randn(keys, 1, dim, device=DEV, generator=g), torch.randn(queries, 1, dim, device=DEV, generator=g)
+    scale = 1.3 if size < 2.0 ** 16 else 1.3 * size / 2.0 ** 16
+    out, dq, dk, dv = _run(q.to(dtype), k.to(dtype), v.to(dtype), grad.to(dtype), plan, None, scale=scale)
+    assert torch.equal(out, v[211:212].to(dtype).expand_as(out))
+    assert float(dq.abs().sum()) == 0 and float(dk.abs().sum()) == 0
