@@ -633,6 +633,16 @@ __device__ __forceinline__ float row_delta_of(const RowFrags<T, DP>& out, const 
     return __shfl(mine, (row / 4) * 16 + row);
 }
 
+// Rows past an item's end are zeros in a tile, and 0 against a key that holds an infinity is NaN:
+// entries from `rows` on of a lane's four leave their sums.
+__device__ __forceinline__ void clear_rows(f32x4& p, f32x4& ds, int rows) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        p[i] = i < rows ? p[i] : 0.0f;
+        ds[i] = i < rows ? ds[i] : 0.0f;
+    }
+}
+
 // Half values lose bits below 2^-14, where ds of keys with small probabilities lies.  A lane
 // holds ds of one query (key) and the sum over keys (queries) that it enters: both are kept
 // in units of a power of two, which falls as the largest ds seen so far rises (like the
@@ -862,11 +872,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         under_in = Under<T>(stats.top, sl2);
         share_in = stats.inv_total;
         delta_in = a.delta[p.row * a.heads + p.head];
-        if (row >= left) {  // probability 0
-            under_in.base = kInf;
-            under_in.off = 0.0f;
-            share_in = 0.0f;
-        }
     };
     if (w.it.rows > 0) fetch(0);
     for (int r0 = 0; r0 < w.it.rows; r0 += BR) {
@@ -928,6 +933,10 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
                         s[t][h][i] = p;
                         dp[t][h][i] = p * (dp[t][h][i] - delta[i]);
                     }
+                }
+                if (left < c * 32 + 32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) clear_rows(s[t][h], dp[t][h], left - (c * 32 + h * 16 + g * 4));
                 }
                 pf[t] = frag_of<T>(s[t][0] * kProbabilityUnit<T>, s[t][1] * kProbabilityUnit<T>);
                 into_unit<T>(dp[t], unit[t], dk[t]);
@@ -1052,14 +1061,10 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         gf[r].template fetch<FIT>(a.grad.data + at[r].row * a.grad.row_stride + at[r].head * a.grad.head_stride, a.dim);
         RowFrags<T, DP> of;
         of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
-        float delta = row_delta_of<T, DP>(of, gf[r]);
-        RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
-        Under<T> under(stats.top, sl2);
+        const float delta = row_delta_of<T, DP>(of, gf[r]);
+        const RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
+        const Under<T> under(stats.top, sl2);
         if (!real[r]) {  // a sum over rows must not see it
-            under.base = kInf;
-            under.off = 0.0f;
-            stats.inv_total = 0.0f;
-            delta = 0.0f;
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) qf[r].f[c] = gf[r].f[c] = Frag<T>(static_cast<T>(0.0f));
         }
@@ -1149,6 +1154,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                     pr[r][i] = exp2_of(fmaf(s2[r][i], sl2, -row_base[i])) * row_share[i];
                     dr[r][i] = pr[r][i] * (dp2[r][i] - row_delta[i]);
                 }
+                if (w.it.rows < 16 * RT) clear_rows(pr[r], dr[r], w.it.rows - (r * 16 + g * 4));
             }
             pf[t] = frag_of<T>(pr[0] * kProbabilityUnit<T>, pr[1] * kProbabilityUnit<T>);
             unit2[t] = kStartUnit<T>;

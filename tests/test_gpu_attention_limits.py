@@ -1,5 +1,5 @@
 """GPU tests of ``mp.cross_attention`` where its numbers run out: probabilities that a 16-bit type cannot hold,
-scores of any size, softmaxes of one key, gradients that are no numbers.
+scores of any size, softmaxes of one key, infinities in keys and gradients.
 
 Scores are made exact here (one value of a query, a power of two, meets one value of a key), so a probability errs by
 its own roundings only: at most 16 units of 2^-24 and one for each unit of the score's distance from the row's maximum,
@@ -248,3 +248,46 @@ def test_a_dominant_key_leaves_no_gradient_of_the_scores(queries, dim, size, dty
     out, dq, dk, dv = _run(q.to(dtype), k.to(dtype), v.to(dtype), grad.to(dtype), plan, None, scale=scale)
     assert torch.equal(out, v[211:212].to(dtype).expand_as(out))
     assert float(dq.abs().sum()) == 0 and float(dk.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [[1, 2], [9, 1], [17, 30], [40, 33], [65, 1], [130, 250]])
+@pytest.mark.parametrize("dim", [20, 64, 128])
+def test_infinite_keys_that_no_query_attends_to(queries, dim, dtype) -> None:
+    """A kept key whose scores are all -inf has the probability 0: dk and dv of it are 0, whatever fills a tile's
+    rows past the graph's, and the other keys go on as if it were left out.  (dq is 0 times infinity, as by the formula.)"""
+    from relmo_amd import mp
+
+    keys = [70, 150]
+    q, k, v, grad, _ = _make(queries, keys, 1, 1, dim, dtype, seed=dim)
+    q[:, 0, 3] = q[:, 0, 3].abs() + 0.5
+    spoilt = torch.zeros(sum(keys), dtype=torch.bool, device=DEV)
+    spoilt[[11, 70, 219]] = True
+    val, tol = _definition(q, k, v, grad, ~spoilt, queries, keys, dim ** -0.5)
+    k[spoilt, 0, 3] = float("-inf")
+    plan = mp.attention_plan(_offsets(queries), _offsets(keys), 1)
+    out, dq, dk, dv = _run(q, k, v, grad, plan, None)
+    assert float(dk[spoilt].abs().sum()) == 0 and float(dv[spoilt].abs().sum()) == 0
+    assert bool(dq[:, 0, 3].isnan().all())
+    dq[:, 0, 3], val[1][:, 0, 3] = 0, 0
+    _check((out, dq, dk, dv), val, tol, 2.0 ** -24 if dtype == torch.float16 else 1e-30)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [[1, 2], [17, 30], [40, 33], [130, 250]])
+def test_infinite_values_leave_their_own_gradient_alone(queries, dtype) -> None:
+    """dv of a key is its probabilities' sum over the gradients, whatever the key's value is."""
+    from relmo_amd import mp
+
+    keys = [70, 150]
+    q, k, v, grad, _ = _make(queries, keys, 1, 1, 32, dtype, seed=5)
+    val, tol = _definition(q, k, v, grad, None, queries, keys, 32 ** -0.5)
+    v = v.clone()
+    v[11, 0, 3] = float("inf")
+    plan = mp.attention_plan(_offsets(queries), _offsets(keys), 1)
+    _out, dq, dk, dv = _run(q, k, v, grad, plan, None)
+    for at, g in ((1, dq), (2, dk)):  # the other graph's are as they were
+        rows = queries[0] if at == 1 else keys[0]
+        over = (g[rows:].double() - val[at][rows:]).abs() - tol[at][rows:] - 2.0 ** -24
+        assert bool((over <= 0).all())
+    assert bool(((dv.double() - val[3]).abs() <= tol[3] + 2.0 ** -24).all())
