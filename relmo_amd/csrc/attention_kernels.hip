@@ -294,10 +294,14 @@ constexpr float kProbabilityUnit = std::is_same_v<T, f16> ? 32768.0f : 1.0f;
 // The exponent of a score s under its row's maximum m, sl2 (s - m).  As fma(s, sl2, -(sl2 m)) it is
 // one instruction, and off by the rounding of sl2 m: nothing of a row's own distribution is
 // lost, but the largest probability is not 1, and from 2^30 on that rounding passes the
-// exponent's range (below the largest float everything was infinite, or 0).  Rows past
-// kFarScore take the difference first, which is exact near the maximum: `off` is then m and
-// `base` 0.  Float rows always do (2^-24 is their own accuracy, and matrix instructions bound
-// them); 16-bit ones have 2^-17 up to there, a thirtieth of a half's unit.
+// exponent's range (below the largest float everything was infinite, or 0).
+//
+// Forward: rows past kFarScore take the difference first, which is exact near the maximum: `off`
+// is then m and `base` 0.  Float rows always do (2^-24 is their own accuracy, and matrix
+// instructions bound them); 16-bit ones have 2^-17 up to there, a thirtieth of a half's unit.
+// The branch that this takes stands behind the tile's maximum, which has read the scores.  One
+// between a matrix instruction and the first use of its result would be wrong: this compiler
+// leaves out the wait that such a use needs behind a taken branch.
 constexpr float kFarScore = 256.0f;
 
 template <typename T>
@@ -318,6 +322,28 @@ __device__ __forceinline__ void lower(f32x4 (&s)[N], float off) {
 #pragma unroll
     for (int t = 0; t < N; ++t) s[t] -= off;
 }
+
+// Backward: the row's statistics are known, so the rounding of its base is too, and goes into the
+// factor that divides by the total: p = 2^(slope s - base) * share, without a branch.  Past
+// kLastScore scores that are not equal lie 64 and more apart in units of the exponent, so
+// only equal ones share the row: there the slope is a power of two, exact on all of them.
+constexpr float kLastScore = 1073741824.0f;  // 2^30
+
+struct RowScore {
+    float slope, base, share;
+    __device__ __forceinline__ RowScore() = default;
+    __device__ __forceinline__ RowScore(RowStats r, float sl2) {
+        slope = sl2;
+        base = r.top * sl2;
+        share = r.inv_total * exp2_of(-fmaf(r.top, sl2, -base));
+        if (!(fabsf(base) < kLastScore)) {
+            const int e = static_cast<int>(__float_as_uint(r.top) >> 23 & 255);  // top * slope in [2^30, 2^31)
+            slope = __uint_as_float(static_cast<unsigned>(min(max(284 - e, 1), 254)) << 23);
+            base = r.top * slope;
+            share = r.inv_total;
+        }
+    }
+};
 
 // Two waves to a SIMD with 16-bit values: one's matrix instructions run beside the other's
 // exponentials.  Float rows need the registers of both.
@@ -371,7 +397,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
     f32x4 o[RT][ND];
     float m[RT], total[RT];
     Under<T> under[RT];
-    bool far = false;  // whether some row of the wave is
+    bool far = sizeof(T) == 4;  // whether some row of the wave is
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         m[r] = -kInf;
@@ -609,13 +635,13 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
 
 // The probabilities of the backward are the forward's: 2^(sl2 (s - top)) / total with the row's
 // maximum and total as they were (the logarithm of the total would enter the exponent
-// rounded at its own size).  dp of a query's keys becomes ds times the query's total, by which
-// dq is divided at the end.
-__device__ __forceinline__ void backward_scores(const f32x4 (&s)[2], f32x4 (&dp)[2], float sl2, float base, float delta) {
+// rounded at its own size).  dp of a query's keys becomes ds but for the query's share, which
+// dq takes at the end.
+__device__ __forceinline__ void backward_scores(const f32x4 (&s)[2], f32x4 (&dp)[2], float slope, float base, float delta) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dp[t][i] = exp2_of(fmaf(s[t][i], sl2, -base)) * (dp[t][i] - delta);
+        for (int i = 0; i < 4; ++i) dp[t][i] = exp2_of(fmaf(s[t][i], slope, -base)) * (dp[t][i] - delta);
 }
 
 // <grad, out> of a wave's 16 rows, each in the four lanes that share its row: the diagonal of a
@@ -697,9 +723,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
     RowFrags<T, DP> qf[RT], gf[RT];
     Place at[RT];
     bool real[RT];
-    Under<T> under[RT];
-    float share[RT], delta[RT], unit[RT];
-    bool far = false;
+    RowScore score[RT];
+    float delta[RT], unit[RT];
     f32x4 dq[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -711,10 +736,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         RowFrags<T, DP> of;
         of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
         delta[r] = row_delta_of<T, DP>(of, gf[r]);
-        const RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
-        under[r] = Under<T>(stats.top, sl2);
-        far = far || __any(under[r].far());
-        share[r] = stats.inv_total;
+        score[r] = RowScore(a.stats[at[r].row * a.heads + at[r].head], sl2);
         unit[r] = kStartUnit<T>;
         if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
 #pragma unroll
@@ -754,8 +776,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
             Frag<T> ds[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                if (far) lower(s[r], under[r].off);
-                backward_scores(s[r], dp[r], sl2, under[r].base, delta[r]);
+                backward_scores(s[r], dp[r], score[r].slope, score[r].base, delta[r]);
                 into_unit<T>(dp[r], unit[r], dq[r]);
                 ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
             }
@@ -771,7 +792,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int n = 0; n < ND; ++n) dq[r][n] = any ? dq[r][n] * (share[r] / unit[r]) : f32x4(0.0f);
+        for (int n = 0; n < ND; ++n) dq[r][n] = any ? dq[r][n] * (score[r].share / unit[r]) : f32x4(0.0f);
     const auto finish = [&](int row, Place p, int col, f32x4 sum) {
         if (w.it.part < 0) {
             put4<T>(a.dq + (p.row * a.heads + p.head) * a.dim, col, a.dim, sum * a.scale);
@@ -817,7 +838,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
     __shared__ __align__(16) T qt[BR * ST];
     __shared__ __align__(16) T gt[BR * ST];
     __shared__ __align__(16) float row_base[BR];
-    __shared__ __align__(16) float row_off[BR];
+    __shared__ __align__(16) float row_slope[BR];
     __shared__ __align__(16) float row_share[BR];
     __shared__ __align__(16) float row_delta[BR];
     // an item's keys are taken by key_tile / (64 KT) workgroups
@@ -852,9 +873,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
     }
 
     TileLoad<T, DP, BR> ql, gl;
-    Under<T> under_in;
-    float share_in = 0.0f, delta_in = 0.0f;
-    static_assert(BR == kWave, "a wave's lanes hold the statistics of a tile's rows");
+    RowScore score_in;
+    float delta_in = 0.0f;
     const auto fetch = [&](int r0) {
         const int left = w.it.rows - r0;
         const auto place = [&](int row) { return place_of(a, w.it.q_first, head, w.it.row0 + r0 + min(row, left - 1)); };
@@ -868,9 +888,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         }, a.dim);
         const int row = static_cast<int>(threadIdx.x) % BR;
         const Place p = place(row);
-        const RowStats stats = a.stats[p.row * a.heads + p.head];
-        under_in = Under<T>(stats.top, sl2);
-        share_in = stats.inv_total;
+        score_in = RowScore(a.stats[p.row * a.heads + p.head], sl2);
         delta_in = a.delta[p.row * a.heads + p.head];
     };
     if (w.it.rows > 0) fetch(0);
@@ -880,12 +898,11 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
         ql.template store<FIT>(qt, a.dim, left >= BR, [&](int row) { return row < left; });
         gl.template store<FIT>(gt, a.dim, left >= BR, [&](int row) { return row < left; });
         if (threadIdx.x < BR) {
-            row_base[threadIdx.x] = under_in.base;
-            row_off[threadIdx.x] = under_in.off;
-            row_share[threadIdx.x] = share_in;
+            row_slope[threadIdx.x] = score_in.slope;
+            row_base[threadIdx.x] = score_in.base;
+            row_share[threadIdx.x] = score_in.share;
             row_delta[threadIdx.x] = delta_in;
         }
-        const bool far = __any(under_in.far());  // a wave's lanes hold all rows of the tile
         __syncthreads();
         if (left > BR) fetch(r0 + BR);
 #pragma unroll
@@ -911,25 +928,18 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Ar
                     }
                 }
             }
-            if (far) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x4 off = *reinterpret_cast<const f32x4*>(row_off + c * 32 + h * 16 + g * 4);
-#pragma unroll
-                    for (int t = 0; t < KT; ++t) s[t][h] -= off;
-                }
-            }
             Frag<T> pf[KT], dsf[KT];
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    const f32x4 slope = *reinterpret_cast<const f32x4*>(row_slope + c * 32 + h * 16 + g * 4);
                     const f32x4 base = *reinterpret_cast<const f32x4*>(row_base + c * 32 + h * 16 + g * 4);
                     const f32x4 share = *reinterpret_cast<const f32x4*>(row_share + c * 32 + h * 16 + g * 4);
                     const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + c * 32 + h * 16 + g * 4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = exp2_of(fmaf(s[t][h][i], sl2, -base[i])) * share[i];
+                        const float p = exp2_of(fmaf(s[t][h][i], slope[i], -base[i])) * share[i];
                         s[t][h][i] = p;
                         dp[t][h][i] = p * (dp[t][h][i] - delta[i]);
                     }
@@ -1020,8 +1030,8 @@ struct FewRows {
     __align__(16) T q[kRows * kStride];
     __align__(16) T g[kRows * kStride];
     __align__(16) float starts[kKeys];
+    __align__(16) float slope[32];
     __align__(16) float base[32];
-    __align__(16) float off[32];
     __align__(16) float share[32];
     __align__(16) float delta[32];
 };
@@ -1050,7 +1060,6 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
     Place at[RT];
     bool real[RT];
     float unit[RT];
-    bool far = false;
     f32x4 dq[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -1062,13 +1071,11 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         RowFrags<T, DP> of;
         of.template fetch<FIT>(a.out + (at[r].row * a.heads + at[r].head) * a.dim, a.dim);
         const float delta = row_delta_of<T, DP>(of, gf[r]);
-        const RowStats stats = a.stats[at[r].row * a.heads + at[r].head];
-        const Under<T> under(stats.top, sl2);
+        const RowScore score(a.stats[at[r].row * a.heads + at[r].head], sl2);
         if (!real[r]) {  // a sum over rows must not see it
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) qf[r].f[c] = gf[r].f[c] = Frag<T>(static_cast<T>(0.0f));
         }
-        far = far || __any(under.far());
         unit[r] = kStartUnit<T>;
 #pragma unroll
         for (int n = 0; n < ND; ++n) dq[r][n] = f32x4(0.0f);
@@ -1079,9 +1086,9 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
                 lds_put<T>(m.g + row * ST + c * 32 + g * 8, gf[r].f[c]);
             }
             if (g == 0) {
-                m.base[row] = under.base;
-                m.off[row] = under.off;
-                m.share[row] = stats.inv_total;
+                m.slope[row] = score.slope;
+                m.base[row] = score.base;
+                m.share[row] = score.share;
                 m.delta[row] = delta;
             }
         }
@@ -1110,8 +1117,7 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = r * 16 + l % 16;  // its statistics from LDS: in registers they spilled others
-            if (far) lower(s[r], m.off[row]);
-            backward_scores(s[r], dp[r], sl2, m.base[row], m.delta[row]);
+            backward_scores(s[r], dp[r], m.slope[row], m.base[row], m.delta[row]);
             into_unit<T>(dp[r], unit[r], dq[r]);
             ds[r] = frag_of<T>(dp[r][0], dp[r][1]);
         }
@@ -1145,13 +1151,13 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
             f32x4 pr[2] = {f32x4(0.0f), f32x4(0.0f)}, dr[2] = {f32x4(0.0f), f32x4(0.0f)}, none[1] = {f32x4(0.0f)};
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
+                const f32x4 row_slope = *reinterpret_cast<const f32x4*>(m.slope + r * 16 + g * 4);
                 const f32x4 row_base = *reinterpret_cast<const f32x4*>(m.base + r * 16 + g * 4);
                 const f32x4 row_share = *reinterpret_cast<const f32x4*>(m.share + r * 16 + g * 4);
                 const f32x4 row_delta = *reinterpret_cast<const f32x4*>(m.delta + r * 16 + g * 4);
-                if (far) s2[r] -= *reinterpret_cast<const f32x4*>(m.off + r * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    pr[r][i] = exp2_of(fmaf(s2[r][i], sl2, -row_base[i])) * row_share[i];
+                    pr[r][i] = exp2_of(fmaf(s2[r][i], row_slope[i], -row_base[i])) * row_share[i];
                     dr[r][i] = pr[r][i] * (dp2[r][i] - row_delta[i]);
                 }
                 if (w.it.rows < 16 * RT) clear_rows(pr[r], dr[r], w.it.rows - (r * 16 + g * 4));
