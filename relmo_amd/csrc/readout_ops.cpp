@@ -460,7 +460,7 @@ std::vector<Tensor> orthogonalise(at::TensorList updates, int64_t steps, at::Arr
     const int32_t count = static_cast<int32_t>(mats.size());
     const size_t need = relm_mp_orthogonalise_workspace_size(mats.data(), count);
     const Tensor ws = need > 0 ? bytes(need, updates[0]) : Tensor();
-    raise_if(relm_mp_orthogonalise(dtype, mats.data(), count, static_cast<int32_t>(std::min<int64_t>(steps, 1 << 30)),
+    raise_if(relm_mp_orthogonalise(dtype, mats.data(), count, static_cast<int32_t>(std::clamp<int64_t>(steps, -1, 1 << 30)),
                                    static_cast<float>(coefficients[0]), static_cast<float>(coefficients[1]),
                                    static_cast<float>(coefficients[2]), static_cast<float>(eps),
                                    need > 0 ? ws.data_ptr() : nullptr, need, current_stream(updates[0])));

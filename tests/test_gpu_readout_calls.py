@@ -57,3 +57,11 @@ def test_forward_mode_over_the_backward_is_refused() -> None:
             with pytest.raises(RuntimeError, match="forward"):
                 torch.autograd.grad(out, x, grad, retain_graph=True)
         torch.autograd.grad(out, x, torch.ones_like(out))
+
+
+def test_steps_past_32_bits_are_refused() -> None:
+    from relmo_amd import mp
+
+    for steps in (5 - (1 << 32), 5 + (1 << 32), -(1 << 62)):
+        with pytest.raises(RuntimeError, match="steps"):
+            mp.orthogonalise(torch.ones(4, 8, device=DEV), steps=steps)
