@@ -13,6 +13,8 @@ from .mp_dispatch import library_op
 from .mp_runtime import torch
 
 FP8_MAX = 448.0
+FLOAT_MAX = 3.4028234663852886e38  # the library's constants are float32
+ORTHO_STEPS = 64
 
 
 def _wants_grad(*tensors) -> bool:
@@ -22,7 +24,12 @@ def _wants_grad(*tensors) -> bool:
 # ---- residual norm ---------------------------------------------------------------
 
 
-def _norm_checks(op_name: str, x, residual, weight) -> None:
+def _eps_check(op_name: str, eps: float) -> None:
+    if not 0.0 <= eps <= FLOAT_MAX:
+        raise RuntimeError(f"{op_name}: eps must be finite and not negative.")
+
+
+def _norm_checks(op_name: str, x, residual, weight, eps: float) -> None:
     if x.dim() < 1 or weight.dim() != 1 or weight.size(0) != x.size(-1):
         raise ValueError(f"{op_name} expects x [..., width] and weight [width].")
     if residual is not None and residual.shape != x.shape:
@@ -30,6 +37,7 @@ def _norm_checks(op_name: str, x, residual, weight) -> None:
     for name, t in (("residual", residual), ("weight", weight)):
         if t is not None and (t.dtype != x.dtype or t.device != x.device):
             raise ValueError(f"{op_name} expects {name} to have the dtype and device of x.")
+    _eps_check(op_name, eps)
 
 
 def _norm_float(x, residual, weight, eps: float):
@@ -46,7 +54,7 @@ def add_rms_norm(x, residual, weight, eps: float):
     op = library_op("add_rms_norm", tensor=x, gpu_only=True)
     if op is not None:
         return op(x, residual, weight, eps)
-    _norm_checks("add_rms_norm", x, residual, weight)
+    _norm_checks("add_rms_norm", x, residual, weight, eps)
     y, h = _norm_float(x, residual, weight, eps)
     return y.to(x.dtype), h.to(x.dtype)
 
@@ -55,7 +63,7 @@ def rms_norm(x, weight, eps: float):
     op = library_op("rms_norm", tensor=x, gpu_only=True)
     if op is not None:
         return op(x, weight, eps)
-    _norm_checks("rms_norm", x, None, weight)
+    _norm_checks("rms_norm", x, None, weight, eps)
     return _norm_float(x, None, weight, eps)[0].to(x.dtype)
 
 
@@ -66,7 +74,7 @@ def add_rms_norm_fp8(x, residual, weight, eps: float):
     if op is not None:
         q, scale, h = op(x, residual, weight, eps)
         return q, scale, x if residual is None else h
-    _norm_checks("add_rms_norm_fp8", x, residual, weight)
+    _norm_checks("add_rms_norm_fp8", x, residual, weight, eps)
     y, h = _norm_float(x, residual, weight, eps)
     scale = (y.abs().amax(-1) if x.size(-1) else y.new_zeros(x.shape[:-1])) / FP8_MAX
     scale = torch.where(scale == 0, torch.ones_like(scale), scale).to(torch.float32)
@@ -162,6 +170,23 @@ def cross_attention(q, k, v, plan, key_mask, scale: float | None):
 # ---- orthogonalised update ---------------------------------------------------------
 
 
+def _orthogonalise_checks(steps: int, coefficients, eps: float) -> None:
+    """What the library refuses: among it polynomials that take values of [0, 1] past 2, on the same grid of them."""
+
+    if not 1 <= steps <= ORTHO_STEPS:
+        raise RuntimeError(f"orthogonalise: steps must be in [1, {ORTHO_STEPS}].")
+    _eps_check("orthogonalise", eps)
+    a, b, c = coefficients
+    x = torch.linspace(0.0, 1.0, 1025, dtype=torch.float64)
+    within = torch.ones((), dtype=torch.bool)
+    for _ in range(steps):
+        square = x.square()
+        x = (a + b * square + c * square.square()) * x
+        within = within & (x.abs() <= 2.0).all()
+    if not bool(within):
+        raise RuntimeError("orthogonalise: these coefficients take singular values past 2.")
+
+
 def _orthogonalise_float(update, steps: int, coefficients, eps: float):
     a, b, c = coefficients
     x = update.to(torch.promote_types(update.dtype, torch.float32))
@@ -190,6 +215,8 @@ def orthogonalise(updates, steps: int, coefficients, eps: float):
         if op is not None:
             results = op(parts, int(steps), coefficients, float(eps))
         else:
+            if parts:
+                _orthogonalise_checks(int(steps), coefficients, eps)
             results = [_orthogonalise_float(u, int(steps), coefficients, eps) for u in parts]
     return results[0] if one else results
 

@@ -126,6 +126,22 @@ def test_argument_checks() -> None:
         mp.orthogonalise([x[0], x[0].double()])
 
 
+def test_cpu_tensors_are_refused_what_gpu_tensors_are() -> None:
+    x, w = torch.ones(4, 8), torch.ones(8)
+    for eps in (-1.0, float("nan"), float("inf")):
+        for call in (lambda: mp.rms_norm(x, w, eps=eps), lambda: mp.add_rms_norm(x, x, w, eps=eps),
+                     lambda: mp.add_rms_norm_fp8(x, x, w, eps=eps), lambda: mp.orthogonalise(x, eps=eps)):
+            with pytest.raises(RuntimeError, match="eps"):
+                call()
+    for steps in (0, -1, 65, 1 << 40, 5 - (1 << 32)):
+        with pytest.raises(RuntimeError, match="steps"):
+            mp.orthogonalise(x, steps=steps)
+    for coefficients in ((4.0, 0.0, 0.0), (float("nan"), 0.0, 0.0), (1.0, float("inf"), 0.0)):
+        with pytest.raises(RuntimeError, match="past 2"):
+            mp.orthogonalise(x, coefficients=coefficients)
+    assert mp.orthogonalise([], steps=0) == []
+
+
 # ---- the attention's plan ---------------------------------------------------------------------
 
 
