@@ -56,7 +56,8 @@ class ObjectReadout(nn.Module):
         r = self.query.repeat(graphs, 1)
         q = self.to_q(mp.rms_norm(self.query, self.query_norm)).repeat(graphs, 1).view(-1, self.heads, self.dim)
         read = mp.cross_attention(q, kv[:, 0], kv[:, 1], plan, key_mask=object_mask)
-        y, _h = mp.add_rms_norm(self.out(read.flatten(1)), r, self.out_norm)
+        # under autocast the projections are 16-bit; the residual stream stays in its parameters' type
+        y, _h = mp.add_rms_norm(self.out(read.flatten(1)).to(r.dtype), r, self.out_norm)
         return self.value(y).view(graphs, self.queries)
 
 

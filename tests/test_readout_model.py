@@ -54,6 +54,39 @@ def test_readout_ignores_masked_objects_and_empty_graphs() -> None:
     assert values.shape == (3, 2)
 
 
+def _autocast_step(device):
+    """Values and gradients of a float32 readout, plain and under autocast to bfloat16."""
+
+    torch.manual_seed(2)
+    readout = ObjectReadout(32, heads=4, kv_heads=2, queries=3).to(device)
+    x = torch.randn(20, 32, generator=torch.Generator().manual_seed(3)).to(device)
+    plan = readout.plan(torch.tensor([0, 7, 7, 20], device=device))
+    results = []
+    for enabled in (False, True):
+        states = x.clone().requires_grad_()
+        with torch.autocast(device, dtype=torch.bfloat16, enabled=enabled):
+            values = readout(states, plan)
+        grads = torch.autograd.grad(values.float().square().sum(), (states, *readout.parameters()))
+        results.append((values.detach(), grads))
+    (want, want_grads), (got, grads) = results
+    assert got.isfinite().all() and [g.dtype for g in grads] == [g.dtype for g in want_grads]
+    # a few roundings of 2^-8 on a path of sums of 32 terms
+    assert float((got.float() - want).abs().max()) <= 0.1 * float(want.abs().max()) + 0.02
+    for a, b in zip(grads, want_grads):
+        assert float((a - b).norm()) <= 0.15 * float(b.norm()) + 1e-3
+
+
+def test_autocast_on_the_cpu() -> None:
+    _autocast_step("cpu")
+
+
+@pytest.mark.gpu
+def test_autocast_on_the_gpu() -> None:
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU visible")
+    _autocast_step("cuda")
+
+
 @pytest.mark.gpu
 def test_training_on_the_gpu_follows_the_64_bit_steps() -> None:
     """The same steps in float32 on the GPU and in float64 on the CPU: equal losses up to what float32 gradients and
