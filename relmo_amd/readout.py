@@ -94,7 +94,7 @@ class Muon(torch.optim.Optimizer):
                 torch._foreach_add_(momenta, grads)
                 updates = torch._foreach_add(grads, momenta, alpha=group["momentum"])
                 results = mp.orthogonalise(updates, steps=group["steps"])
-                rates = [-group["lr"] * max(1.0, p.size(0) / p.size(1)) ** 0.5 for p in params]
+                rates = [-group["lr"] * max(1.0, p.size(0) / max(1, p.size(1))) ** 0.5 for p in params]
                 torch._foreach_mul_(results, rates)
                 torch._foreach_add_(params, results)
         return loss

@@ -42,6 +42,20 @@ def test_muon_takes_matrices_only() -> None:
         Muon([torch.nn.Parameter(torch.zeros(3))])
 
 
+def test_muon_steps_past_empty_matrices() -> None:
+    """A relation without features: nothing to step, and the others are stepped as without it."""
+
+    def params():
+        return [torch.nn.Parameter(torch.ones(*s)) for s in ((3, 0), (0, 4), (4, 3))]
+
+    some, alone = params(), params()[2:]
+    for group in (some, alone):
+        for p in group:
+            p.grad = torch.arange(float(p.numel())).view(p.shape) + 1.0
+        Muon(group).step()
+    assert torch.equal(some[2], alone[0]) and not torch.equal(some[2], torch.ones(4, 3))
+
+
 def test_readout_ignores_masked_objects_and_empty_graphs() -> None:
     torch.manual_seed(1)
     readout = ObjectReadout(8, heads=2, queries=2).double()
