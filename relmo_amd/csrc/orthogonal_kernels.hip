@@ -20,6 +20,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <vector>
 
@@ -686,12 +687,28 @@ void product(const OrthoBatch& b, const OrthoRule& rule, int count, int step, bo
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, st, b, rule, count, step, ws);
 }
 
+// Sets the kernel's LDS limit on the current device, if that has not been done there.
+template <typename T>
+hipError_t allow_small_lds() {
+    constexpr int kDevices = 64;
+    static std::atomic<bool> done[kDevices];
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    const bool known = device >= 0 && device < kDevices;
+    if (known && done[device].load(std::memory_order_acquire)) return hipSuccess;
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_ortho_small<T>), hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds);
+    if (e == hipSuccess && known) done[device].store(true, std::memory_order_release);
+    return e;
+}
+
 template <typename T>
 hipError_t run(const std::vector<OrthoMatrix>& small, const std::vector<OrthoMatrix>& large, const OrthoRule& rule, void* ws,
                hipStream_t st) {
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(k_ortho_small<T>),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds);
-    if (!small.empty() && allowed != hipSuccess) return allowed;
+    if (!small.empty()) {
+        const hipError_t e = allow_small_lds<T>();
+        if (e != hipSuccess) return e;
+    }
     for (size_t i = 0; i < small.size(); i += kOrthoBatch) {
         OrthoBatch b{};
         const size_t count = std::min<size_t>(kOrthoBatch, small.size() - i);
