@@ -637,11 +637,32 @@ __global__ __launch_bounds__(kThreads) void k_attention_join(Args<T> a) {
 // maximum and total as they were (the logarithm of the total would enter the exponent
 // rounded at its own size).  dp of a query's keys becomes ds but for the query's share, which
 // dq takes at the end.
+//
+// delta comes from the output as it was stored.  With few keys ds is a small difference, and the
+// rounding of a 16-bit output made dq and dk err 2.2 times as much (two keys; 1.6 with nine, nothing
+// to speak of from 32 on).  Where all keys of a graph are these 32, what a row's ds add up to, which
+// should be nothing, shows that rounding: row_rest is added to delta before the walk.
 __device__ __forceinline__ void backward_scores(const f32x4 (&s)[2], f32x4 (&dp)[2], float slope, float base, float delta) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) dp[t][i] = exp2_of(fmaf(s[t][i], slope, -base)) * (dp[t][i] - delta);
+}
+
+__device__ __forceinline__ float row_rest(const f32x4 (&s)[2], f32x4 (&dp)[2], float slope, float base, float share, float delta) {
+    backward_scores(s, dp, slope, base, delta);
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += dp[t][i];
+    return lanes_sum(sum) * share;
+}
+
+// Whether an item's keys are its graph's and one wave's 32, and their outputs rounded.
+template <typename T>
+__device__ __forceinline__ bool few_keys(const AttnItem& it) {
+    return sizeof(T) == 2 && it.part < 0 && it.keys > 0 && it.keys <= 32;
 }
 
 // <grad, out> of a wave's 16 rows, each in the four lanes that share its row: the diagonal of a
@@ -738,7 +759,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         delta[r] = row_delta_of<T, DP>(of, gf[r]);
         score[r] = RowScore(a.stats[at[r].row * a.heads + at[r].head], sl2);
         unit[r] = kStartUnit<T>;
-        if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
 #pragma unroll
         for (int n = 0; n < ND; ++n) dq[r][n] = f32x4(0.0f);
     }
@@ -754,8 +774,28 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
         vl.template fetch<FIT>([&](int row) { return vp + min(row, left - 1) * a.v.row_stride; }, a.dim);
         bits.fetch(a.key_mask, first, left);
     };
-    bool any = false;  // whether some key of the item is kept (the same for all waves)
     if (w.it.keys > 0) fetch(0);
+    if (few_keys<T>(w.it)) {
+        bits.settle();
+        kl.template store<FIT>(kt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        vl.template store<FIT>(vt, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        if (threadIdx.x < BN) starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
+        __syncthreads();
+        if (key_wave == 0) {  // the one that has the keys
+            const f32x4 zero[2] = {f32x4(0.0f), f32x4(0.0f)};
+            f32x4 start[2], s[RT][2], dp[RT][2];
+            key_starts(starts, 0, start);
+            keys_by_rows<T, DP, RT>(kt, 0, qf, start, s);
+            keys_by_rows<T, DP, RT>(vt, 0, gf, zero, dp);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                delta[r] += row_rest(s[r], dp[r], score[r].slope, score[r].base, score[r].share, delta[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+        if (real[r] && key_wave == 0 && g == 0) a.delta[at[r].row * a.heads + at[r].head] = delta[r];
+    bool any = false;  // whether some key of the item is kept (the same for all waves)
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();
         any = any || !bits.none();
@@ -1094,6 +1134,26 @@ __device__ __forceinline__ void few_rows_backward(const Args<T>& a, const Work& 
         }
     }
 
+    if (few_keys<T>(w.it)) {
+        bits.settle();
+        kl.template store<FIT>(m.k, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        vl.template store<FIT>(m.v, a.dim, bits.all(), [&](int row) { return bits.has(row); });
+        if (threadIdx.x < BN) m.starts[threadIdx.x] = bits.has(threadIdx.x) ? 0.0f : -kInf;
+        __syncthreads();
+        if (wave == 0) {  // the one that has the keys, and wrote the rows
+            const f32x4 zero[2] = {f32x4(0.0f), f32x4(0.0f)};
+            f32x4 start[2], s[RT][2], dp[RT][2];
+            key_starts(m.starts, 0, start);
+            keys_by_rows<T, DP, RT>(m.k, 0, qf, start, s);
+            keys_by_rows<T, DP, RT>(m.v, 0, gf, zero, dp);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const int row = r * 16 + l % 16;
+                const float rest = row_rest(s[r], dp[r], m.slope[row], m.base[row], m.share[row], m.delta[row]);
+                if (g == 0) m.delta[row] += rest;
+            }
+        }
+    }
     bool any = false;  // whether some key of the item is kept (the same for all waves)
     for (int k0 = 0; k0 < w.it.keys; k0 += BN) {
         bits.settle();

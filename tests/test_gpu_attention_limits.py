@@ -291,3 +291,22 @@ def test_infinite_values_leave_their_own_gradient_alone(queries, dtype) -> None:
         over = (g[rows:].double() - val[at][rows:]).abs() - tol[at][rows:] - 2.0 ** -24
         assert bool((over <= 0).all())
     assert bool(((dv.double() - val[3]).abs() <= tol[3] + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("graphs,queries,dim", [(300, 16, 64), (150, 30, 32), (80, 60, 64), (30, 200, 128)])
+@pytest.mark.parametrize("keys", [2, 3, 9])
+def test_few_keys_lose_no_more_than_two_roundings(graphs, queries, dim, keys, dtype) -> None:
+    """With few keys ds is the small difference of <grad, v> and delta.  dq and dk then err by two roundings to 16 bits of
+    the same size, ds and the result: 1.42 times one of them, and not by the output's on top (1.6 times with 4 keys, 2.2
+    with 2)."""
+    from relmo_amd import mp
+
+    lengths = [queries] * graphs, [keys] * graphs
+    q, k, v, grad, _ = _make(*lengths, 1, 1, dim, dtype, seed=keys)
+    plan = mp.attention_plan(_offsets(lengths[0]), _offsets(lengths[1]), 1)
+    got = _run(q, k, v, grad, plan, None)
+    val, _tol = _definition(q, k, v, grad, None, *lengths, dim ** -0.5)
+    for name, g, w in (("dq", got[1], val[1]), ("dk", got[2], val[2])):
+        once = float((w.to(dtype).double() - w).norm())
+        assert float((g.double() - w).norm()) <= 1.55 * once, (name, float((g.double() - w).norm()) / once)
