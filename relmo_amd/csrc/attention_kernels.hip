@@ -349,6 +349,10 @@ struct RowScore {
 // exponentials.  Float rows need the registers of both.
 template <typename T>
 constexpr int kWavesPerSimd = sizeof(T) == 2 ? 2 : 1;
+// Float rows of 32 values, one tile to a wave: LDS holds four workgroups, and so do registers
+// when asked to (of themselves they take 130, for three: 512 graphs of 8 x 200 in 16.1 us, not 14.8).
+template <typename T, int DP, int RT>
+constexpr int kForwardWaves = sizeof(T) == 4 && DP == 32 && RT == 1 ? 4 : kWavesPerSimd<T>;
 
 // Shapes of the row kernels: a wave has RT tiles of 16 rows; WM waves have rows of their
 // own and 4 / WM share each row tile, taking different keys of a tile.
@@ -369,7 +373,7 @@ struct RowShape {
 // precision, in 512 parts 31 us (4.3 TB/s); 2048 graphs of 64 to 512 keys, up to 32 queries,
 // 4 heads of 32 in bfloat16 92 us (3.5 TB/s).
 template <typename T, int DP, int RT, int WM, int FIT>
-__global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T> a) {
+__global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP, RT>)) void k_attention(Args<T> a) {
     using S = RowShape<RT, WM>;
     constexpr int BN = S::kKeys, ST = kLdsStride<T, DP>, ND = DP / 16;
     constexpr int kTileBytes = 2 * BN * ST * static_cast<int>(sizeof(T));
@@ -397,7 +401,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
     f32x4 o[RT][ND];
     float m[RT], total[RT];
     Under<T> under[RT];
-    bool far = sizeof(T) == 4;  // whether some row of the wave is
+    bool far = false;  // whether some row of the wave is
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         m[r] = -kInf;
@@ -453,12 +457,16 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
 #pragma unroll
                 for (int n = 0; n < ND; ++n) o[r][n] *= shrink;
                 m[r] = most;
-                under[r] = Under<T>(most, sl2);
-                far = far || __any(under[r].far());
+                if constexpr (sizeof(T) == 2) {
+                    under[r] = Under<T>(most, sl2);
+                    far = far || __any(under[r].far());
+                }
             }
-            if (far) {
+            // (of float rows from m: a register more to a row cost a wave to a SIMD)
+            const Under<T> now = sizeof(T) == 2 ? under[r] : Under<T>(m[r], sl2);
+            if (sizeof(T) == 4 || far) {
 #pragma unroll
-                for (int c = 0; c < S::kChunks; ++c) lower(s[c][r], under[r].off);
+                for (int c = 0; c < S::kChunks; ++c) lower(s[c][r], now.off);
             }
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c)
@@ -466,7 +474,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention(Args<T
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = exp2_of(fmaf(s[c][r][t][i], sl2, -under[r].base));
+                        const float p = exp2_of(fmaf(s[c][r][t][i], sl2, -now.base));
                         s[c][r][t][i] = p * kProbabilityUnit<T>;
                         total[r] += p;
                     }
