@@ -9,10 +9,12 @@
 // queries across): a lane then holds four neighbouring keys of one query, which is
 // what the next product wants as an operand, so probabilities go from one matrix
 // instruction to the next without leaving the lane, and a query's statistics are one
-// value per lane.  Scores, statistics, totals and all accumulators are float;
-// probabilities and ds are rounded to the values' type for the products that read
-// them (each such rounding is independent of the others and of the size of the
-// outputs' own; with float values nothing is rounded).
+// value per lane.  Scores, statistics, totals and all accumulators are float.
+// Probabilities and ds are rounded to the values' type for the products that read
+// them: each such rounding is independent of the others and of the size of the
+// outputs' own, so that an output errs by up to 1.5 times that one (two roundings in
+// the place of one; 16-bit products are nine times the float ones' rate).  With float
+// values nothing is rounded.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -368,10 +370,10 @@ struct RowShape {
 // when a key tile raises it, what has been added up is scaled by exp(m_old - m_new).
 // Long rows of work are bound by the exponentials and conversions beside the matrix
 // instructions: 4 x 2048 queries x 4096 keys,
-// 16 heads of 128 over 4 key heads, bfloat16, 335 us (820 TFLOP/s).  Few rows are bound by
+// 16 heads of 128 over 4 key heads, bfloat16, 338 us (815 TFLOP/s).  Few rows are bound by
 // the reads of keys and values: one query over 262,147 keys, 2 key heads of 64 in half
 // precision, in 512 parts 31 us (4.3 TB/s); 2048 graphs of 64 to 512 keys, up to 32 queries,
-// 4 heads of 32 in bfloat16 92 us (3.5 TB/s).
+// 4 heads of 32 in bfloat16 95 us (3.4 TB/s).
 template <typename T, int DP, int RT, int WM, int FIT>
 __global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP, RT>)) void k_attention(Args<T> a) {
     using S = RowShape<RT, WM>;
@@ -733,7 +735,7 @@ __device__ __forceinline__ void into_unit(f32x4 (&ds)[2], float& unit, f32x4 (&s
 // dq of a row item: like the forward, with the probabilities recomputed from its statistics.  A row's
 // delta is left for the key kernel (parts of one row leave the same).  Three products to the
 // forward's two, bound alike: 8 graphs of 500 to 1500 queries x 900 to 2100 keys, 8 heads
-// of 64 in bfloat16, 70 us (490 TFLOP/s).
+// of 64 in bfloat16, 73 us (470 TFLOP/s).
 template <typename T, int DP, int RT, int WM, int FIT>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Args<T> a) {
     using S = RowShape<RT, WM>;
@@ -879,7 +881,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dq(Arg
 // dk and dv of a key item: a wave keeps KT tiles of 16 keys and walks the graph's rows
 // (rows down, keys across, so that a lane's probabilities are the operand of the products
 // over rows).  Four products, bound by LDS reads (each of a wave's products reads its
-// operand for 16 KT keys) and the exponentials: the batch above 86 us (530 TFLOP/s).
+// operand for 16 KT keys) and the exponentials: the batch above 89 us (510 TFLOP/s).
 template <typename T, int DP, int KT, int FIT>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd<T>) void k_attention_dkv(Args<T> a) {
     constexpr int BR = 64, ST = kLdsStride<T, DP>, ND = DP / 16;
@@ -1066,8 +1068,8 @@ __global__ __launch_bounds__(kThreads) void k_attention_dkv_join(Args<T> a) {
 // scores are computed both ways, from the same fragments with the operands exchanged, and
 // their exponentials twice.  Bound by latency, then by the reads and writes
 // (keys, values and their gradients once each): 2048 graphs of 64 to 512 keys, up to 32
-// queries, 4 heads of 32 in bfloat16 192 us (291 before the items were dealt by length, then
-// 318 for the two kernels of longer rows).
+// queries, 4 heads of 32 in bfloat16 214 us (291 before the items were dealt by length, then
+// 318 for the two kernels of longer rows, when this one took 192).
 template <typename T, int DP>
 struct FewRows {
     static constexpr int kKeys = 128, kStride = kLdsStride<T, DP>;
@@ -1384,7 +1386,10 @@ void with_rows(int row_tile, F&& f) {
     }
 }
 
-// Rows of up to kFewParts parts on average are joined a thread group to a row.
+// Rows of up to kFewParts parts on average are joined a thread group to a row; with more, a
+// workgroup to a row.  4 heads of 64 in bfloat16, forward, us: 60 queries x 3000 keys in 6 parts
+// 17.0 and 15.8, x 5000 in 10 18.4 and 15.6; 128 x 9000 in 18 25.0 and 20.5; 500 x 9000 in 18 29.7 and
+// 28.1.  (At 5 to 6 parts the second form is already a microsecond faster.)
 constexpr int kFewParts = 8;
 
 template <typename T, int DP, bool DQ>

@@ -13,11 +13,18 @@ namespace relm_mp {
 namespace {
 
 // Workgroups of a launch at least, where the lengths allow: four to each of 256 CUs, two of
-// those that keep 64 or more rows (keys: 128) in registers.
+// those that keep 64 or more rows (keys: 128) in registers.  Measured, us: one query over
+// 2,000,000 keys, 8 / 2 heads of 64 in half precision, 270 at 256, 186 at 512, 208 at 1024, 200 at 2048
+// (262,147 keys: 38, 29, 37, 34: 512 would serve these two better); large ones, 4 x 2048 x 4096
+// with 4 heads of 128 in bfloat16, 153 at 256, 102 at 512, 113 at 1024, in training with heads of 64
+// 313, 228, 259.
 constexpr int64_t kWorkgroups = 1024;
 constexpr int64_t kLargeWorkgroups = 512;
 constexpr int64_t kPartUnit = 128;     // parts end on whole tiles of keys and rows
-constexpr int64_t kLeastKeys = 512;    // of a part: shorter ones cost more to join than to walk
+// Of a part: shorter ones cost more to join than to walk.  The query above over 32,000 keys: 11.9 us at
+// 128, 11.1 at 256, 13.8 at 512, 17.3 at 1024 (over 2000: 10.6, 10.9, 11.8, 16.4).
+constexpr int64_t kLeastKeys = 512;
+// The same for rows: 5003 queries over 40 keys in training take 70 to 71 us at 128 to 1024 and 142 at 4096.
 constexpr int64_t kLeastRows = 256;
 constexpr int64_t kIdleKeys = 1024;    // of an item of a graph without queries, whose keys get zeros: at most 1 MB of them
 
@@ -83,6 +90,13 @@ int lay_out(const int64_t* qo, const int64_t* ko, int64_t graphs, int64_t group,
     // Rows of an item.  Up to 32, its waves take different keys and a row's sums meet at
     // the end; from there on each wave has rows of its own, 16 or 32.  128 rows read a
     // key tile half as often as 64, unless the lengths leave a fifth more rows empty.
+    // Measured, us (this tile and the next larger one): 512 graphs of up to 16 x 200, 2 heads of 64, 14.9
+    // and 17.6 in bfloat16, 30 and 53 in float, in training 47 and 50, 121 and 144; up to 32 x 300, 4 heads
+    // of 64, 37 and 32, 151 and 116, in training 131 and 155, 481 and 543.  64 and 128 rows of 8 heads of 64
+    // over 1000 keys, bfloat16: of 65 rows 41 and 37, of 150 33 and 37, of 1000 25 and 30; float: 175 and
+    // 157, 125 and 152, 89 and 88; 4 x 2048 rows over 4096 keys, 16 / 4 heads of 128 in bfloat16, 437 and 338.
+    // Keys, in training: of 150 70 and 73 in bfloat16, 267 and 313 in float.  (One graph of more than 32
+    // rows moves a whole batch: 2048 graphs of up to 32, 33 and 64 rows take 290, 353 and 360 us in training.)
     if (most_rows <= 16)
         L.row_tile = 16;
     else if (most_rows <= 32)

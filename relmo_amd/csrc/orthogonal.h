@@ -24,9 +24,11 @@ struct OrthoMatrix {
 constexpr int kOrthoBatch = 28;
 constexpr int kNormParts = 256;  // partial sums of squares of a matrix: a wave adds them
 // Tiles of 128 x 128 from which on they are taken instead of 64 x 64 ones: of the symmetric
-// products, of the update.  Symmetric: 2048 x 2048 (136 tiles) takes 855 us with large ones,
-// 1018 with small.  Update: 2048 x 2048 (256 tiles) 836 us with large ones, 941 with small,
-// 1500 x 2600 (252) 661 and 732.  The thresholds between measured counts are not tuned.
+// products, of the update.  A call's us with large ones and with small, in a loop.  Symmetric:
+// 1200 x 1200 (55 tiles) 461 and 284, 1500 x 1500 (78) 596 and 528, 1700 x 1700 (105) 631 and 602, 1800 x
+// 1800 (120) 708 and 690, 2048 x 2048 (136) 742 and 897.  Update: 1200 x 1200 (100) 330 and 283, 2048 x
+// 1024 (128) 322 and 293, 1450 x 1600 (156) 492 and 511, 1500 x 2600 (252) 627 and 712, 2048 x 2048
+// (256) 742 and 851.  (Both thresholds lie some 25 tiles too low.)
 constexpr int64_t kLargeTiles[2] = {100, 128};
 
 struct OrthoRule {

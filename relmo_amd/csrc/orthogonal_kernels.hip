@@ -3,7 +3,9 @@
 //   A = X X^T,   B = b A + c A A,   X <- a X + B X
 //
 // on the shorter side (a taller G is read and written transposed), which drives the
-// singular values towards 1 and keeps the singular vectors.
+// singular values towards 1 and keeps the singular vectors.  The iteration is Schulz's (1933);
+// the quintic with the facade's default coefficients was published with the optimiser
+// Muon (Jordan and others, 2024).
 //
 // Arithmetic.  The iteration multiplies small singular values by about a per step, and the
 // rounding of what it multiplies with them, so 11 or 8 bits are too few for the iterates.
@@ -336,7 +338,7 @@ __device__ __forceinline__ Planes planes_a(void* ws, const OrthoMatrix& d) { ret
 __device__ __forceinline__ Planes planes_b(void* ws, const OrthoMatrix& d) { return planes(ws, d.b, d.m, d.mp); }
 
 // X and its transpose as pairs, 32 x 32 entries to a workgroup; the padding of every plane.
-// Bound by memory and the launch: 2048 x 2048 floats 14.7 us.
+// Bound by memory and the launch: 2048 x 2048 floats 14 us.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_ortho_split(OrthoBatch batch, OrthoRule rule, void* ws) {
     __shared__ float tile[32][33];
@@ -401,8 +403,9 @@ enum Product { kGram, kSquare, kUpdate };
 // fragments come from LDS, the one after it goes from registers to LDS and the third is on
 // its way from memory: one barrier a stage.  Bound by the matrix instructions: a wave of the
 // 128-tile runs 48 of them (768 cycles) a stage beside 16 LDS reads and 8 writes of 1 KB.
-// 2048 x 2048: the 136 lower tiles 50 us (matrix instructions are busy for 48% of the
-// waves' cycles), the update's 256 tiles 67 us; as 528 tiles of 64 x 64 the lower ones take 68.
+// 2048 x 2048, per launch under the profiler: the 136 lower tiles 45 to 49 us (matrix instructions
+// are busy for 48% of the waves' cycles), the update's 256 tiles 64 us; as 528 tiles of 64 x 64 the
+// lower ones take 68.
 template <typename T, int PRODUCT, int BT>
 __global__ __launch_bounds__(kThreads, 2) void k_ortho_product(OrthoBatch batch, OrthoRule rule, int count, int step, void* ws) {
     constexpr int MT = BT / 32;

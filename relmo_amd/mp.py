@@ -214,7 +214,8 @@ def add_rms_norm(
     ``x`` and ``residual`` [..., width] and ``weight`` [width] share a dtype (float32,
     bfloat16 or float16 on the GPU).  The sum and its statistics are float32, rounded once
     as each output is stored; the norm is that of the unrounded sum.  ``residual=None``
-    leaves the addition out (``h`` is ``x``).  No counterpart in relmo."""
+    leaves the addition out (``h`` is ``x``).  On the GPU reverse mode once: second and
+    forward-mode derivatives raise.  No counterpart in relmo."""
 
     require_torch("add_rms_norm")
     return _readout.add_rms_norm(x, residual, weight, float(eps))
@@ -278,7 +279,8 @@ def cross_attention(
     left out: whatever they hold, NaN included, does not enter.  A query without a key to
     attend to gets zeros.  ``scale`` (default ``head_dim ** -0.5``) is positive.  Scores,
     softmax statistics and sums are float32; the gradients of shared key heads add up over
-    their query heads, in a fixed order.  No counterpart in relmo."""
+    their query heads, in a fixed order.  On the GPU reverse mode once: second and forward-mode
+    derivatives raise.  No counterpart in relmo."""
 
     require_torch("cross_attention")
     return _readout.cross_attention(q, k, v, plan, key_mask, scale)
@@ -298,8 +300,8 @@ def orthogonalise(
     ``updates`` is one tensor or a list of them, as all of a model's (few launches for all
     together); each a matrix or a stack of matrices, of one dtype (float32, bfloat16 or
     float16 on the GPU).  Iterates are held in 22 bits and sums in float32 whatever the
-    dtype.  The polynomial must keep [0, 1] within [-2, 2].  No gradient.  No counterpart
-    in relmo."""
+    dtype.  The polynomial must keep [0, 1] within [-2, 2] over the steps (1 to 64).  No
+    gradient.  No counterpart in relmo."""
 
     require_torch("orthogonalise")
     return _readout.orthogonalise(updates, steps, coefficients, eps)
